@@ -1,0 +1,427 @@
+// Layer norm over the last dimension, forward and backward, and the same with
+// the input kept as an 8-bit checkpoint (include/gmdn_lm.h).
+//
+// A row x of d values:  m = mean(x),  r = 1 / sqrt(mean((x - m)^2) + eps),
+// xh = (x - m) r,  y = xh w + b.  With g = dy w:
+//   dx = r (g - mean(g) - xh mean(g xh)),   dw = sum dy xh,  db = sum dy
+// over the rows.
+#include "../../include/gmdn_lm.h"
+#include <type_traits>
+#include "rows8.h"
+
+namespace gmdn {
+namespace {
+
+constexpr int LN_THREADS = 256;      // threads of a workgroup, or a row's if more
+constexpr int LN_MAX_D = 16384;
+constexpr int LN_MAX_BLOCKS = 1024;  // workgroups of the backward (partial sums)
+
+constexpr int ln_threads(int tpr) { return tpr > LN_THREADS ? tpr : LN_THREADS; }
+
+// Sum over the TPR threads of a row: butterflies within a wave, then the
+// row's waves through LDS.  `slot` alternates between two halves of red, so
+// that one barrier a sum is enough.
+template <int TPR>
+GMDN_DEV float row_sum(float x, float (*red)[16], int& slot) {
+  x = lanes_sum<(TPR < 64 ? TPR : 64)>(x);
+  if constexpr (TPR > 64) {
+    constexpr int W = TPR / 64;
+    const int w = wave_id(), first = w / W * W;
+    if (lane_id() == 0) red[slot][w] = x;
+    __syncthreads();
+    x = red[slot][first];
+#pragma unroll
+    for (int i = 1; i < W; ++i) x += red[slot][first + i];
+    slot ^= 1;
+  }
+  return x;
+}
+
+// A row is TPR threads with NV pieces each, piece i of thread t at
+// i TPR + t; a workgroup takes its threads / TPR rows at a time.
+template <typename TX, typename TY, int TPR, int NV, bool PACK>
+__global__ void __launch_bounds__(ln_threads(TPR))
+ln_fwd(const TX* __restrict__ x, const void* __restrict__ w, const void* __restrict__ b, bool w16,
+       TY* __restrict__ y, float* __restrict__ mean, float* __restrict__ rstd, int8_t* __restrict__ q,
+       float* __restrict__ scale, int64_t rows, int d, int64_t xs, float eps) {
+  constexpr int RPB = ln_threads(TPR) / TPR;
+  __shared__ float red[2][16];
+  const int lr = threadIdx.x / TPR, t = threadIdx.x % TPR;
+  int slot = 0;
+  float wv[NV][8], bv[NV][8];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = 8 * (i * TPR + t);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      wv[i][j] = 1.f;
+      bv[i][j] = 0.f;
+    }
+    if (c < d && w) load8_weight(w, w16, c, d - c, wv[i]);
+    if (c < d && b) load8_weight(b, w16, c, d - c, bv[i]);
+  }
+  for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < rows; r0 += (int64_t)gridDim.x * RPB) {
+    const int64_t r = r0 + lr;
+    const bool live = r < rows;
+    float v[NV][8];
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = 8 * (i * TPR + t);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
+      if (live && c < d) load8(x + r * xs + c, d - c, v[i]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s += v[i][j];
+    }
+    const float m = row_sum<TPR>(s, red, slot) / (float)d;
+    float ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = 8 * (i * TPR + t);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float u = c + j < d ? v[i][j] - m : 0.f;
+        ss += u * u;
+      }
+    }
+    const float rs = 1.f / sqrtf(row_sum<TPR>(ss, red, slot) / (float)d + eps);
+    if constexpr (PACK) {
+      constexpr int GL = TPR < GROUP8_PIECES ? TPR : GROUP8_PIECES;  // lanes of a group
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int c = 8 * (i * TPR + t);
+        const Scale8 sc = scale8(lanes_max<GL>(amax_bits(v[i])));
+        if (live && c < d) {
+          store_q8(q + r * d + c, d - c, quant8(v[i], sc.inverse));
+          if (t % GL == 0) scale[r * groups8(d) + c / GROUP8] = sc.scale;
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = 8 * (i * TPR + t);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[i][j] = (v[i][j] - m) * rs * wv[i][j] + bv[i][j];
+      if (live && c < d) store8(y + r * d + c, d - c, v[i]);
+    }
+    if (live && t == 0) {
+      mean[r] = m;
+      rstd[r] = rs;
+    }
+  }
+}
+
+// Where the backward's input comes from: x itself, or its checkpoint.
+template <typename TX>
+struct FromX {
+  const TX* x;
+  int64_t stride;
+  GMDN_DEV void load(int64_t r, int c, int d, float (&v)[8]) const { load8(x + r * stride + c, d - c, v); }
+};
+struct From8 {
+  const int8_t* q;
+  const float* scale;
+  GMDN_DEV void load(int64_t r, int c, int d, float (&v)[8]) const {
+    dequant8(load_q8(q + r * d + c, d - c), scale[r * groups8(d) + c / GROUP8], v);
+  }
+};
+
+// dx, and per workgroup the sums of dy xh and dy over its rows: part is
+// (workgroups, 2, d).  A thread's columns are the same in every row, so the
+// sums stay in its registers; the rows a workgroup takes side by side are
+// added in LDS at the end, in a fixed order.
+template <typename Src, typename TX, typename TY, int TPR, int NV>
+__global__ void __launch_bounds__(ln_threads(TPR))
+ln_bwd(Src src, const TY* __restrict__ dy, int64_t ds, const void* __restrict__ w, bool w16,
+       const float* __restrict__ mean, const float* __restrict__ rstd, TX* __restrict__ dx,
+       float* __restrict__ part, int64_t rows, int d) {
+  constexpr int RPB = ln_threads(TPR) / TPR;
+  __shared__ float red[2][16];
+  const int lr = threadIdx.x / TPR, t = threadIdx.x % TPR;
+  int slot = 0;
+  float wv[NV][8], dw[NV][8], db[NV][8];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = 8 * (i * TPR + t);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      wv[i][j] = 1.f;
+      dw[i][j] = db[i][j] = 0.f;
+    }
+    if (c < d && w) load8_weight(w, w16, c, d - c, wv[i]);
+  }
+  for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < rows; r0 += (int64_t)gridDim.x * RPB) {
+    const int64_t r = r0 + lr;
+    const bool live = r < rows;
+    float v[NV][8], g[NV][8];
+    const float m = live ? mean[r] : 0.f, rs = live ? rstd[r] : 0.f;
+    float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = 8 * (i * TPR + t);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[i][j] = g[i][j] = 0.f;
+      if (live && c < d) {
+        src.load(r, c, d, v[i]);
+        load8(dy + r * ds + c, d - c, g[i]);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        v[i][j] = (v[i][j] - m) * rs;  // xh; a dead lane's g is 0
+        dw[i][j] += g[i][j] * v[i][j];
+        db[i][j] += g[i][j];
+        g[i][j] *= wv[i][j];
+        s0 += g[i][j];
+        s1 += g[i][j] * v[i][j];
+      }
+    }
+    const float mg = row_sum<TPR>(s0, red, slot) / (float)d;
+    const float mx = row_sum<TPR>(s1, red, slot) / (float)d;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = 8 * (i * TPR + t);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) g[i][j] = rs * (g[i][j] - mg - v[i][j] * mx);
+      if (live && c < d) store8(dx + r * d + c, d - c, g[i]);
+    }
+  }
+  if (!w) return;
+  float* out = part + (int64_t)blockIdx.x * 2 * d;
+  if constexpr (RPB == 1) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = 8 * (i * TPR + t);
+      if (c < d) {
+        store8(out + c, d - c, dw[i]);
+        store8(out + d + c, d - c, db[i]);
+      }
+    }
+  } else {
+    __shared__ float sums[RPB][TPR * NV * 8];
+    for (int which = 0; which < 2; ++which) {
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sums[lr][8 * (i * TPR + t) + j] = which ? db[i][j] : dw[i][j];
+      __syncthreads();
+      for (int c = threadIdx.x; c < d; c += ln_threads(TPR)) {
+        float s = sums[0][c];
+#pragma unroll
+        for (int i = 1; i < RPB; ++i) s += sums[i][c];
+        out[which * d + c] = s;
+      }
+    }
+  }
+}
+
+// dweight and dbias from the workgroups' sums, one column of (2, d) a lane
+// group: a workgroup takes 32 columns, 8 threads each with every 8th partial
+// row; added in a fixed order, the same bits on every run.
+constexpr int LN_COLS = 32;
+constexpr int LN_SPLIT = LN_THREADS / LN_COLS;
+__global__ void __launch_bounds__(LN_THREADS)
+ln_sums(const float* __restrict__ part, void* __restrict__ dw, void* __restrict__ db, bool w16, int d, int nblk) {
+  __shared__ float red[LN_SPLIT][LN_COLS];
+  const int cl = threadIdx.x % LN_COLS, sp = threadIdx.x / LN_COLS;
+  const int c = blockIdx.x * LN_COLS + cl;
+  float a0 = 0.f, a1 = 0.f, a2 = 0.f, a3 = 0.f;
+  if (c < 2 * d) {
+    int i = sp;
+    for (; i + 3 * LN_SPLIT < nblk; i += 4 * LN_SPLIT) {
+      a0 += part[(int64_t)i * 2 * d + c];
+      a1 += part[(int64_t)(i + LN_SPLIT) * 2 * d + c];
+      a2 += part[(int64_t)(i + 2 * LN_SPLIT) * 2 * d + c];
+      a3 += part[(int64_t)(i + 3 * LN_SPLIT) * 2 * d + c];
+    }
+    for (; i < nblk; i += LN_SPLIT) a0 += part[(int64_t)i * 2 * d + c];
+  }
+  red[sp][cl] = (a0 + a1) + (a2 + a3);
+  __syncthreads();
+  if (sp == 0 && c < 2 * d) {
+    float s = red[0][cl];
+#pragma unroll
+    for (int i = 1; i < LN_SPLIT; ++i) s += red[i][cl];
+    void* out = c < d ? dw : db;
+    const int at = c < d ? c : c - d;
+    if (w16)
+      reinterpret_cast<bf16*>(out)[at] = (bf16)s;
+    else
+      reinterpret_cast<float*>(out)[at] = s;
+  }
+}
+
+// y again from the checkpoint and the saved statistics; one piece a thread.
+template <typename TY>
+__global__ void __launch_bounds__(256)
+ln_rebuild(From8 src, const void* __restrict__ w, const void* __restrict__ b, bool w16,
+           const float* __restrict__ mean, const float* __restrict__ rstd, TY* __restrict__ y, int64_t rows, int d) {
+  const int pieces = (d + 7) / 8;
+  const int64_t total = rows * pieces;
+  for (int64_t p = (int64_t)blockIdx.x * 256 + threadIdx.x; p < total; p += (int64_t)gridDim.x * 256) {
+    const int64_t r = p / pieces;
+    const int c = 8 * (int)(p - r * pieces);
+    float v[8], wv[8], bv[8];
+    src.load(r, c, d, v);
+    const float m = mean[r], rs = rstd[r];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      wv[j] = 1.f;
+      bv[j] = 0.f;
+    }
+    if (w) load8_weight(w, w16, c, d - c, wv);
+    if (b) load8_weight(b, w16, c, d - c, bv);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = (v[j] - m) * rs * wv[j] + bv[j];
+    store8(y + r * d + c, d - c, v);
+  }
+}
+
+template <int TPR_, int NV_>
+struct Shape {
+  static constexpr int TPR = TPR_, NV = NV_;
+};
+// f(Shape) with the threads and pieces of a row of d values: one piece a
+// thread while the row fits a wave, then two.
+template <class F>
+void with_shape(int64_t d, F&& f) {
+  if (d <= 64) f(Shape<8, 1>{});
+  else if (d <= 128) f(Shape<16, 1>{});
+  else if (d <= 256) f(Shape<32, 1>{});
+  else if (d <= 512) f(Shape<64, 1>{});
+  else if (d <= 1024) f(Shape<64, 2>{});
+  else if (d <= 2048) f(Shape<128, 2>{});
+  else if (d <= 4096) f(Shape<256, 2>{});
+  else if (d <= 8192) f(Shape<512, 2>{});
+  else f(Shape<1024, 2>{});
+}
+
+int64_t ln_blocks(int64_t rows, int64_t d) {
+  int64_t n = 0;
+  with_shape(d, [&](auto s) {
+    using S = decltype(s);
+    constexpr int RPB = ln_threads(S::TPR) / S::TPR;
+    n = (rows + RPB - 1) / RPB;
+  });
+  return n < LN_MAX_BLOCKS ? n : LN_MAX_BLOCKS;
+}
+
+// The built pairs of types: (bf16, bf16), (float32, float32) and a float32
+// input beside a bf16 output.
+bool pair_ok(int32_t xt, int32_t yt) {
+  return type_ok(xt) && type_ok(yt) && !(xt == GMDN_DTYPE_BF16 && yt == GMDN_DTYPE_F32);
+}
+template <class F>
+void with_types(int32_t xt, int32_t yt, F&& f) {
+  if (xt == GMDN_DTYPE_BF16) f(bf16{}, bf16{});
+  else if (yt == GMDN_DTYPE_F32) f(float{}, float{});
+  else f(float{}, bf16{});
+}
+
+int check_dims(int64_t rows, int64_t d) {
+  if (rows < 0 || d <= 0 || rows > ((int64_t)1 << 40)) return GMDN_ERR_ARG;
+  return d > LN_MAX_D ? GMDN_ERR_UNSUPPORTED : GMDN_OK;
+}
+
+}  // namespace
+}  // namespace gmdn
+
+using namespace gmdn;
+
+extern "C" {
+
+int gmdn_layer_norm_fwd(const void* x, const void* weight, const void* bias, void* y, float* mean, float* rstd,
+                        int8_t* q, float* scale, int64_t rows, int64_t d, int64_t x_stride, float eps,
+                        int32_t x_type, int32_t y_type, int32_t w_type, void* stream) {
+  const int rc = check_dims(rows, d);
+  if (rc != GMDN_OK) return rc;
+  if (!pair_ok(x_type, y_type) || !type_ok(w_type)) return GMDN_ERR_UNSUPPORTED;
+  if (!(eps >= 0.f) || x_stride < 0 || (bias && !weight) || !q != !scale) return GMDN_ERR_ARG;
+  if (rows == 0) return GMDN_OK;
+  if (!x || !y || !mean || !rstd) return GMDN_ERR_ARG;
+  const dim3 grid((unsigned)ln_blocks(rows, d));
+  const bool w16 = w_type == GMDN_DTYPE_BF16;
+  with_types(x_type, y_type, [&](auto tx, auto ty) {
+    using TX = decltype(tx);
+    using TY = decltype(ty);
+    with_shape(d, [&](auto s) {
+      using S = decltype(s);
+      const dim3 block(ln_threads(S::TPR));
+      if (q)
+        hipLaunchKernelGGL((ln_fwd<TX, TY, S::TPR, S::NV, true>), grid, block, 0, (hipStream_t)stream, (const TX*)x,
+                           weight, bias, w16, (TY*)y, mean, rstd, q, scale, rows, (int)d, x_stride, eps);
+      else
+        hipLaunchKernelGGL((ln_fwd<TX, TY, S::TPR, S::NV, false>), grid, block, 0, (hipStream_t)stream, (const TX*)x,
+                           weight, bias, w16, (TY*)y, mean, rstd, q, scale, rows, (int)d, x_stride, eps);
+    });
+  });
+  return launched();
+}
+
+size_t gmdn_layer_norm_bwd_workspace_floats(int64_t rows, int64_t d) {
+  if (rows <= 0 || check_dims(rows, d) != GMDN_OK) return 0;
+  return (size_t)(ln_blocks(rows, d) * 2 * d);
+}
+
+int gmdn_layer_norm_bwd(const void* dy, const void* x, const int8_t* q, const float* scale, const void* weight,
+                        const float* mean, const float* rstd, void* dx, void* dweight, void* dbias, float* workspace,
+                        size_t workspace_floats, int64_t rows, int64_t d, int64_t dy_stride, int64_t x_stride,
+                        int32_t x_type, int32_t y_type, int32_t w_type, void* stream) {
+  const int rc = check_dims(rows, d);
+  if (rc != GMDN_OK) return rc;
+  if (!pair_ok(x_type, y_type) || !type_ok(w_type)) return GMDN_ERR_UNSUPPORTED;
+  if (dy_stride < 0 || x_stride < 0 || !q != !scale) return GMDN_ERR_ARG;
+  if (weight && (!dweight || !dbias)) return GMDN_ERR_ARG;
+  const bool w16 = w_type == GMDN_DTYPE_BF16;
+  const hipStream_t st = (hipStream_t)stream;
+  int64_t nb = 0;
+  if (rows > 0) {
+    if (!dy || (!x && !q) || (x && q) || !mean || !rstd || !dx) return GMDN_ERR_ARG;
+    nb = ln_blocks(rows, d);
+    if (weight && (!workspace || workspace_floats < (size_t)(nb * 2 * d))) return GMDN_ERR_WORKSPACE;
+    with_types(x_type, y_type, [&](auto tx, auto ty) {
+      using TX = decltype(tx);
+      using TY = decltype(ty);
+      with_shape(d, [&](auto s) {
+        using S = decltype(s);
+        const dim3 grid((unsigned)nb), block(ln_threads(S::TPR));
+        if (q)
+          hipLaunchKernelGGL((ln_bwd<From8, TX, TY, S::TPR, S::NV>), grid, block, 0, st, From8{q, scale},
+                             (const TY*)dy, dy_stride, weight, w16, mean, rstd, (TX*)dx, workspace, rows, (int)d);
+        else
+          hipLaunchKernelGGL((ln_bwd<FromX<TX>, TX, TY, S::TPR, S::NV>), grid, block, 0, st,
+                             FromX<TX>{(const TX*)x, x_stride}, (const TY*)dy, dy_stride, weight, w16, mean, rstd,
+                             (TX*)dx, workspace, rows, (int)d);
+      });
+    });
+    if (hipGetLastError() != hipSuccess) return GMDN_ERR_LAUNCH;
+  }
+  if (!weight) return GMDN_OK;
+  hipLaunchKernelGGL(ln_sums, dim3((unsigned)((2 * d + LN_COLS - 1) / LN_COLS)), dim3(LN_THREADS), 0, st, workspace,
+                     dweight, dbias, w16, (int)d, (int)nb);
+  return launched();
+}
+
+int gmdn_layer_norm8_rebuild(const int8_t* q, const float* scale, const void* weight, const void* bias,
+                             const float* mean, const float* rstd, void* y, int64_t rows, int64_t d, int32_t y_type,
+                             int32_t w_type, void* stream) {
+  const int rc = check_dims(rows, d);
+  if (rc != GMDN_OK) return rc;
+  if (!type_ok(y_type) || !type_ok(w_type)) return GMDN_ERR_UNSUPPORTED;
+  if (bias && !weight) return GMDN_ERR_ARG;
+  if (rows == 0) return GMDN_OK;
+  if (!q || !scale || !mean || !rstd || !y) return GMDN_ERR_ARG;
+  const int64_t blocks = (rows * ((d + 7) / 8) + 255) / 256;
+  const dim3 grid((unsigned)(blocks < (1 << 20) ? blocks : (1 << 20)));
+  const bool w16 = w_type == GMDN_DTYPE_BF16;
+  if (y_type == GMDN_DTYPE_BF16)
+    hipLaunchKernelGGL(ln_rebuild<bf16>, grid, dim3(256), 0, (hipStream_t)stream, From8{q, scale}, weight, bias, w16,
+                       mean, rstd, (bf16*)y, rows, (int)d);
+  else
+    hipLaunchKernelGGL(ln_rebuild<float>, grid, dim3(256), 0, (hipStream_t)stream, From8{q, scale}, weight, bias, w16,
+                       mean, rstd, (float*)y, rows, (int)d);
+  return launched();
+}
+
+}  // extern "C"

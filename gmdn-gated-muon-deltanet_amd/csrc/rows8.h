@@ -1,0 +1,183 @@
+// Rows of values in pieces of eight, for the kernels that stream (rows, d)
+// matrices: loads and stores of a piece at any alignment, sums and maxima
+// over the threads of a row, and the 8-bit checkpoint format.
+//
+// A piece is 8 consecutive values of a row (16 bytes of bf16, 32 of float32).
+// Rows of odd widths start at any element, so the vector types below promise
+// element alignment only; gfx950 loads and stores them by one instruction all
+// the same (measured at 16384 x 1001 beside 16384 x 1024).  Only the short
+// last piece of a row is read and written by elements.
+#pragma once
+#include "../../include/gmdn_scan.h"
+#include "tile.h"
+
+namespace gmdn {
+
+typedef bf16 bf16x8_any __attribute__((ext_vector_type(8), aligned(2)));
+typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(1)));
+
+// Piece of n >= 1 values at p; values from n on are `pad`.
+GMDN_DEV void load8(const bf16* p, int n, float (&x)[8], float pad = 0.f) {
+  if (n >= 8) {
+    const bf16x8_any v = *reinterpret_cast<const bf16x8_any*>(p);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = (float)v[j];
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = j < n ? (float)p[j] : pad;
+  }
+}
+GMDN_DEV void load8(const float* p, int n, float (&x)[8], float pad = 0.f) {
+  if (n >= 8) {
+    const f32x4_any a = *reinterpret_cast<const f32x4_any*>(p), b = *reinterpret_cast<const f32x4_any*>(p + 4);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      x[j] = a[j];
+      x[4 + j] = b[j];
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = j < n ? p[j] : pad;
+  }
+}
+GMDN_DEV void store8(bf16* p, int n, const float (&x)[8]) {
+  const bf16x8 v = cat8(to_bf16x4(f32x4{x[0], x[1], x[2], x[3]}), to_bf16x4(f32x4{x[4], x[5], x[6], x[7]}));
+  if (n >= 8) {
+    *reinterpret_cast<bf16x8_any*>(p) = v;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j < n) p[j] = v[j];
+  }
+}
+GMDN_DEV void store8(float* p, int n, const float (&x)[8]) {
+  if (n >= 8) {
+    *reinterpret_cast<f32x4_any*>(p) = f32x4{x[0], x[1], x[2], x[3]};
+    *reinterpret_cast<f32x4_any*>(p + 4) = f32x4{x[4], x[5], x[6], x[7]};
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j < n) p[j] = x[j];
+  }
+}
+// Values of a weight vector held in float32 or bf16 (is_bf16).
+GMDN_DEV void load8_weight(const void* w, bool is_bf16, int at, int n, float (&x)[8]) {
+  if (is_bf16)
+    load8(reinterpret_cast<const bf16*>(w) + at, n, x);
+  else
+    load8(reinterpret_cast<const float*>(w) + at, n, x);
+}
+
+// ------------------------------------------------- the 8-bit checkpoint
+// Groups of 128 consecutive values of a row (the last one may be short).
+// With amax the group's largest magnitude:
+//   scale = amax * STEP8     q = rint(x * (127 / amax))     x' = q * scale
+// in float32, each operation rounded by itself (no contraction), so that any
+// float32 evaluation gives the same bytes.  STEP8 is the float32 below
+// 1 / 127: 127 * scale does not exceed amax, so that x' is finite wherever x
+// is, up to the type's largest value.  A group whose amax is below 2^-100
+// is kept as zeros; one that holds an infinity or a NaN reads back as NaN
+// (scale NaN).  |x' - x| <= amax / 254 up to rounding.
+constexpr int GROUP8 = 128;
+constexpr int GROUP8_PIECES = GROUP8 / 8;
+constexpr float STEP8 = 0x1.020406p-7f;
+constexpr uint32_t TINY8 = 0x0d800000u;  // bits of 2^-100
+constexpr uint32_t INF_BITS = 0x7f800000u;
+
+inline __host__ __device__ int64_t groups8(int64_t d) { return (d + GROUP8 - 1) / GROUP8; }
+
+// Largest magnitude of a piece, as bits: their order is that of the values,
+// with infinity and then NaN at the end.
+GMDN_DEV uint32_t amax_bits(const float (&x)[8]) {
+  uint32_t a = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const uint32_t b = __builtin_bit_cast(uint32_t, x[j]) & 0x7fffffffu;
+    a = b > a ? b : a;
+  }
+  return a;
+}
+
+struct Scale8 {
+  float inverse, scale;
+};
+GMDN_DEV Scale8 scale8(uint32_t amax) {
+#pragma clang fp contract(off)
+  if (amax < TINY8) return {0.f, 0.f};
+  if (amax >= INF_BITS) return {0.f, __builtin_nanf("")};
+  const float a = __builtin_bit_cast(float, amax);
+  return {127.f / a, a * STEP8};
+}
+// The bytes of a piece.  x * inverse is rounded to float32, then to an
+// integer by adding 1.5 * 2^23 (round to nearest even), whose low byte is
+// the integer's; inverse 0 (a group without a scale) gives 0 for every x, as
+// the product may be NaN there.
+GMDN_DEV u32x2_any quant8(const float (&x)[8], float inverse) {
+#pragma clang fp contract(off)
+  uint32_t b[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float t = x[j] * inverse;
+    b[j] = __builtin_bit_cast(uint32_t, t + 12582912.f);
+  }
+  u32x2_any r;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const uint32_t lo = __builtin_amdgcn_perm(b[4 * h + 1], b[4 * h], 0x0c0c0400u);
+    const uint32_t hi = __builtin_amdgcn_perm(b[4 * h + 3], b[4 * h + 2], 0x04000c0cu);
+    r[h] = inverse == 0.f ? 0u : lo | hi;
+  }
+  return r;
+}
+GMDN_DEV void store_q8(int8_t* p, int n, u32x2_any v) {
+  if (n >= 8) {
+    *reinterpret_cast<u32x2_any*>(p) = v;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j < n) p[j] = (int8_t)(v[j / 4] >> (8 * (j % 4)));
+  }
+}
+GMDN_DEV void dequant8(u32x2_any v, float scale, float (&x)[8]) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) x[j] = (float)(int8_t)(v[j / 4] >> (8 * (j % 4))) * scale;
+}
+GMDN_DEV u32x2_any load_q8(const int8_t* p, int n) {
+  if (n >= 8) return *reinterpret_cast<const u32x2_any*>(p);
+  u32x2_any v = {0u, 0u};
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (j < n) v[j / 4] |= (uint32_t)(uint8_t)p[j] << (8 * (j % 4));
+  return v;
+}
+
+// ------------------------------------------------- over the threads of a row
+// Sum over aligned groups of N lanes (N a power of two up to 64).
+template <int N>
+GMDN_DEV float lanes_sum(float x) {
+#pragma unroll
+  for (int o = 1; o < N; o <<= 1) x += __shfl_xor(x, o, 64);
+  return x;
+}
+template <int N>
+GMDN_DEV uint32_t lanes_max(uint32_t x) {
+#pragma unroll
+  for (int o = 1; o < N; o <<= 1) {
+    const uint32_t y = (uint32_t)__shfl_xor((int)x, o, 64);
+    x = y > x ? y : x;
+  }
+  return x;
+}
+template <int N>
+GMDN_DEV float lanes_max(float x) {
+#pragma unroll
+  for (int o = 1; o < N; o <<= 1) x = fmaxf(x, __shfl_xor(x, o, 64));
+  return x;
+}
+
+// Element type codes of the C-ABI.
+inline bool type_ok(int32_t t) { return t == GMDN_DTYPE_BF16 || t == GMDN_DTYPE_F32; }
+inline int launched() { return hipGetLastError() == hipSuccess ? GMDN_OK : GMDN_ERR_LAUNCH; }
+
+}  // namespace gmdn

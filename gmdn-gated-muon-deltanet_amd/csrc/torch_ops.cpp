@@ -16,51 +16,21 @@
 // (moments, checkpoints, 1 / rms) reaches the caller through a pointer, since
 // compiled autograd takes no function with non-differentiable outputs.
 #include "../../include/gmdn_front.h"
-#include "../../include/gmdn_scan.h"
 #include "../../include/gmdn_tail.h"
+#include "torch_ops.h"
 
-#include <ATen/ATen.h>
 #include <algorithm>
 #include <array>
-#include <c10/core/DeviceGuard.h>
-#include <c10/hip/HIPStream.h>
-#include <torch/csrc/autograd/autograd_not_implemented_fallback.h>
-#include <torch/csrc/autograd/custom_function.h>
-#include <torch/library.h>
-
 #include <atomic>
-#include <optional>
-#include <tuple>
-#include <type_traits>
-#include <vector>
 
 namespace {
 
-using at::Tensor;
-using OptTensor = std::optional<Tensor>;
-using torch::autograd::AutogradContext;
-using torch::autograd::variable_list;
+using namespace gmdn_ops;
 constexpr int64_t CHUNK = 64;
 
 // The process's product precision (gmdn_amd.scan.set_precision), read by the
 // muon core's backward.
 std::atomic<int64_t> default_precision{GMDN_PREC_TF32};
-
-void check(int rc, const char* what) {
-  TORCH_CHECK(rc == GMDN_OK, what, " failed with code ", rc, ": ", gmdn_error_string(rc));
-}
-void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
-float* fp(const Tensor& t) { return t.numel() ? t.data_ptr<float>() : nullptr; }
-const float* fp(const OptTensor& t) { return t ? t->data_ptr<float>() : nullptr; }
-Tensor f32_empty(const Tensor& like, at::IntArrayRef size) { return at::empty(size, like.options().dtype(at::kFloat)); }
-Tensor none_of(const Tensor& like) { return f32_empty(like, {0}); }
-Tensor bytes_of(const Tensor& like, size_t n) {
-  return at::empty({(int64_t)n}, like.options().dtype(at::kByte));
-}
-
-void check_rank(const Tensor& t, int64_t rank, const char* what) {
-  TORCH_CHECK(t.dim() == rank, what, " must have ", rank, " dimensions, got shape ", t.sizes());
-}
 
 // ------------------------------------------------------------ token streams
 void check_tokens(const Tensor& q, const Tensor& k, const Tensor& v) {
@@ -369,31 +339,6 @@ std::tuple<Tensor, Tensor> head_norm_bwd(const Tensor& x, const Tensor& weight, 
 }
 
 // ------------------------------------------------------------------ autograd
-// Calls through the dispatcher, below autograd.
-template <class F>
-auto op(const char* name) {
-  return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<F>();
-}
-// A kernel's signature with symbolic integers: a traced size reaches the
-// schema unspecialised, and only the kernels themselves see plain integers.
-template <class F>
-struct Symbolic;
-template <class R, class... A>
-struct Symbolic<R(A...)> {
-  using T = R(std::conditional_t<std::is_same_v<A, int64_t>, c10::SymInt, A>...);
-};
-#define GMDN_OP(fn) \
-  ([]() -> const auto& { static const auto h = op<Symbolic<decltype(fn)>::T>("gmdn::" #fn); return h; }())
-
-bool wants_grad(std::initializer_list<const Tensor*> ts) {
-  if (!at::GradMode::is_enabled()) return false;
-  for (const Tensor* t : ts)
-    if (t->defined() && t->requires_grad()) return true;
-  return false;
-}
-Tensor opt(const OptTensor& t) { return t ? *t : Tensor(); }
-OptTensor opt(const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
-
 struct StateScan : torch::autograd::Function<StateScan> {
   static constexpr bool is_traceable = true;
   static Tensor forward(AutogradContext* ctx, const Tensor& U, const Tensor& K, const Tensor& a, const Tensor& b,

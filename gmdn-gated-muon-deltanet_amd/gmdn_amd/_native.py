@@ -1,5 +1,6 @@
 """ctypes binding of ``libgmdn_scan.so`` (the C ABI declared in include/gmdn_scan.h,
-include/gmdn_front.h, include/gmdn_tail.h and include/gmdn_msign.h).
+include/gmdn_front.h, include/gmdn_tail.h, include/gmdn_msign.h and
+include/gmdn_lm.h).
 
 The libraries (it, and ``libgmdn_ops.so`` with the torch operators over it) are
 built in-tree by ``gmdn_amd.build`` and loaded after torch, so
@@ -76,6 +77,18 @@ SIGNATURES = {
     # include/gmdn_msign.h
     "gmdn_msign_workspace_bytes": (c_size, [c_i64, c_i64, c_i64]),
     "gmdn_msign": (c_i32, [c_vp, c_vp, c_i64, c_i64, c_i64, c_i32, ctypes.c_float, c_i32, c_vp, c_size, c_vp]),
+    # include/gmdn_lm.h
+    "gmdn_layer_norm_fwd": (c_i32, [c_vp] * 8 + [c_i64] * 3 + [ctypes.c_float] + [c_i32] * 3 + [c_vp]),
+    "gmdn_layer_norm_bwd_workspace_floats": (c_size, [c_i64, c_i64]),
+    "gmdn_layer_norm_bwd": (c_i32, [c_vp] * 11 + [c_size] + [c_i64] * 4 + [c_i32] * 3 + [c_vp]),
+    "gmdn_layer_norm8_rebuild": (c_i32, [c_vp] * 7 + [c_i64] * 2 + [c_i32] * 2 + [c_vp]),
+    "gmdn_act8_groups": (c_i64, [c_i64]),
+    "gmdn_act8_pack": (c_i32, [c_vp] * 3 + [c_i64] * 3 + [c_i32, c_vp]),
+    "gmdn_act8_unpack": (c_i32, [c_vp] * 3 + [c_i64] * 2 + [c_i32, c_vp]),
+    "gmdn_gelu8_fwd": (c_i32, [c_vp] * 4 + [c_i64] * 3 + [c_i32, c_vp]),
+    "gmdn_gelu8_bwd": (c_i32, [c_vp] * 5 + [c_i64] * 3 + [c_i32, c_vp]),
+    "gmdn_logprobs_fwd": (c_i32, [c_vp] * 7 + [c_i64] * 3 + [c_i32, c_i64, c_i32, c_vp]),
+    "gmdn_logprobs_bwd": (c_i32, [c_vp] * 9 + [c_i64] * 3 + [c_i32, c_i64, c_i32, c_vp]),
 }
 
 

@@ -1,7 +1,7 @@
 """``torch.ops.gmdn.*``: the C-ABI entry points as registered torch operators.
 
 Each operator wraps one call of ``libgmdn_scan.so`` (include/gmdn_scan.h) on
-the tensors' current stream.  All but ``msign`` are C++ (csrc/torch_ops.cpp,
+the tensors' current stream.  All but ``msign`` are C++ (csrc/torch_ops*.cpp,
 ``libgmdn_ops.so``), with autograd on the forward operators; this module
 registers their shape-only fake implementations, so that ``torch.compile``
 traces through the scan without a graph break (the reference trainer compiles
@@ -26,6 +26,21 @@ its model, train_ablation.py:420-422):
   ``gmdn::head_norm_bwd`` -- the per-head RMSNorm of the output (:188).
 * ``gmdn::chunk_bwd_muon`` -- the muon core's backward.
 * ``gmdn::wy_fwd`` / ``gmdn::wy_bwd`` -- the token-exact mode (gmdn_amd.wy).
+* ``gmdn::layer_norm_fwd(x, weight, bias, eps, dtype, pack) -> (y, mean, rstd,
+  q, scale)`` -- layer norm with an output of ``dtype``; ``pack`` keeps ``x``
+  as an 8-bit checkpoint ``q``, ``scale`` (else empty), and the backward runs
+  from it.  ``gmdn::layer_norm_bwd(dy, x, weight, mean, rstd)`` and
+  ``gmdn::layer_norm8_bwd(dy, q, scale, weight, mean, rstd, dtype) -> (dx,
+  dweight, dbias)``; ``gmdn::layer_norm8_rebuild(q, scale, weight, bias, mean,
+  rstd, dtype) -> y`` (gmdn_amd.layer_norm).
+* ``gmdn::act8_pack(x) -> (q, scale)``, ``gmdn::act8_unpack(q, scale, dtype)
+  -> x`` -- 8-bit activation checkpoints; ``gmdn::gelu8_fwd(h) -> (a, q,
+  scale)`` and ``gmdn::gelu8_bwd(da, q, scale, with_output) -> (dh, a)`` --
+  GELU that keeps its input in one (gmdn_amd.act8).
+* ``gmdn::logprobs_fwd(logits, tokens, top, ignore_index) -> (logprob, entropy,
+  top_logprobs, top_tokens, stats)`` and ``gmdn::logprobs_bwd(logits, tokens,
+  stats, entropy, top_tokens, dlogprob, dentropy, dtop, ignore_index) ->
+  dlogits`` -- log probabilities of given tokens (gmdn_amd.logprobs).
 * ``gmdn::msign(M, steps, eps) -> X`` -- the outer Muon optimizer's msign of
   a batch of matrices (train_ablation.py:60-73); no autograd (the optimizer
   runs it under ``no_grad``).
@@ -177,6 +192,53 @@ def _head_norm_bwd_fake(x, weight, rstd, dout):
     return torch.empty_like(x, memory_format=torch.contiguous_format), weight.new_empty(weight.shape)
 
 
+def _act8_fakes(x):
+    return (x.new_empty(x.shape, dtype=torch.int8),
+            x.new_empty((*x.shape[:-1], (x.shape[-1] + 127) // 128), dtype=torch.float32))
+
+
+def _layer_norm_fwd_fake(x, weight, bias, eps, dtype, pack):
+    stats = [x.new_empty(x.shape[:-1], dtype=torch.float32) for _ in range(2)]
+    kept = _act8_fakes(x) if pack else (x.new_empty((0,), dtype=torch.int8), _empty(x))
+    return x.new_empty(x.shape, dtype=dtype), *stats, *kept
+
+
+def _layer_norm_bwd_fake(dy, x, weight, mean, rstd):
+    return _layer_norm8_bwd_fake(dy, None, None, weight, mean, rstd, x.dtype)
+
+
+def _layer_norm8_bwd_fake(dy, q, scale, weight, mean, rstd, dtype):
+    dw = [weight.new_empty(weight.shape) if weight is not None else _empty(dy) for _ in range(2)]
+    return dy.new_empty(dy.shape, dtype=dtype), *dw
+
+
+def _layer_norm8_rebuild_fake(q, scale, weight, bias, mean, rstd, dtype):
+    return q.new_empty(q.shape, dtype=dtype)
+
+
+def _act8_unpack_fake(q, scale, dtype):
+    return q.new_empty(q.shape, dtype=dtype)
+
+
+def _gelu8_fwd_fake(h):
+    return h.new_empty(h.shape), *_act8_fakes(h)
+
+
+def _gelu8_bwd_fake(da, q, scale, with_output):
+    return da.new_empty(da.shape), da.new_empty(da.shape if with_output else (0,))
+
+
+def _logprobs_fwd_fake(logits, tokens, top, ignore_index):
+    lead = logits.shape[:-1]
+    return (*(logits.new_empty(lead, dtype=torch.float32) for _ in range(2)),
+            logits.new_empty((*lead, top), dtype=torch.float32), logits.new_empty((*lead, top), dtype=torch.int64),
+            logits.new_empty((*lead, 2), dtype=torch.float32))
+
+
+def _logprobs_bwd_fake(logits, tokens, stats, entropy, top_tokens, dlogprob, dentropy, dtop, ignore_index):
+    return logits.new_empty(logits.shape)
+
+
 _FAKES = {
     "state_scan": _state_scan_fake,
     "state_scan_bwd": _state_scan_bwd_fake,
@@ -191,6 +253,16 @@ _FAKES = {
     "gates_bwd": _gates_bwd_fake,
     "head_norm_fwd": _head_norm_fwd_fake,
     "head_norm_bwd": _head_norm_bwd_fake,
+    "layer_norm_fwd": _layer_norm_fwd_fake,
+    "layer_norm_bwd": _layer_norm_bwd_fake,
+    "layer_norm8_bwd": _layer_norm8_bwd_fake,
+    "layer_norm8_rebuild": _layer_norm8_rebuild_fake,
+    "act8_pack": _act8_fakes,
+    "act8_unpack": _act8_unpack_fake,
+    "gelu8_fwd": _gelu8_fwd_fake,
+    "gelu8_bwd": _gelu8_bwd_fake,
+    "logprobs_fwd": _logprobs_fwd_fake,
+    "logprobs_bwd": _logprobs_bwd_fake,
 }
 # Set by _register_fakes.  Without the native libraries the operators do not
 # exist: every entry point calls ensure(), which raises what _native.load raises.
