@@ -27,8 +27,10 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from . import act8, logprobs
 from . import ops  # registers torch.ops.gmdn.*
 from .chunk import chunk_scan
+from .layer_norm import LayerNorm, checked_checkpoint
 
 
 class FastWeightMixer(nn.Module):
@@ -105,31 +107,63 @@ class FastWeightMixer(nn.Module):
         return self.out(y if bf16_autocast else y.to(x.dtype))
 
 
-class Block(nn.Module):
-    """Pre-norm residual block: mixer, then a 4x GELU MLP (train_ablation.py:197-210)."""
+def _norm(kind: str, dim: int, checkpoint: str | None = None) -> nn.Module:
+    if kind == "rms":
+        return nn.RMSNorm(dim)
+    if kind == "layer":
+        return LayerNorm(dim, checkpoint=checkpoint)
+    raise ValueError(f"norm is 'rms' or 'layer', got {kind!r}")
 
-    def __init__(self, d_model, n_heads, inner, chunk, ns_steps=3):
+
+class Block(nn.Module):
+    """Pre-norm residual block: mixer, then a 4x GELU MLP (train_ablation.py:197-210).
+
+    ``norm="layer"`` takes layer norm (HIP) in place of RMSNorm.
+    ``checkpoint="int8"`` keeps the MLP's activations, and a layer norm's input,
+    for the backward in 8 bits (gmdn_amd.act8); the parameters are the same.
+    """
+
+    def __init__(self, d_model, n_heads, inner, chunk, ns_steps=3, norm="rms", checkpoint=None):
         super().__init__()
-        self.n1 = nn.RMSNorm(d_model)
+        self.keep8 = checked_checkpoint(checkpoint)
+        self.n1 = _norm(norm, d_model, checkpoint)
         self.mixer = FastWeightMixer(d_model, n_heads, inner, chunk, ns_steps)
-        self.n2 = nn.RMSNorm(d_model)
+        self.n2 = _norm(norm, d_model, checkpoint)
         self.mlp = nn.Sequential(nn.Linear(d_model, 4 * d_model, bias=False), nn.GELU(),
                                  nn.Linear(4 * d_model, d_model, bias=False))
 
+    def _mlp(self, x):
+        if not self.keep8:
+            return self.mlp(self.n2(x))
+        w1, w2 = self.mlp[0].weight, self.mlp[2].weight
+        if isinstance(self.n2, LayerNorm):
+            return act8.norm_mlp(x, self.n2.weight, self.n2.bias, w1, w2, self.n2.eps)
+        return act8.mlp(self.n2(x), w1, w2)
+
     def forward(self, x):
         x = x + self.mixer(self.n1(x))
-        return x + self.mlp(self.n2(x))
+        return x + self._mlp(x)
 
 
 class LM(nn.Module):
     """Embedding, blocks, final RMSNorm and a tied head; next-token cross
-    entropy in float32 (train_ablation.py:213-243)."""
+    entropy in float32 (train_ablation.py:213-243).
 
-    def __init__(self, vocab, d_model, n_layers, n_heads, inner, chunk=64, ns_steps=3):
+    ``norm`` and ``checkpoint`` are the blocks'.  ``loss="logprobs"`` takes the
+    same loss from the logits where they are, without their float32 copy
+    (gmdn_amd.logprobs).
+    """
+
+    def __init__(self, vocab, d_model, n_layers, n_heads, inner, chunk=64, ns_steps=3, norm="rms", checkpoint=None,
+                 loss="torch"):
         super().__init__()
+        if loss not in ("torch", "logprobs"):
+            raise ValueError(f"loss is 'torch' or 'logprobs', got {loss!r}")
+        self.loss = loss
         self.emb = nn.Embedding(vocab, d_model)
-        self.blocks = nn.ModuleList(Block(d_model, n_heads, inner, chunk, ns_steps) for _ in range(n_layers))
-        self.norm_f = nn.RMSNorm(d_model)
+        self.blocks = nn.ModuleList(Block(d_model, n_heads, inner, chunk, ns_steps, norm, checkpoint)
+                                    for _ in range(n_layers))
+        self.norm_f = _norm(norm, d_model, checkpoint)
         self.lm_head = nn.Linear(d_model, vocab, bias=False)
         self.lm_head.weight = self.emb.weight  # tied
         self.apply(self._init)
@@ -154,5 +188,16 @@ class LM(nn.Module):
         logits = self.lm_head(self.norm_f(x))
         if targets is None:
             return logits, None
+        if self.loss == "logprobs":
+            return logits, logprobs.cross_entropy(logits, targets)
         loss = F.cross_entropy(logits.view(-1, logits.size(-1)).float(), targets.reshape(-1))
         return logits, loss
+
+    @torch.no_grad()
+    def score(self, idx, tokens=None, top=0):
+        """Log probabilities of ``tokens`` (B, T) -- by default each position's
+        next token, the last one's left out (``gmdn_amd.logprobs.IGNORE``) --
+        with entropies and ``top`` alternatives (``TokenLogprobs``)."""
+        if tokens is None:
+            tokens = F.pad(idx[:, 1:], (0, 1), value=logprobs.IGNORE)
+        return logprobs.token_logprobs(self(idx)[0], tokens, top)
