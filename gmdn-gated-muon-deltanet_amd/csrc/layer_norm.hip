@@ -12,9 +12,10 @@
 namespace gmdn {
 namespace {
 
-constexpr int LN_THREADS = 256;      // threads of a workgroup, or a row's if more
+constexpr int LN_THREADS = 512;      // threads of a workgroup, or a row's if more
 constexpr int LN_MAX_D = 16384;
-constexpr int LN_MAX_BLOCKS = 1024;  // workgroups of the backward (partial sums)
+constexpr int LN_FWD_BLOCKS = 1024;
+constexpr int LN_BWD_BLOCKS = 256;   // of the backward: each writes 2 d partial sums
 
 constexpr int ln_threads(int tpr) { return tpr > LN_THREADS ? tpr : LN_THREADS; }
 
@@ -60,20 +61,29 @@ ln_fwd(const TX* __restrict__ x, const void* __restrict__ w, const void* __restr
     if (c < d && w) load8_weight(w, w16, c, d - c, wv[i]);
     if (c < d && b) load8_weight(b, w16, c, d - c, bv[i]);
   }
-  for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < rows; r0 += (int64_t)gridDim.x * RPB) {
-    const int64_t r = r0 + lr;
+  // the next row's pieces are loaded before this row's sums
+  Raw8<TX> raw[NV];
+  auto fetch = [&](int64_t r) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = 8 * (i * TPR + t);
+      raw[i].load(x + r * xs + c, r < rows ? d - c : 0);
+    }
+  };
+  const int64_t step = (int64_t)gridDim.x * RPB;
+  int64_t r = (int64_t)blockIdx.x * RPB + lr;
+  fetch(r);
+  for (; r - lr < rows; r += step) {
     const bool live = r < rows;
     float v[NV][8];
     float s = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = 8 * (i * TPR + t);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
-      if (live && c < d) load8(x + r * xs + c, d - c, v[i]);
+      raw[i].get(v[i]);
 #pragma unroll
       for (int j = 0; j < 8; ++j) s += v[i][j];
     }
+    fetch(r + step);
     const float m = row_sum<TPR>(s, red, slot) / (float)d;
     float ss = 0.f;
 #pragma unroll
@@ -117,14 +127,24 @@ template <typename TX>
 struct FromX {
   const TX* x;
   int64_t stride;
-  GMDN_DEV void load(int64_t r, int c, int d, float (&v)[8]) const { load8(x + r * stride + c, d - c, v); }
+  struct Raw : Raw8<TX> {
+    GMDN_DEV void load(const FromX& src, int64_t r, int c, int n, int) {
+      Raw8<TX>::load(src.x + r * src.stride + c, n);
+    }
+  };
 };
 struct From8 {
   const int8_t* q;
   const float* scale;
-  GMDN_DEV void load(int64_t r, int c, int d, float (&v)[8]) const {
-    dequant8(load_q8(q + r * d + c, d - c), scale[r * groups8(d) + c / GROUP8], v);
-  }
+  struct Raw {
+    u32x2_any v;
+    float s;
+    GMDN_DEV void load(const From8& src, int64_t r, int c, int n, int d) {
+      v = load_q8(src.q + r * d + c, n);
+      s = n > 0 ? src.scale[r * groups8(d) + c / GROUP8] : 0.f;
+    }
+    GMDN_DEV void get(float (&x)[8]) const { dequant8(v, s, x); }
+  };
 };
 
 // dx, and per workgroup the sums of dy xh and dy over its rows: part is
@@ -137,6 +157,7 @@ ln_bwd(Src src, const TY* __restrict__ dy, int64_t ds, const void* __restrict__ 
        const float* __restrict__ mean, const float* __restrict__ rstd, TX* __restrict__ dx,
        float* __restrict__ part, int64_t rows, int d) {
   constexpr int RPB = ln_threads(TPR) / TPR;
+  constexpr bool AHEAD = TPR < 1024;  // a row's loads before the last row's work, where the registers hold them
   __shared__ float red[2][16];
   const int lr = threadIdx.x / TPR, t = threadIdx.x % TPR;
   int slot = 0;
@@ -151,21 +172,37 @@ ln_bwd(Src src, const TY* __restrict__ dy, int64_t ds, const void* __restrict__ 
     }
     if (c < d && w) load8_weight(w, w16, c, d - c, wv[i]);
   }
-  for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < rows; r0 += (int64_t)gridDim.x * RPB) {
-    const int64_t r = r0 + lr;
+  typename Src::Raw xr[NV];
+  Raw8<TY> gr[NV];
+  float mr, rr;
+  auto fetch = [&](int64_t r) {
     const bool live = r < rows;
-    float v[NV][8], g[NV][8];
-    const float m = live ? mean[r] : 0.f, rs = live ? rstd[r] : 0.f;
-    float s0 = 0.f, s1 = 0.f;
+    mr = live ? mean[r] : 0.f;
+    rr = live ? rstd[r] : 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = 8 * (i * TPR + t);
+      xr[i].load(src, r, c, live ? d - c : 0, d);
+      gr[i].load(dy + r * ds + c, live ? d - c : 0);
+    }
+  };
+  const int64_t step = (int64_t)gridDim.x * RPB;
+  int64_t r = (int64_t)blockIdx.x * RPB + lr;
+  if constexpr (AHEAD) fetch(r);
+  for (; r - lr < rows; r += step) {
+    if constexpr (!AHEAD) fetch(r);
+    const bool live = r < rows;
+    float v[NV][8], g[NV][8];
+    const float m = mr, rs = rr;
+    float s0 = 0.f, s1 = 0.f;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[i][j] = g[i][j] = 0.f;
-      if (live && c < d) {
-        src.load(r, c, d, v[i]);
-        load8(dy + r * ds + c, d - c, g[i]);
-      }
+    for (int i = 0; i < NV; ++i) {
+      xr[i].get(v[i]);
+      gr[i].get(g[i]);
+    }
+    if constexpr (AHEAD) fetch(r + step);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         v[i][j] = (v[i][j] - m) * rs;  // xh; a dead lane's g is 0
@@ -216,39 +253,55 @@ ln_bwd(Src src, const TY* __restrict__ dy, int64_t ds, const void* __restrict__ 
   }
 }
 
-// dweight and dbias from the workgroups' sums, one column of (2, d) a lane
-// group: a workgroup takes 32 columns, 8 threads each with every 8th partial
-// row; added in a fixed order, the same bits on every run.
+// dweight and dbias from the workgroups' sums: a workgroup takes 32 columns
+// of (2, d) -- 8 lanes of 4 -- and 128 lane groups every 128th partial row, four
+// of them in flight; joined in a wave, then over the waves in LDS.  The order
+// is fixed: the same bits on every run.
 constexpr int LN_COLS = 32;
-constexpr int LN_SPLIT = LN_THREADS / LN_COLS;
-__global__ void __launch_bounds__(LN_THREADS)
+constexpr int LN_SUM_THREADS = 1024;
+__global__ void __launch_bounds__(LN_SUM_THREADS)
 ln_sums(const float* __restrict__ part, void* __restrict__ dw, void* __restrict__ db, bool w16, int d, int nblk) {
-  __shared__ float red[LN_SPLIT][LN_COLS];
-  const int cl = threadIdx.x % LN_COLS, sp = threadIdx.x / LN_COLS;
-  const int c = blockIdx.x * LN_COLS + cl;
-  float a0 = 0.f, a1 = 0.f, a2 = 0.f, a3 = 0.f;
-  if (c < 2 * d) {
-    int i = sp;
-    for (; i + 3 * LN_SPLIT < nblk; i += 4 * LN_SPLIT) {
-      a0 += part[(int64_t)i * 2 * d + c];
-      a1 += part[(int64_t)(i + LN_SPLIT) * 2 * d + c];
-      a2 += part[(int64_t)(i + 2 * LN_SPLIT) * 2 * d + c];
-      a3 += part[(int64_t)(i + 3 * LN_SPLIT) * 2 * d + c];
-    }
-    for (; i < nblk; i += LN_SPLIT) a0 += part[(int64_t)i * 2 * d + c];
-  }
-  red[sp][cl] = (a0 + a1) + (a2 + a3);
-  __syncthreads();
-  if (sp == 0 && c < 2 * d) {
-    float s = red[0][cl];
+  constexpr int SPLIT = LN_SUM_THREADS / 8;
+  __shared__ f32x4 red[LN_SUM_THREADS / 64][8];
+  const int64_t width = 2 * (int64_t)d;
+  const int quad = threadIdx.x % 8, sp = threadIdx.x / 8;
+  const int64_t c = (int64_t)blockIdx.x * LN_COLS + 4 * quad;
+  f32x4 a[4] = {zero4(), zero4(), zero4(), zero4()};
+  for (int i0 = sp; i0 < nblk; i0 += 4 * SPLIT)
 #pragma unroll
-    for (int i = 1; i < LN_SPLIT; ++i) s += red[i][cl];
-    void* out = c < d ? dw : db;
-    const int at = c < d ? c : c - d;
-    if (w16)
-      reinterpret_cast<bf16*>(out)[at] = (bf16)s;
-    else
-      reinterpret_cast<float*>(out)[at] = s;
+    for (int k = 0; k < 4; ++k) {
+      const int i = i0 + k * SPLIT;
+      if (i >= nblk) continue;
+      const float* p = part + i * width + c;
+      if (c + 4 <= width) {
+        a[k] += *reinterpret_cast<const f32x4_any*>(p);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (c + j < width) a[k][j] += p[j];
+      }
+    }
+  f32x4 s = (a[0] + a[1]) + (a[2] + a[3]);
+#pragma unroll
+  for (int o = 8; o < 64; o <<= 1)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s[j] += __shfl_xor(s[j], o, 64);
+  if (lane_id() < 8) red[wave_id()][quad] = s;
+  __syncthreads();
+  if (threadIdx.x < 8) {
+    s = red[0][quad];
+#pragma unroll
+    for (int i = 1; i < LN_SUM_THREADS / 64; ++i) s += red[i][quad];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (c + j >= width) continue;
+      void* out = c + j < d ? dw : db;
+      const int64_t at = c + j < d ? c + j : c + j - d;
+      if (w16)
+        reinterpret_cast<bf16*>(out)[at] = (bf16)s[j];
+      else
+        reinterpret_cast<float*>(out)[at] = s[j];
+    }
   }
 }
 
@@ -263,7 +316,9 @@ ln_rebuild(From8 src, const void* __restrict__ w, const void* __restrict__ b, bo
     const int64_t r = p / pieces;
     const int c = 8 * (int)(p - r * pieces);
     float v[8], wv[8], bv[8];
-    src.load(r, c, d, v);
+    From8::Raw raw;
+    raw.load(src, r, c, d - c, d);
+    raw.get(v);
     const float m = mean[r], rs = rstd[r];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -297,14 +352,14 @@ void with_shape(int64_t d, F&& f) {
   else f(Shape<1024, 2>{});
 }
 
-int64_t ln_blocks(int64_t rows, int64_t d) {
+int64_t ln_blocks(int64_t rows, int64_t d, int64_t most) {
   int64_t n = 0;
   with_shape(d, [&](auto s) {
     using S = decltype(s);
     constexpr int RPB = ln_threads(S::TPR) / S::TPR;
     n = (rows + RPB - 1) / RPB;
   });
-  return n < LN_MAX_BLOCKS ? n : LN_MAX_BLOCKS;
+  return n < most ? n : most;
 }
 
 // The built pairs of types: (bf16, bf16), (float32, float32) and a float32
@@ -340,7 +395,7 @@ int gmdn_layer_norm_fwd(const void* x, const void* weight, const void* bias, voi
   if (!(eps >= 0.f) || x_stride < 0 || (bias && !weight) || !q != !scale) return GMDN_ERR_ARG;
   if (rows == 0) return GMDN_OK;
   if (!x || !y || !mean || !rstd) return GMDN_ERR_ARG;
-  const dim3 grid((unsigned)ln_blocks(rows, d));
+  const dim3 grid((unsigned)ln_blocks(rows, d, LN_FWD_BLOCKS));
   const bool w16 = w_type == GMDN_DTYPE_BF16;
   with_types(x_type, y_type, [&](auto tx, auto ty) {
     using TX = decltype(tx);
@@ -361,7 +416,7 @@ int gmdn_layer_norm_fwd(const void* x, const void* weight, const void* bias, voi
 
 size_t gmdn_layer_norm_bwd_workspace_floats(int64_t rows, int64_t d) {
   if (rows <= 0 || check_dims(rows, d) != GMDN_OK) return 0;
-  return (size_t)(ln_blocks(rows, d) * 2 * d);
+  return (size_t)(ln_blocks(rows, d, LN_BWD_BLOCKS) * 2 * d);
 }
 
 int gmdn_layer_norm_bwd(const void* dy, const void* x, const int8_t* q, const float* scale, const void* weight,
@@ -378,7 +433,7 @@ int gmdn_layer_norm_bwd(const void* dy, const void* x, const int8_t* q, const fl
   int64_t nb = 0;
   if (rows > 0) {
     if (!dy || (!x && !q) || (x && q) || !mean || !rstd || !dx) return GMDN_ERR_ARG;
-    nb = ln_blocks(rows, d);
+    nb = ln_blocks(rows, d, LN_BWD_BLOCKS);
     if (weight && (!workspace || workspace_floats < (size_t)(nb * 2 * d))) return GMDN_ERR_WORKSPACE;
     with_types(x_type, y_type, [&](auto tx, auto ty) {
       using TX = decltype(tx);
@@ -398,7 +453,7 @@ int gmdn_layer_norm_bwd(const void* dy, const void* x, const int8_t* q, const fl
     if (hipGetLastError() != hipSuccess) return GMDN_ERR_LAUNCH;
   }
   if (!weight) return GMDN_OK;
-  hipLaunchKernelGGL(ln_sums, dim3((unsigned)((2 * d + LN_COLS - 1) / LN_COLS)), dim3(LN_THREADS), 0, st, workspace,
+  hipLaunchKernelGGL(ln_sums, dim3((unsigned)((2 * d + LN_COLS - 1) / LN_COLS)), dim3(LN_SUM_THREADS), 0, st, workspace,
                      dweight, dbias, w16, (int)d, (int)nb);
   return launched();
 }

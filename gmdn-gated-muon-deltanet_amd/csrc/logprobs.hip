@@ -36,10 +36,11 @@ GMDN_DEV void rescale(Sums& a, float m) {
   a.s *= k;
   a.m = m;
 }
-GMDN_DEV void add8(Sums& a, const float (&x)[8]) {
-  float m = a.m;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) m = fmaxf(m, x[j]);
+GMDN_DEV float max8(const float (&x)[8]) {
+  return fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+}
+GMDN_DEV void add8(Sums& a, const float (&x)[8], float most) {
+  const float m = fmaxf(a.m, most);
   rescale(a, m);
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
@@ -48,6 +49,7 @@ GMDN_DEV void add8(Sums& a, const float (&x)[8]) {
     a.w += e * fmaxf(u, FAR);
   }
 }
+GMDN_DEV void add8(Sums& a, const float (&x)[8]) { add8(a, x, max8(x)); }
 
 // The row's sums from its threads': the maximum of all, then s and w at it.
 template <int NT>
@@ -98,6 +100,8 @@ GMDN_DEV void write_row(const Row& r, const T* x, int64_t token, int64_t ignore,
   stats[2 * row + 1] = r.logs;
 }
 
+constexpr int PIECES = 4;  // pieces a thread loads before it works on them
+
 template <typename T, int NT>
 __global__ void __launch_bounds__(NT)
 lp_fwd(const T* __restrict__ logits, const int64_t* __restrict__ tokens, float* __restrict__ lp,
@@ -106,9 +110,21 @@ lp_fwd(const T* __restrict__ logits, const int64_t* __restrict__ tokens, float* 
   const int64_t row = blockIdx.x;
   const T* x = logits + row * stride;
   Sums a = no_sums();
-  for (int c = 8 * threadIdx.x; c < V; c += 8 * NT) {
+  int c0 = 8 * threadIdx.x;
+  for (; c0 + 8 * NT * (PIECES - 1) + 8 <= V; c0 += 8 * NT * PIECES) {
+    Raw8<T> raw[PIECES];
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) raw[i].load(x + c0 + 8 * NT * i, 8);
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+      float v[8];
+      raw[i].get(v);
+      add8(a, v);
+    }
+  }
+  for (; c0 < V; c0 += 8 * NT) {
     float v[8];
-    load8(x + c, V - c, v, -INFINITY);
+    load8(x + c0, V - c0, v, -INFINITY);
     add8(a, v);
   }
   a = join<NT>(a, red);
@@ -122,6 +138,11 @@ GMDN_DEV uint64_t key_of(float x, int index) {
   uint32_t b = __builtin_bit_cast(uint32_t, x + 0.f);  // -0 as 0
   b = x != x ? 0xfffffffeu : (b & 0x80000000u) ? ~b : b | 0x80000000u;
   return ((uint64_t)b << 32) | (0xffffffffu - (uint32_t)index);
+}
+// The value of a key (none: -inf, which every logit reaches).
+GMDN_DEV float value_of(uint64_t key) {
+  const uint32_t b = (uint32_t)(key >> 32);
+  return b == 0 ? -INFINITY : __builtin_bit_cast(float, (b & 0x80000000u) ? b & 0x7fffffffu : ~b);
 }
 GMDN_DEV int index_of(uint64_t key) { return (int)(0xffffffffu - (uint32_t)key); }
 
@@ -143,8 +164,11 @@ GMDN_DEV uint64_t lanes_max64(uint64_t x) {
 // threads of the same lane number form 64 groups; the top-th best of the 64
 // groups' best logits bounds the tile's top-th best from below, and few
 // logits reach it (24 of random ones for 20 wanted: each group's pieces lie
-// 512 apart, so that neighbours do not share a group).  Those join the best
-// of the tiles before in a list, and a logit's rank is the number of better
+// 512 apart, so that neighbours do not share a group).  A group's best is its
+// largest value with the last index of the first piece that has it, which no
+// better logit of that value exceeds: equal logits, masked ones above all,
+// stay out of the list by their index.  Those that reach the bound join the best
+// of the tiles before in the list, and a logit's rank is the number of better
 // ones in it.  A tile that gives more than the list holds, or a row with a
 // NaN, is done over by `slow_top`.
 template <typename T, int NT>
@@ -195,21 +219,20 @@ lp_top(const T* __restrict__ logits, const int64_t* __restrict__ tokens, float* 
       for (int j = 0; j < 8; ++j) v[i][j] = -INFINITY;
       if (c < V) load8(x + c, V - c, v[i], -INFINITY);
     }
-    // the thread's best: its value, and the first index that has it
-    float bv = v[0][0];
-    int bi = c0 + 8 * tid;
+    // the thread's best: its value, and the first piece that has it
+    float bv = -INFINITY;
+    int bp = 0;
 #pragma unroll
     for (int i = 0; i < TOP_PIECES; ++i) {
-      add8(a, v[i]);
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (v[i][j] > bv) {
-          bv = v[i][j];
-          bi = c0 + 8 * (i * NT + tid) + j;
-        }
+      const float pm = max8(v[i]);
+      add8(a, v[i], pm);
+      if (pm > bv) {
+        bv = pm;
+        bp = i;
+      }
     }
     if (over) continue;
-    best[tid] = c0 + 8 * tid < V ? key_of(bv, bi) : 0;
+    best[tid] = c0 + 8 * tid < V ? key_of(bv, c0 + 8 * (bp * NT + tid) + 7) : 0;
     if (tid == 0) count = 0;
     __syncthreads();
     if (wave_id() == 0) {
@@ -229,18 +252,21 @@ lp_top(const T* __restrict__ logits, const int64_t* __restrict__ tokens, float* 
       if (rank == top - 1) bound = have == top && run[cur][top - 1] > k ? run[cur][top - 1] : k;
     }
     __syncthreads();
+    // by value first: few logits come as far as their keys
     const uint64_t least = bound;
+    const float lv = value_of(least);
 #pragma unroll
     for (int i = 0; i < TOP_PIECES; ++i)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int c = c0 + 8 * (i * NT + tid) + j;
-        const uint64_t k = key_of(v[i][j], c);
-        if (c < V && k >= least) {
-          const int at = atomicAdd(&count, 1);
-          if (at < TOP_LIST) list[at] = k;
+      for (int j = 0; j < 8; ++j)
+        if (v[i][j] >= lv) {
+          const int c = c0 + 8 * (i * NT + tid) + j;
+          const uint64_t k = key_of(v[i][j], c);
+          if (c < V && k >= least) {
+            const int at = atomicAdd(&count, 1);
+            if (at < TOP_LIST) list[at] = k;
+          }
         }
-      }
     __syncthreads();
     int n = count;
     over = n > TOP_LIST;

@@ -61,6 +61,35 @@ GMDN_DEV void store8(float* p, int n, const float (&x)[8]) {
       if (j < n) p[j] = x[j];
   }
 }
+// A piece as it lies in memory, for loads that are to be in flight over other
+// work; values from n on are 0.
+template <typename T>
+struct Raw8;
+template <>
+struct Raw8<bf16> {
+  bf16x8 v;
+  GMDN_DEV void load(const bf16* p, int n) {
+    if (n >= 8) {
+      v = *reinterpret_cast<const bf16x8_any*>(p);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = j < n ? p[j] : (bf16)0.f;
+    }
+  }
+  GMDN_DEV void get(float (&x)[8]) const {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = (float)v[j];
+  }
+};
+template <>
+struct Raw8<float> {
+  float v[8];
+  GMDN_DEV void load(const float* p, int n) { load8(p, n, v); }
+  GMDN_DEV void get(float (&x)[8]) const {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = v[j];
+  }
+};
 // Values of a weight vector held in float32 or bf16 (is_bf16).
 GMDN_DEV void load8_weight(const void* w, bool is_bf16, int at, int n, float (&x)[8]) {
   if (is_bf16)
