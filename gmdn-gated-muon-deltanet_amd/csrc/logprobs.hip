@@ -20,6 +20,7 @@ constexpr float LOG2E = 1.44269504088896340736f;
 // Differences of logits are clamped here where they multiply a sum: e^-200
 // is 0 in float32, and 0 times the clamped value is 0, not NaN.
 constexpr float FAR = -200.f;
+constexpr int PIECES = 4;  // pieces a thread loads before it works on them
 
 GMDN_DEV float exp_of(float x) { return __builtin_amdgcn_exp2f(x * LOG2E); }
 
@@ -36,8 +37,15 @@ GMDN_DEV void rescale(Sums& a, float m) {
   a.s *= k;
   a.m = m;
 }
+// The instruction by name: for fmaxf of loaded values the compiler first
+// quiets each one, which costs as much again.  A NaN gives way to the others.
+GMDN_DEV float max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
 GMDN_DEV float max8(const float (&x)[8]) {
-  return fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+  return max3(max3(x[0], x[1], x[2]), max3(x[3], x[4], x[5]), fmaxf(x[6], x[7]));
 }
 GMDN_DEV void add8(Sums& a, const float (&x)[8], float most) {
   const float m = fmaxf(a.m, most);
@@ -52,26 +60,32 @@ GMDN_DEV void add8(Sums& a, const float (&x)[8], float most) {
 GMDN_DEV void add8(Sums& a, const float (&x)[8]) { add8(a, x, max8(x)); }
 
 // The row's sums from its threads': the maximum of all, then s and w at it.
+// A row of one wave needs no LDS.
 template <int NT>
 GMDN_DEV Sums join(Sums a, float (*red)[16]) {
   constexpr int W = NT / 64;
   float m = lanes_max<64>(a.m);
-  if (lane_id() == 0) red[0][wave_id()] = m;
-  __syncthreads();
+  if constexpr (W > 1) {
+    if (lane_id() == 0) red[0][wave_id()] = m;
+    __syncthreads();
 #pragma unroll
-  for (int i = 0; i < W; ++i) m = fmaxf(m, red[0][i]);
-  rescale(a, m);
-  const float s = lanes_sum<64>(a.s), w = lanes_sum<64>(a.w);
-  if (lane_id() == 0) {
-    red[1][wave_id()] = s;
-    red[2][wave_id()] = w;
+    for (int i = 0; i < W; ++i) m = fmaxf(m, red[0][i]);
   }
-  __syncthreads();
-  a.s = a.w = 0.f;
+  rescale(a, m);
+  a.s = lanes_sum<64>(a.s);
+  a.w = lanes_sum<64>(a.w);
+  if constexpr (W > 1) {
+    if (lane_id() == 0) {
+      red[1][wave_id()] = a.s;
+      red[2][wave_id()] = a.w;
+    }
+    __syncthreads();
+    a.s = a.w = 0.f;
 #pragma unroll
-  for (int i = 0; i < W; ++i) {
-    a.s += red[1][i];
-    a.w += red[2][i];
+    for (int i = 0; i < W; ++i) {
+      a.s += red[1][i];
+      a.w += red[2][i];
+    }
   }
   return a;
 }
@@ -89,32 +103,47 @@ GMDN_DEV Row row_of(const Sums& a) {
   return {a.m, logs, h < 0.f ? 0.f : h, false};
 }
 
-template <typename T>
-GMDN_DEV void write_row(const Row& r, const T* x, int64_t token, int64_t ignore, int V, int64_t row, float* lp,
-                        float* entropy, float* stats) {
-  float l = 0.f;
-  if (token != ignore) l = token >= 0 && token < V ? r.logprob((float)x[token]) : NAN;
-  lp[row] = l;
-  entropy[row] = r.entropy;
-  stats[2 * row] = r.m;
-  stats[2 * row + 1] = r.logs;
-}
+// The outputs of a call, and its tokens.
+struct Out {
+  const int64_t* tokens;
+  int64_t ignore;
+  float *lp, *entropy, *stats, *top_lp;
+  int64_t* top_tokens;
+  int V, top;
+  template <typename T>
+  GMDN_DEV void row(int64_t row, const Row& r, const T* x) const {
+    const int64_t token = tokens[row];
+    float l = 0.f;
+    if (token != ignore) l = token >= 0 && token < V ? r.logprob((float)x[token]) : NAN;
+    lp[row] = l;
+    entropy[row] = r.entropy;
+    stats[2 * row] = r.m;
+    stats[2 * row + 1] = r.logs;
+  }
+  template <typename T>
+  GMDN_DEV void alternative(int64_t row, int i, int token, const Row& r, const T* x) const {
+    top_tokens[row * top + i] = token;
+    top_lp[row * top + i] = r.logprob((float)x[token]);
+  }
+};
 
-constexpr int PIECES = 4;  // pieces a thread loads before it works on them
+// Where a row's columns are shared by several workgroups: what each leaves
+// for lp_join, its sums and its best logits.
+struct Parts {
+  Sums* sums;      // (rows, parts)
+  uint64_t* best;  // (rows, parts, top)
+  int parts, span; // workgroups of a row, columns of each
+};
 
+// The sums of columns first .. last - 1 of a row by NT threads.
 template <typename T, int NT>
-__global__ void __launch_bounds__(NT)
-lp_fwd(const T* __restrict__ logits, const int64_t* __restrict__ tokens, float* __restrict__ lp,
-       float* __restrict__ entropy, float* __restrict__ stats, int V, int64_t stride, int64_t ignore) {
-  __shared__ float red[3][16];
-  const int64_t row = blockIdx.x;
-  const T* x = logits + row * stride;
+GMDN_DEV Sums sums_of(const T* x, int first, int last, int t) {
   Sums a = no_sums();
-  int c0 = 8 * threadIdx.x;
-  for (; c0 + 8 * NT * (PIECES - 1) + 8 <= V; c0 += 8 * NT * PIECES) {
+  int c0 = first + 8 * t;
+  for (; c0 + 8 * NT * (PIECES - 1) + 8 <= last; c0 += 8 * NT * PIECES) {
     Raw8<T> raw[PIECES];
 #pragma unroll
-    for (int i = 0; i < PIECES; ++i) raw[i].load(x + c0 + 8 * NT * i, 8);
+    for (int i = 0; i < PIECES; ++i) raw[i].stream(x + c0 + 8 * NT * i);
 #pragma unroll
     for (int i = 0; i < PIECES; ++i) {
       float v[8];
@@ -122,13 +151,33 @@ lp_fwd(const T* __restrict__ logits, const int64_t* __restrict__ tokens, float* 
       add8(a, v);
     }
   }
-  for (; c0 < V; c0 += 8 * NT) {
+  for (; c0 < last; c0 += 8 * NT) {
     float v[8];
-    load8(x + c0, V - c0, v, -INFINITY);
+    load8(x + c0, last - c0, v, -INFINITY);
     add8(a, v);
   }
-  a = join<NT>(a, red);
-  if (threadIdx.x == 0) write_row(row_of(a), x, tokens[row], ignore, V, row, lp, entropy, stats);
+  return a;
+}
+
+// A row is TPR threads of the workgroup's 256 (SPLIT: 256 for a part of it).
+constexpr int LP_THREADS = 256;
+template <typename T, int TPR, bool SPLIT>
+__global__ void __launch_bounds__(LP_THREADS)
+lp_fwd(const T* __restrict__ logits, int64_t stride, int64_t rows, Out out, Parts parts) {
+  __shared__ float red[3][16];
+  const int64_t item = (int64_t)blockIdx.x * (LP_THREADS / TPR) + threadIdx.x / TPR;
+  const int t = threadIdx.x % TPR;
+  if (item >= rows * (SPLIT ? parts.parts : 1)) return;  // whole waves, and of rows of one wave only
+  const int64_t row = SPLIT ? item / parts.parts : item;
+  const int first = SPLIT ? (int)(item - row * parts.parts) * parts.span : 0;
+  const int last = SPLIT && first + parts.span < out.V ? first + parts.span : out.V;
+  const T* x = logits + row * stride;
+  const Sums a = join<TPR>(sums_of<T, TPR>(x, first, last, t), red);
+  if (t != 0) return;
+  if constexpr (SPLIT)
+    parts.sums[item] = a;
+  else
+    out.row(row, row_of(a), x);
 }
 
 // ------------------------------------------------------------ top alternatives
@@ -146,10 +195,10 @@ GMDN_DEV float value_of(uint64_t key) {
 }
 GMDN_DEV int index_of(uint64_t key) { return (int)(0xffffffffu - (uint32_t)key); }
 
-constexpr int TOP_MAX = 32;
-constexpr int TOP_PIECES = 4;    // pieces a thread holds of a tile
-constexpr int TOP_LIST = 1024;   // candidates of a tile
-
+GMDN_DEV uint64_t lane_key(uint64_t k, int lane) {
+  return ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(k >> 32), lane) << 32) |
+         (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)k, lane);
+}
 GMDN_DEV uint64_t lanes_max64(uint64_t x) {
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
@@ -160,7 +209,57 @@ GMDN_DEV uint64_t lanes_max64(uint64_t x) {
   return x;
 }
 
-// The row goes by in tiles of NT x 4 pieces held in registers.  Of a tile,
+constexpr int TOP_MAX = 32;
+constexpr int TOP_LIST = 1024;  // candidates of a tile
+
+struct TopLds {
+  uint64_t groups[64];
+  uint64_t list[TOP_LIST + TOP_MAX];
+  uint64_t run[TOP_MAX];  // the best so far, in order
+  uint64_t bound;
+  uint64_t red64[16];
+  float red[3][16];
+  int count;
+};
+
+// The n keys of the list by rank into run: a key's rank is the number of
+// better ones, counted over 64 lanes at a time; a wave ranks every W-th key.
+template <int NT>
+GMDN_DEV void rank_list(TopLds& lds, int n, int top) {
+  const int lane = lane_id();
+  const uint64_t a = lane < n ? lds.list[lane] : 0, b = 64 + lane < n ? lds.list[64 + lane] : 0;
+  for (int i = wave_id(); i < n; i += NT / 64) {
+    const uint64_t k = i < 64 ? lane_key(a, i) : i < 128 ? lane_key(b, i - 64) : lds.list[i];
+    int rank = __popcll(__ballot(a > k)) + __popcll(__ballot(b > k));
+    for (int o = 128; o < n; o += 64) rank += __popcll(__ballot(o + lane < n && lds.list[o + lane] > k));
+    if (rank < top && lane == 0) lds.run[rank] = k;
+  }
+}
+
+// The best `top` of columns first .. last - 1 by one logit a round: for rows
+// that the tiles below give up on.
+template <typename T, int NT>
+GMDN_DEV void slow_top(const T* x, int first, int last, int top, TopLds& lds) {
+  uint64_t prev = ~0ull;
+  for (int k = 0; k < top; ++k) {
+    uint64_t best = 0;
+    for (int c = first + threadIdx.x; c < last; c += NT) {
+      const uint64_t key = key_of((float)x[c], c);
+      if (key < prev && key > best) best = key;
+    }
+    best = lanes_max64(best);
+    __syncthreads();
+    if (lane_id() == 0) lds.red64[wave_id()] = best;
+    __syncthreads();
+    prev = lds.red64[0];
+    for (int i = 1; i < NT / 64; ++i) prev = lds.red64[i] > prev ? lds.red64[i] : prev;
+    if (threadIdx.x == 0) lds.run[k] = prev;
+  }
+  __syncthreads();
+}
+
+// Sums and the best `top` (into lds.run, `have` of them) of columns
+// first .. last - 1, in tiles of NT x 4 pieces held in registers.  Of a tile,
 // threads of the same lane number form 64 groups; the top-th best of the 64
 // groups' best logits bounds the tile's top-th best from below, and few
 // logits reach it (24 of random ones for 20 wanted: each group's pieces lie
@@ -168,146 +267,178 @@ GMDN_DEV uint64_t lanes_max64(uint64_t x) {
 // largest value with the last index of the first piece that has it, which no
 // better logit of that value exceeds: equal logits, masked ones above all,
 // stay out of the list by their index.  Those that reach the bound join the best
-// of the tiles before in the list, and a logit's rank is the number of better
-// ones in it.  A tile that gives more than the list holds, or a row with a
-// NaN, is done over by `slow_top`.
+// of the tiles before in the list, which is ranked.  A tile that gives more
+// than the list holds, or a NaN, is left to slow_top.
 template <typename T, int NT>
-GMDN_DEV void slow_top(const T* x, int V, int top, uint64_t* run, uint64_t* red) {
-  uint64_t prev = ~0ull;
-  for (int k = 0; k < top; ++k) {
-    uint64_t best = 0;
-    for (int c = threadIdx.x; c < V; c += NT) {
-      const uint64_t key = key_of((float)x[c], c);
-      if (key < prev && key > best) best = key;
-    }
-    best = lanes_max64(best);
-    __syncthreads();
-    if (lane_id() == 0) red[wave_id()] = best;
-    __syncthreads();
-    prev = red[0];
-    for (int i = 1; i < NT / 64; ++i) prev = red[i] > prev ? red[i] : prev;
-    if (threadIdx.x == 0) run[k] = prev;
-  }
-  __syncthreads();
-}
-
-template <typename T, int NT>
-__global__ void __launch_bounds__(NT)
-lp_top(const T* __restrict__ logits, const int64_t* __restrict__ tokens, float* __restrict__ lp,
-       float* __restrict__ entropy, float* __restrict__ top_lp, int64_t* __restrict__ top_tokens,
-       float* __restrict__ stats, int V, int64_t stride, int top, int64_t ignore) {
-  constexpr int TILE = NT * TOP_PIECES * 8;
-  __shared__ float red[3][16];
-  __shared__ uint64_t red64[16];
-  __shared__ uint64_t best[NT];
-  __shared__ uint64_t list[TOP_LIST + TOP_MAX];
-  __shared__ uint64_t run[2][TOP_MAX];
-  __shared__ uint64_t bound;
-  __shared__ int count;
+GMDN_DEV Sums top_of(const T* x, int first, int last, int top, TopLds& lds, int& have) {
   const int tid = threadIdx.x;
-  const int64_t row = blockIdx.x;
-  const T* x = logits + row * stride;
   Sums a = no_sums();
-  int have = 0, cur = 0;  // of the best so far, and which half of run holds them
+  have = 0;
   bool over = false;
-  for (int c0 = 0; c0 < V; c0 += TILE) {
-    float v[TOP_PIECES][8];
+  if (tid < 64) lds.groups[tid] = 0;
+  if (tid == 0) lds.count = 0;
+  __syncthreads();
+  for (int c0 = first; c0 < last; c0 += 8 * NT * PIECES) {
+    Raw8<T> raw[PIECES];
+    float most[PIECES];
 #pragma unroll
-    for (int i = 0; i < TOP_PIECES; ++i) {
+    for (int i = 0; i < PIECES; ++i) {
       const int c = c0 + 8 * (i * NT + tid);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[i][j] = -INFINITY;
-      if (c < V) load8(x + c, V - c, v[i], -INFINITY);
+      if (c + 8 <= last)
+        raw[i].stream(x + c);
+      else
+        raw[i].load(x + c, last - c, -INFINITY);
     }
     // the thread's best: its value, and the first piece that has it
     float bv = -INFINITY;
     int bp = 0;
 #pragma unroll
-    for (int i = 0; i < TOP_PIECES; ++i) {
-      const float pm = max8(v[i]);
-      add8(a, v[i], pm);
-      if (pm > bv) {
-        bv = pm;
+    for (int i = 0; i < PIECES; ++i) {
+      float v[8];
+      raw[i].get(v);
+      most[i] = max8(v);
+      add8(a, v, most[i]);
+      if (most[i] > bv) {
+        bv = most[i];
         bp = i;
       }
+      __builtin_amdgcn_sched_barrier(0);  // one piece's values at a time in registers
     }
     if (over) continue;
-    best[tid] = c0 + 8 * tid < V ? key_of(bv, c0 + 8 * (bp * NT + tid) + 7) : 0;
-    if (tid == 0) count = 0;
+    if (c0 + 8 * tid < last)
+      atomicMax((unsigned long long*)&lds.groups[lane_id()],
+                (unsigned long long)key_of(bv, c0 + 8 * (bp * NT + tid) + 7));
     __syncthreads();
-    if (wave_id() == 0) {
-      uint64_t k = best[tid];
-#pragma unroll
-      for (int i = 1; i < NT / 64; ++i) {
-        const uint64_t o = best[i * 64 + tid];
-        k = o > k ? o : k;
+    {
+      // a wave ranks its share of the groups against all 64; equal only where there is none
+      const uint64_t mine = lds.groups[lane_id()];
+      constexpr int SHARE = 64 / (NT / 64);
+      for (int g = wave_id() * SHARE; g < (wave_id() + 1) * SHARE; ++g) {
+        const uint64_t k = lane_key(mine, g);
+        if (__popcll(__ballot(mine > k || (mine == k && lane_id() < g))) == top - 1 && lane_id() == 0)
+          lds.bound = have == top && lds.run[top - 1] > k ? lds.run[top - 1] : k;
       }
-      int rank = 0;
-#pragma unroll
-      for (int i = 0; i < 64; ++i) {
-        const uint64_t o = ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(k >> 32), i) << 32) |
-                           (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)k, i);
-        rank += o > k || (o == k && i < tid);  // equal only where there is none
-      }
-      if (rank == top - 1) bound = have == top && run[cur][top - 1] > k ? run[cur][top - 1] : k;
     }
     __syncthreads();
-    // by value first: few logits come as far as their keys
-    const uint64_t least = bound;
+    if (tid < 64) lds.groups[tid] = 0;
+    // candidates: by value first, then by key; places in the list by one
+    // addition a wave
+    const uint64_t least = lds.bound;
     const float lv = value_of(least);
+    uint32_t found = 0;
 #pragma unroll
-    for (int i = 0; i < TOP_PIECES; ++i)
+    for (int i = 0; i < PIECES; ++i) {
+      if (!(most[i] >= lv)) continue;
+      float v[8];
+      raw[i].get(v);
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (v[i][j] >= lv) {
-          const int c = c0 + 8 * (i * NT + tid) + j;
-          const uint64_t k = key_of(v[i][j], c);
-          if (c < V && k >= least) {
-            const int at = atomicAdd(&count, 1);
-            if (at < TOP_LIST) list[at] = k;
-          }
-        }
-    __syncthreads();
-    int n = count;
-    over = n > TOP_LIST;
-    if (!over) {
-      if (tid < have) list[n + tid] = run[cur][tid];
-      __syncthreads();
-      n += have;
-      for (int i = tid; i < n; i += NT) {
-        const uint64_t k = list[i];
-        int rank = 0;
-        for (int o = 0; o < n; ++o) rank += list[o] > k;
-        if (rank < top) run[cur ^ 1][rank] = k;
+      for (int j = 0; j < 8; ++j) {
+        const int c = c0 + 8 * (i * NT + tid) + j;
+        if (c < last && key_of(v[j], c) >= least) found |= 1u << (8 * i + j);
       }
+    }
+    if (__ballot(found != 0)) {
+      const int mine = __popc(found);
+      int upto = mine;  // of lanes up to this one
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const int y = __shfl_up(upto, o, 64);
+        if (lane_id() >= o) upto += y;
+      }
+      int at = 0;
+      if (lane_id() == 63) at = atomicAdd(&lds.count, upto);
+      at = __shfl(at, 63, 64) + upto - mine;
+#pragma unroll
+      for (int i = 0; i < PIECES; ++i) {
+        if (!(found >> (8 * i) & 0xff)) continue;
+        float v[8];
+        raw[i].get(v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (found >> (8 * i + j) & 1) {
+            if (at < TOP_LIST) lds.list[at] = key_of(v[j], c0 + 8 * (i * NT + tid) + j);
+            ++at;
+          }
+      }
+    }
+    __syncthreads();
+    int n = lds.count;
+    over = n > TOP_LIST;
+    if (!over && tid < have) lds.list[n + tid] = lds.run[tid];
+    __syncthreads();
+    if (tid == 0) lds.count = 0;
+    if (!over) {
+      n += have;
+      rank_list<NT>(lds, n, top);
       have = n < top ? n : top;
-      cur ^= 1;
     }
     __syncthreads();
   }
-  a = join<NT>(a, red);
-  const Row r = row_of(a);
-  if (over || a.s != a.s) slow_top<T, NT>(x, V, top, run[cur], red64);
-  if (tid == 0) write_row(r, x, tokens[row], ignore, V, row, lp, entropy, stats);
-  if (tid < top) {
-    const int i = index_of(run[cur][tid]);
-    top_tokens[row * top + tid] = i;
-    top_lp[row * top + tid] = r.logprob((float)x[i]);
+  a = join<NT>(a, lds.red);
+  if (over || a.s != a.s) {
+    slow_top<T, NT>(x, first, last, top < last - first ? top : last - first, lds);
+    have = top < last - first ? top : last - first;
+  }
+  return a;
+}
+
+template <typename T, int NT, bool SPLIT>
+__global__ void __launch_bounds__(NT, 8)
+lp_top(const T* __restrict__ logits, int64_t stride, Out out, Parts parts) {
+  __shared__ TopLds lds;
+  const int64_t item = blockIdx.x, row = SPLIT ? item / parts.parts : item;
+  const int first = SPLIT ? (int)(item - row * parts.parts) * parts.span : 0;
+  const int last = SPLIT && first + parts.span < out.V ? first + parts.span : out.V;
+  const T* x = logits + row * stride;
+  int have;
+  const Sums a = top_of<T, NT>(x, first, last, out.top, lds, have);
+  const int i = threadIdx.x;
+  if constexpr (SPLIT) {
+    if (i == 0) parts.sums[item] = a;
+    if (i < out.top) parts.best[item * out.top + i] = i < have ? lds.run[i] : 0;
+  } else {
+    const Row r = row_of(a);
+    if (i == 0) out.row(row, r, x);
+    if (i < out.top) out.alternative(row, i, index_of(lds.run[i]), r, x);
   }
 }
 
-// ------------------------------------------------------------------ backward
-// A workgroup takes `span` columns of a row.  The columns of the token and
-// the alternatives are written again with their terms once the others are.
-constexpr int LPB_THREADS = 256;
+// A row's outputs from its parts.
+constexpr int MAX_PARTS = 32;
 template <typename T>
-__global__ void __launch_bounds__(LPB_THREADS)
-lp_bwd(const T* __restrict__ logits, const int64_t* __restrict__ tokens, const float* __restrict__ stats,
-       const float* __restrict__ entropy, const int64_t* __restrict__ top_tokens, const float* __restrict__ dlp,
-       const float* __restrict__ dent, const float* __restrict__ dtop, T* __restrict__ dx, int V, int64_t stride,
-       int top, int64_t ignore, int span, int parts) {
-  const int64_t row = blockIdx.x / parts;
-  const int first = (int)(blockIdx.x % parts) * span, last = first + span < V ? first + span : V;
+__global__ void __launch_bounds__(LP_THREADS)
+lp_join(const T* __restrict__ logits, int64_t stride, Out out, Parts parts) {
+  static_assert(MAX_PARTS * TOP_MAX <= TOP_LIST, "the parts' best fit the list");
+  __shared__ TopLds lds;
+  const int64_t row = blockIdx.x;
+  const T* x = logits + row * stride;
+  const int n = parts.parts * out.top;
+  for (int i = threadIdx.x; i < n; i += LP_THREADS) lds.list[i] = parts.best[row * n + i];
+  Sums a = no_sums();
+  if ((int)threadIdx.x < parts.parts) a = parts.sums[row * parts.parts + threadIdx.x];
+  const Row r = row_of(join<LP_THREADS>(a, lds.red));
+  if (threadIdx.x == 0) out.row(row, r, x);
+  if (n == 0) return;
+  rank_list<LP_THREADS>(lds, n, out.top);
+  __syncthreads();
+  if ((int)threadIdx.x < out.top) out.alternative(row, threadIdx.x, index_of(lds.run[threadIdx.x]), r, x);
+}
+
+// ------------------------------------------------------------------ backward
+// TPR threads take `span` columns of a row; a workgroup NT / TPR rows.  The
+// token's term goes to its column where that is computed.  TOP: the columns of
+// token and alternatives are written again with their terms at the end.
+template <typename T, int NT, int TPR, bool TOP>
+__global__ void __launch_bounds__(NT)
+lp_bwd(const T* __restrict__ logits, int64_t stride, int64_t rows, const int64_t* __restrict__ tokens,
+       const float* __restrict__ stats, const float* __restrict__ entropy, const int64_t* __restrict__ top_tokens,
+       const float* __restrict__ dlp, const float* __restrict__ dent, const float* __restrict__ dtop,
+       T* __restrict__ dx, int V, int top, int64_t ignore, int span, int parts) {
+  const int64_t item = (int64_t)blockIdx.x * (NT / TPR) + threadIdx.x / TPR;
+  const int t = threadIdx.x % TPR;
+  if (item >= rows * parts) return;  // rows of one wave only
+  const int64_t row = item / parts;
+  const int first = (int)(item - row * parts) * span, last = first + span < V ? first + span : V;
   const T* x = logits + row * stride;
   T* out = dx + row * V;
   const int64_t token = tokens[row];
@@ -317,7 +448,7 @@ lp_bwd(const T* __restrict__ logits, const int64_t* __restrict__ tokens, const f
   float gl = dlp && token != ignore ? dlp[row] : 0.f;
   if (token != ignore && (token < 0 || token >= V)) gl = NAN;
   float all = gl;
-  if (dtop)
+  if constexpr (TOP)
     for (int i = 0; i < top; ++i) all += dtop[row * top + i];
   // the terms of p (0 throughout an empty row), p as the square of e^(l / 2):
   // the exponential flushes results below 2^-126, the product does not
@@ -325,23 +456,46 @@ lp_bwd(const T* __restrict__ logits, const int64_t* __restrict__ tokens, const f
     const float l = z - m - logs, e = __builtin_amdgcn_exp2f(l * (0.5f * LOG2E));
     return -e * (e * (all + gh * (fmaxf(l, FAR) + h)));
   };
-  for (int c = first + 8 * threadIdx.x; c < last; c += 8 * LPB_THREADS) {
-    float v[8];
-    load8(x + c, last - c, v);
+  auto grad8 = [&](float (&v)[8], int c) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = grad(v[j]);
-    store8(out + c, last - c, v);
+    if constexpr (!TOP)
+      if (token >= c && token < c + 8 && !empty)
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (token == c + j) v[j] += gl;
+  };
+  int c0 = first + 8 * t;
+  for (; c0 + 8 * TPR * (PIECES - 1) + 8 <= last; c0 += 8 * TPR * PIECES) {
+    Raw8<T> raw[PIECES];
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) raw[i].stream(x + c0 + 8 * TPR * i);
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+      float v[8];
+      raw[i].get(v);
+      grad8(v, c0 + 8 * TPR * i);
+      stream8(out + c0 + 8 * TPR * i, v);
+    }
   }
-  __syncthreads();
-  const int n = dtop ? top : 0;
-  if ((int)threadIdx.x <= n && !empty) {
-    auto which = [&](int i) { return i == 0 ? token : top_tokens[row * top + i - 1]; };
-    const int64_t c = which(threadIdx.x);
-    if (c >= first && c < last) {
-      float g = 0.f;
-      for (int i = 0; i <= n; ++i)
-        if (which(i) == c) g += i == 0 ? gl : dtop[row * top + i - 1];
-      out[c] = (T)(grad((float)x[c]) + g);
+  for (; c0 < last; c0 += 8 * TPR) {
+    float v[8];
+    load8(x + c0, last - c0, v);
+    grad8(v, c0);
+    store8(out + c0, last - c0, v);
+  }
+  if constexpr (TOP) {
+    static_assert(NT == TPR, "all of a workgroup comes here");
+    __syncthreads();
+    if (t <= top && !empty) {
+      auto which = [&](int i) { return i == 0 ? token : top_tokens[row * top + i - 1]; };
+      const int64_t c = which(t);
+      if (c >= first && c < last) {
+        float g = 0.f;
+        for (int i = 0; i <= top; ++i)
+          if (which(i) == c) g += i == 0 ? gl : dtop[row * top + i - 1];
+        out[c] = (T)(grad((float)x[c]) + g);
+      }
     }
   }
 }
@@ -349,24 +503,65 @@ lp_bwd(const T* __restrict__ logits, const int64_t* __restrict__ tokens, const f
 int check_lp(int64_t rows, int64_t V, int64_t stride, int32_t top, int32_t dtype) {
   if (rows < 0 || V <= 0 || stride < 0 || top < 0 || top > V) return GMDN_ERR_ARG;
   if (!type_ok(dtype) || top > TOP_MAX || V > (1 << 30)) return GMDN_ERR_UNSUPPORTED;
-  if (rows >= ((int64_t)1 << 31)) return GMDN_ERR_ARG;
+  if (rows > ((int64_t)1 << 30)) return GMDN_ERR_ARG;
   return GMDN_OK;
 }
 
+// Workgroups of a row in the forward.
+constexpr int64_t SPLIT_GRID = 512, SPLIT_SPAN = 16384;
+constexpr int64_t ONE_WAVE = 2048;  // rows of at most so many logits are a wave's
+int parts_of(int64_t rows, int64_t V) {
+  const int64_t room = SPLIT_GRID / rows, most = V / SPLIT_SPAN;
+  const int64_t n = room < most ? room : most;
+  return n < 2 ? 1 : (int)(n < MAX_PARTS ? n : MAX_PARTS);
+}
+int span_of(int64_t V, int parts) { return (int)(((V + parts - 1) / parts + 7) / 8 * 8); }
+
 template <typename T>
-void fwd_launch(const T* x, const int64_t* tokens, float* lp, float* entropy, float* top_lp, int64_t* top_tokens,
-                float* stats, int64_t rows, int64_t V, int64_t stride, int32_t top, int64_t ignore, hipStream_t st) {
-  const dim3 grid((unsigned)rows);
-  if (top > 0) {
-    if (V <= 8192)
-      hipLaunchKernelGGL((lp_top<T, 256>), grid, dim3(256), 0, st, x, tokens, lp, entropy, top_lp, top_tokens, stats,
-                         (int)V, stride, top, ignore);
+void fwd_launch(const T* x, int64_t stride, int64_t rows, const Out& out, Parts p, hipStream_t st) {
+  const dim3 grid((unsigned)(rows * p.parts)), block(LP_THREADS);
+  const bool split = p.parts > 1;
+  if (out.top > 0) {
+    if (split)
+      hipLaunchKernelGGL((lp_top<T, 1024, true>), grid, dim3(1024), 0, st, x, stride, out, p);
+    else if (out.V <= 8 * 256 * PIECES || rows > 256)
+      hipLaunchKernelGGL((lp_top<T, 256, false>), grid, block, 0, st, x, stride, out, p);
     else
-      hipLaunchKernelGGL((lp_top<T, 1024>), grid, dim3(1024), 0, st, x, tokens, lp, entropy, top_lp, top_tokens, stats,
-                         (int)V, stride, top, ignore);
+      hipLaunchKernelGGL((lp_top<T, 1024, false>), grid, dim3(1024), 0, st, x, stride, out, p);
+  } else if (split) {
+    hipLaunchKernelGGL((lp_fwd<T, 256, true>), grid, block, 0, st, x, stride, rows, out, p);
+  } else if (out.V <= ONE_WAVE) {
+    hipLaunchKernelGGL((lp_fwd<T, 64, false>), dim3((unsigned)((rows + 3) / 4)), block, 0, st, x, stride, rows, out, p);
   } else {
-    hipLaunchKernelGGL((lp_fwd<T, 256>), grid, dim3(256), 0, st, x, tokens, lp, entropy, stats, (int)V, stride, ignore);
+    hipLaunchKernelGGL((lp_fwd<T, 256, false>), grid, block, 0, st, x, stride, rows, out, p);
   }
+  if (split) hipLaunchKernelGGL((lp_join<T>), dim3((unsigned)rows), block, 0, st, x, stride, out, p);
+}
+
+template <typename T>
+void bwd_launch(const T* x, int64_t stride, int64_t rows, const int64_t* tokens, const float* stats,
+                const float* entropy, const int64_t* top_tokens, const float* dlp, const float* dent,
+                const float* dtop, T* dx, int64_t V, int32_t top, int64_t ignore, hipStream_t st) {
+  const bool alternatives = dtop && top > 0;
+  // a row's columns over several workgroups where rows do not fill the chip
+  int64_t parts = 512 / rows, most = V / 8192;
+  parts = parts < most ? parts : most;
+  parts = parts < 1 ? 1 : parts;
+  const int span = span_of(V, (int)parts);
+  const int64_t items = rows * parts;
+#define GMDN_LP_BWD(NT, TPR, TOP)                                                                                    \
+  hipLaunchKernelGGL((lp_bwd<T, NT, TPR, TOP>), dim3((unsigned)((items + NT / TPR - 1) / (NT / TPR))), dim3(NT), 0, \
+                     st, x, stride, rows, tokens, stats, entropy, top_tokens, dlp, dent, dtop, dx, (int)V, top,     \
+                     ignore, span, (int)parts)
+  if (alternatives)
+    GMDN_LP_BWD(256, 256, true);
+  else if (V <= ONE_WAVE)
+    GMDN_LP_BWD(256, 64, false);
+  else if (V <= 8 * 256 * PIECES)
+    GMDN_LP_BWD(256, 256, false);
+  else
+    GMDN_LP_BWD(1024, 1024, false);
+#undef GMDN_LP_BWD
 }
 
 }  // namespace
@@ -376,19 +571,30 @@ using namespace gmdn;
 
 extern "C" {
 
+size_t gmdn_logprobs_fwd_workspace_bytes(int64_t rows, int64_t vocab, int32_t top) {
+  if (check_lp(rows, vocab, 0, top, GMDN_DTYPE_F32) != GMDN_OK || rows == 0) return 0;
+  const int64_t items = rows * parts_of(rows, vocab);
+  return items == rows ? 0 : (size_t)(items * (16 + 8 * top));
+}
+
 int gmdn_logprobs_fwd(const void* logits, const int64_t* tokens, float* logprob, float* entropy, float* top_logprobs,
-                      int64_t* top_tokens, float* stats, int64_t rows, int64_t vocab, int64_t stride, int32_t top,
-                      int64_t ignore_index, int32_t dtype, void* stream) {
+                      int64_t* top_tokens, float* stats, void* workspace, size_t workspace_bytes, int64_t rows,
+                      int64_t vocab, int64_t stride, int32_t top, int64_t ignore_index, int32_t dtype, void* stream) {
   const int rc = check_lp(rows, vocab, stride, top, dtype);
   if (rc != GMDN_OK || rows == 0) return rc;
   if (!logits || !tokens || !logprob || !entropy || !stats || (top && (!top_logprobs || !top_tokens)))
     return GMDN_ERR_ARG;
+  const size_t need = gmdn_logprobs_fwd_workspace_bytes(rows, vocab, top);
+  if (need && (!workspace || workspace_bytes < need)) return GMDN_ERR_WORKSPACE;
+  const Out out{tokens, ignore_index, logprob, entropy, stats, top_logprobs, top_tokens, (int)vocab, top};
+  const int parts = parts_of(rows, vocab);
+  // the keys first: 8-byte values at the workspace's start, the sums behind them
+  uint64_t* best = static_cast<uint64_t*>(workspace);
+  const Parts p{need ? reinterpret_cast<Sums*>(best + rows * parts * top) : nullptr, best, parts, span_of(vocab, parts)};
   if (dtype == GMDN_DTYPE_BF16)
-    fwd_launch((const bf16*)logits, tokens, logprob, entropy, top_logprobs, top_tokens, stats, rows, vocab, stride, top,
-               ignore_index, (hipStream_t)stream);
+    fwd_launch((const bf16*)logits, stride, rows, out, p, (hipStream_t)stream);
   else
-    fwd_launch((const float*)logits, tokens, logprob, entropy, top_logprobs, top_tokens, stats, rows, vocab, stride,
-               top, ignore_index, (hipStream_t)stream);
+    fwd_launch((const float*)logits, stride, rows, out, p, (hipStream_t)stream);
   return launched();
 }
 
@@ -398,17 +604,13 @@ int gmdn_logprobs_bwd(const void* logits, const int64_t* tokens, const float* st
                       int32_t dtype, void* stream) {
   const int rc = check_lp(rows, vocab, stride, top, dtype);
   if (rc != GMDN_OK || rows == 0) return rc;
-  if (!logits || !tokens || !stats || !entropy || !dlogits || (dtop && !top_tokens)) return GMDN_ERR_ARG;
-  const int64_t parts = 1, span = (vocab + 7) / 8 * 8;
-  const dim3 grid((unsigned)(rows * parts)), block(LPB_THREADS);
+  if (!logits || !tokens || !stats || !entropy || !dlogits || (dtop && top && !top_tokens)) return GMDN_ERR_ARG;
   if (dtype == GMDN_DTYPE_BF16)
-    hipLaunchKernelGGL(lp_bwd<bf16>, grid, block, 0, (hipStream_t)stream, (const bf16*)logits, tokens, stats, entropy,
-                       top_tokens, dlogprob, dentropy, dtop, (bf16*)dlogits, (int)vocab, stride, top, ignore_index,
-                       (int)span, (int)parts);
+    bwd_launch((const bf16*)logits, stride, rows, tokens, stats, entropy, top_tokens, dlogprob, dentropy, dtop,
+               (bf16*)dlogits, vocab, top, ignore_index, (hipStream_t)stream);
   else
-    hipLaunchKernelGGL(lp_bwd<float>, grid, block, 0, (hipStream_t)stream, (const float*)logits, tokens, stats, entropy,
-                       top_tokens, dlogprob, dentropy, dtop, (float*)dlogits, (int)vocab, stride, top, ignore_index,
-                       (int)span, (int)parts);
+    bwd_launch((const float*)logits, stride, rows, tokens, stats, entropy, top_tokens, dlogprob, dentropy, dtop,
+               (float*)dlogits, vocab, top, ignore_index, (hipStream_t)stream);
   return launched();
 }
 

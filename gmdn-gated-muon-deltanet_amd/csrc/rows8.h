@@ -14,6 +14,8 @@
 namespace gmdn {
 
 typedef bf16 bf16x8_any __attribute__((ext_vector_type(8), aligned(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
 typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
 typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(1)));
 
@@ -51,6 +53,16 @@ GMDN_DEV void store8(bf16* p, int n, const float (&x)[8]) {
       if (j < n) p[j] = v[j];
   }
 }
+// The same for a whole piece that is not read again soon (nontemporal).
+GMDN_DEV void stream8(bf16* p, const float (&x)[8]) {
+  const bf16x8_any v = cat8(to_bf16x4(f32x4{x[0], x[1], x[2], x[3]}), to_bf16x4(f32x4{x[4], x[5], x[6], x[7]}));
+  __builtin_nontemporal_store(v, reinterpret_cast<bf16x8_any*>(p));
+}
+GMDN_DEV void stream8(float* p, const float (&x)[8]) {
+  f32x4_any* q = reinterpret_cast<f32x4_any*>(p);
+  __builtin_nontemporal_store(f32x4_any{x[0], x[1], x[2], x[3]}, q);
+  __builtin_nontemporal_store(f32x4_any{x[4], x[5], x[6], x[7]}, q + 1);
+}
 GMDN_DEV void store8(float* p, int n, const float (&x)[8]) {
   if (n >= 8) {
     *reinterpret_cast<f32x4_any*>(p) = f32x4{x[0], x[1], x[2], x[3]};
@@ -62,29 +74,48 @@ GMDN_DEV void store8(float* p, int n, const float (&x)[8]) {
   }
 }
 // A piece as it lies in memory, for loads that are to be in flight over other
-// work; values from n on are 0.
+// work; values from n on are `pad` (0 or an infinity).  `stream` loads a whole piece that is not
+// wanted again soon (nontemporal).
 template <typename T>
 struct Raw8;
 template <>
 struct Raw8<bf16> {
-  bf16x8 v;
-  GMDN_DEV void load(const bf16* p, int n) {
+  u32x4 v;
+  GMDN_DEV void stream(const bf16* p) {
+    v = __builtin_nontemporal_load(reinterpret_cast<const u32x4_any*>(p));
+  }
+  GMDN_DEV void load(const bf16* p, int n, float pad = 0.f) {
     if (n >= 8) {
-      v = *reinterpret_cast<const bf16x8_any*>(p);
+      v = *reinterpret_cast<const u32x4_any*>(p);
     } else {
+      const uint32_t bits = __builtin_bit_cast(uint32_t, pad) >> 16;
+      const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = j < n ? p[j] : (bf16)0.f;
+      for (int j = 0; j < 4; ++j)
+        v[j] = (2 * j < n ? h[2 * j] : bits) | (2 * j + 1 < n ? (uint32_t)h[2 * j + 1] : bits) << 16;
     }
   }
   GMDN_DEV void get(float (&x)[8]) const {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = (float)v[j];
+    for (int j = 0; j < 4; ++j) {
+      x[2 * j] = __builtin_bit_cast(float, v[j] << 16);
+      x[2 * j + 1] = __builtin_bit_cast(float, v[j] & 0xffff0000u);
+    }
   }
 };
 template <>
 struct Raw8<float> {
   float v[8];
-  GMDN_DEV void load(const float* p, int n) { load8(p, n, v); }
+  GMDN_DEV void stream(const float* p) {
+    const f32x4_any* q = reinterpret_cast<const f32x4_any*>(p);
+    const f32x4_any a = __builtin_nontemporal_load(q), b = __builtin_nontemporal_load(q + 1);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      v[j] = a[j];
+      v[4 + j] = b[j];
+    }
+  }
+  GMDN_DEV void load(const float* p, int n, float pad = 0.f) { load8(p, n, v, pad); }
   GMDN_DEV void get(float (&x)[8]) const {
 #pragma unroll
     for (int j = 0; j < 8; ++j) x[j] = v[j];

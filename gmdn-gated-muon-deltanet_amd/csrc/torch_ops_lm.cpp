@@ -241,9 +241,12 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> logprobs_fwd(const Tensor& lo
   Tensor lp = f32_empty(logits, shape), entropy = f32_empty(logits, shape), stats = f32_empty(logits, with_last(shape, 2));
   Tensor top_lp = f32_empty(logits, with_last(shape, top));
   Tensor top_tokens = at::empty(with_last(shape, top), logits.options().dtype(at::kLong));
+  const size_t need = gmdn_logprobs_fwd_workspace_bytes(r.rows, r.d, (int32_t)top);
+  const Tensor ws = need ? bytes_of(logits, need) : Tensor();
   if (r.rows)
     check(gmdn_logprobs_fwd(r.ptr(), tk.data_ptr<int64_t>(), fp(lp), fp(entropy), fp(top_lp),
-                            top ? top_tokens.data_ptr<int64_t>() : nullptr, fp(stats), r.rows, r.d, r.stride,
+                            top ? top_tokens.data_ptr<int64_t>() : nullptr, fp(stats),
+                            need ? ws.data_ptr() : nullptr, need, r.rows, r.d, r.stride,
                             (int32_t)top, ignore_index, code, stream_of(logits)),
           "gmdn_logprobs_fwd");
   return {lp, entropy, top_lp, top_tokens, stats};

@@ -87,7 +87,8 @@ SIGNATURES = {
     "gmdn_act8_unpack": (c_i32, [c_vp] * 3 + [c_i64] * 2 + [c_i32, c_vp]),
     "gmdn_gelu8_fwd": (c_i32, [c_vp] * 4 + [c_i64] * 3 + [c_i32, c_vp]),
     "gmdn_gelu8_bwd": (c_i32, [c_vp] * 5 + [c_i64] * 3 + [c_i32, c_vp]),
-    "gmdn_logprobs_fwd": (c_i32, [c_vp] * 7 + [c_i64] * 3 + [c_i32, c_i64, c_i32, c_vp]),
+    "gmdn_logprobs_fwd_workspace_bytes": (c_size, [c_i64, c_i64, c_i32]),
+    "gmdn_logprobs_fwd": (c_i32, [c_vp] * 8 + [c_size] + [c_i64] * 3 + [c_i32, c_i64, c_i32, c_vp]),
     "gmdn_logprobs_bwd": (c_i32, [c_vp] * 9 + [c_i64] * 3 + [c_i32, c_i64, c_i32, c_vp]),
 }
 

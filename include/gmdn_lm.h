@@ -84,8 +84,12 @@ int gmdn_gelu8_bwd(const void* da, const int8_t* q, const float* scale, void* dh
  * and entropy 0, and no gradient.  A NaN or +inf in a row makes it NaN (its
  * alternatives are then ordered with NaN first). */
 int gmdn_logprobs_fwd(const void* logits, const int64_t* tokens, float* logprob, float* entropy, float* top_logprobs,
-                      int64_t* top_tokens, float* stats, int64_t rows, int64_t vocab, int64_t stride, int32_t top,
-                      int64_t ignore_index, int32_t dtype, void* stream);
+                      int64_t* top_tokens, float* stats, void* workspace, size_t workspace_bytes, int64_t rows,
+                      int64_t vocab, int64_t stride, int32_t top, int64_t ignore_index, int32_t dtype, void* stream);
+
+/* Bytes of the forward's workspace (8-byte aligned): 0 but for few rows of
+ * large vocabularies, whose columns several workgroups share. */
+size_t gmdn_logprobs_fwd_workspace_bytes(int64_t rows, int64_t vocab, int32_t top);
 
 /* dlogits (rows, vocab) from the cotangents of logprob, entropy and
  * top_logprobs, each of which may be NULL. */

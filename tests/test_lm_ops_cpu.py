@@ -67,8 +67,12 @@ def test_act8_argument_checks():
 def test_logprobs_argument_checks():
     lib = _native.load()
 
-    def fwd(rows=4, V=100, stride=100, top=0, dtype=BF16, logits=P, topp=P, stats=P):
-        return lib.gmdn_logprobs_fwd(logits, P, P, P, topp, topp, stats, rows, V, stride, top, -100, dtype, None)
+    def fwd(rows=4, V=100, stride=100, top=0, dtype=BF16, logits=P, topp=P, stats=P, ws=None, n=0):
+        return lib.gmdn_logprobs_fwd(logits, P, P, P, topp, topp, stats, ws, n, rows, V, stride, top, -100, dtype, None)
+
+    need = lib.gmdn_logprobs_fwd_workspace_bytes(1, 1 << 17, 20)
+    assert need > 0 and lib.gmdn_logprobs_fwd_workspace_bytes(4096, 1 << 17, 20) == 0
+    assert fwd(rows=1, V=1 << 17, top=20) == 3 and fwd(rows=1, V=1 << 17, top=20, ws=P, n=need - 1) == 3
 
     assert fwd(V=0) == 1 and fwd(rows=-1) == 1 and fwd(stride=-1) == 1 and fwd(rows=1 << 31) == 1
     assert fwd(top=-1) == 1 and fwd(V=8, top=9) == 1 and fwd(top=33) == 2
