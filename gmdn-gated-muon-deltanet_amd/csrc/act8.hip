@@ -10,23 +10,39 @@ namespace gmdn {
 namespace {
 
 constexpr int A8_THREADS = 256;
-constexpr int A8_GROUPS = A8_THREADS / GROUP8_PIECES;  // groups of a workgroup
+constexpr int A8_PIECES = 2;  // pieces a thread has in flight, A8_THREADS apart
+constexpr int A8_SPAN = A8_THREADS * A8_PIECES;
+constexpr int64_t A8_GRID = 1 << 20;
 
-// The group, and the piece in it, of this thread: row, first column, values
-// of the piece (0: past the row's end), and the group's index in `scale`.
+// A piece's place.  Groups are 16 pieces; where rows are whole groups and lie
+// one after the other (`flat`), groups are numbered through the matrix.
 struct Place {
-  int64_t row, unit;
-  int c, n;
+  int64_t row, unit;  // the group's index in `scale`
+  int c, n;           // first column, values (0: past the row's or the matrix's end)
 };
-GMDN_DEV Place place(int64_t unit, int64_t d) {
-  const int64_t g = groups8(d);
+struct Shape {
+  int64_t units, d, groups;
+  bool flat;
+};
+GMDN_DEV Place place(int64_t piece, const Shape& s) {
   Place p;
-  p.unit = unit;
-  p.row = unit / g;
-  const int64_t c = (unit - p.row * g) * GROUP8 + 8 * (threadIdx.x % GROUP8_PIECES);
+  p.unit = piece / GROUP8_PIECES;
+  const int lane = (int)(piece % GROUP8_PIECES);
+  if (s.flat) {  // as one row
+    p.row = 0;
+    p.c = 0;
+    p.n = p.unit < s.units ? 8 : 0;
+    return p;
+  }
+  p.row = p.unit < ((int64_t)1 << 32) ? (uint32_t)p.unit / (uint32_t)s.groups : p.unit / s.groups;
+  const int64_t c = (p.unit - p.row * s.groups) * GROUP8 + 8 * lane;
   p.c = (int)c;
-  p.n = c < d ? (int)(d - c < 8 ? d - c : 8) : 0;
+  p.n = p.unit < s.units && c < s.d ? (int)(s.d - c < 8 ? s.d - c : 8) : 0;
   return p;
+}
+// Offsets of a piece in a matrix of row stride `stride`, and in a contiguous one.
+GMDN_DEV int64_t offset(const Place& p, int64_t piece, const Shape& s, int64_t stride) {
+  return s.flat ? piece * 8 : p.row * stride + p.c;
 }
 
 // GELU with the normal distribution function Phi, and its derivative
@@ -65,57 +81,81 @@ GMDN_DEV void gelu(float h, float& a, float& slope) {
   slope = __builtin_fmaf(h * (0.39894228040143268f * half), half, cdf);
 }
 
-template <typename T, bool GELU>
+template <typename T, bool GELU, bool FAR>
 __global__ void __launch_bounds__(A8_THREADS)
-pack(const T* __restrict__ x, T* __restrict__ a, int8_t* __restrict__ q, float* __restrict__ scale, int64_t units,
-     int64_t d, int64_t xs) {
-  for (int64_t u0 = (int64_t)blockIdx.x * A8_GROUPS; u0 < units; u0 += (int64_t)gridDim.x * A8_GROUPS) {
-    const int64_t u = u0 + threadIdx.x / GROUP8_PIECES;
-    if (u >= units) continue;  // whole groups of 16 lanes
-    const Place p = place(u, d);
-    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (p.n) load8(x + p.row * xs + p.c, p.n, v);
-    const Scale8 sc = scale8(lanes_max<GROUP8_PIECES>(amax_bits(v)));
-    if (threadIdx.x % GROUP8_PIECES == 0) scale[u] = sc.scale;
-    if (!p.n) continue;
-    const int64_t at = p.row * d + p.c;
-    store_q8(q + at, p.n, quant8(v, sc.inverse));
-    if constexpr (GELU) {
-      float y[8];
+pack(const T* __restrict__ x, T* __restrict__ a, int8_t* __restrict__ q, float* __restrict__ scale, Shape s,
+     int64_t xs) {
+  for (int64_t b0 = (int64_t)blockIdx.x * A8_SPAN; b0 < s.units * GROUP8_PIECES; b0 += (int64_t)gridDim.x * A8_SPAN) {
+    Raw8<T> raw[A8_PIECES];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) y[j] = gelu(v[j]);
-      store8(a + at, p.n, y);
+    for (int i = 0; i < A8_PIECES; ++i) {
+      const int64_t piece = b0 + i * A8_THREADS + threadIdx.x;
+      const Place p = place(piece, s);
+      const T* from = x + offset(p, piece, s, xs);
+      raw[i].template load<FAR>(from, p.n);
+    }
+#pragma unroll
+    for (int i = 0; i < A8_PIECES; ++i) {
+      const int64_t piece = b0 + i * A8_THREADS + threadIdx.x;
+      const Place p = place(piece, s);
+      float v[8];
+      raw[i].get(v);
+      const Scale8 sc = scale8(lanes_max<GROUP8_PIECES>(amax_bits(v)));
+      if (!p.n) continue;
+      if (piece % GROUP8_PIECES == 0) scale[p.unit] = sc.scale;
+      const int64_t at = offset(p, piece, s, s.d);
+      store_q8(q + at, p.n, quant8(v, sc.inverse));
+      if constexpr (GELU) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = gelu(v[j]);
+        stream8(a + at, p.n, v);
+      }
     }
   }
 }
 
 // UNPACK: x from the checkpoint.  Otherwise GELU's backward: dh, and the
 // output again where `a` is given.
-template <typename T, bool UNPACK>
+template <typename T, bool UNPACK, bool FAR>
 __global__ void __launch_bounds__(A8_THREADS)
 unpack(const int8_t* __restrict__ q, const float* __restrict__ scale, const T* __restrict__ da, int64_t das,
-       T* __restrict__ dh, T* __restrict__ a, int64_t units, int64_t d) {
-  for (int64_t u0 = (int64_t)blockIdx.x * A8_GROUPS; u0 < units; u0 += (int64_t)gridDim.x * A8_GROUPS) {
-    const int64_t u = u0 + threadIdx.x / GROUP8_PIECES;
-    if (u >= units) continue;
-    const Place p = place(u, d);
-    if (!p.n) continue;
-    const int64_t at = p.row * d + p.c;
-    float v[8];
-    dequant8(load_q8(q + at, p.n), scale[u], v);
-    if constexpr (UNPACK) {
-      store8(a + at, p.n, v);
-    } else {
-      float g[8], y[8];
-      load8(da + p.row * das + p.c, p.n, g);
+       T* __restrict__ dh, T* __restrict__ a, Shape s) {
+  for (int64_t b0 = (int64_t)blockIdx.x * A8_SPAN; b0 < s.units * GROUP8_PIECES; b0 += (int64_t)gridDim.x * A8_SPAN) {
+    Raw8<T> raw[A8_PIECES];
+    u32x2_any kept[A8_PIECES];
+    float sc[A8_PIECES];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        float slope;
-        gelu(v[j], y[j], slope);
-        g[j] *= slope;
+    for (int i = 0; i < A8_PIECES; ++i) {
+      const int64_t piece = b0 + i * A8_THREADS + threadIdx.x;
+      const Place p = place(piece, s);
+      kept[i] = load_q8(q + offset(p, piece, s, s.d), p.n);
+      sc[i] = p.n ? scale[p.unit] : 0.f;
+      if constexpr (!UNPACK) {
+        const T* from = da + offset(p, piece, s, das);
+        raw[i].template load<FAR>(from, p.n);
       }
-      store8(dh + at, p.n, g);
-      if (a) store8(a + at, p.n, y);
+    }
+#pragma unroll
+    for (int i = 0; i < A8_PIECES; ++i) {
+      const int64_t piece = b0 + i * A8_THREADS + threadIdx.x;
+      const Place p = place(piece, s);
+      if (!p.n) continue;
+      const int64_t at = offset(p, piece, s, s.d);
+      float v[8];
+      dequant8(kept[i], sc[i], v);
+      if constexpr (!UNPACK) {
+        float g[8];
+        raw[i].get(g);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          float y, slope;
+          gelu(v[j], y, slope);
+          g[j] *= slope;
+          v[j] = y;
+        }
+        stream8(dh + at, p.n, g);
+      }
+      if (UNPACK || a) stream8(a + at, p.n, v);
     }
   }
 }
@@ -126,9 +166,13 @@ int check8(int64_t rows, int64_t d, int64_t stride, int32_t dtype) {
   if (d >= ((int64_t)1 << 31) || rows > ((int64_t)1 << 40)) return GMDN_ERR_ARG;
   return GMDN_OK;
 }
-dim3 grid8(int64_t units) {
-  const int64_t n = (units + A8_GROUPS - 1) / A8_GROUPS;
-  return dim3((unsigned)(n < ((int64_t)1 << 30) ? n : (int64_t)1 << 30));
+Shape shape_of(int64_t rows, int64_t d, int64_t stride) {
+  const int64_t g = groups8(d);
+  return {rows * g, d, g, d % GROUP8 == 0 && (stride == d || rows == 1)};
+}
+dim3 grid8(const Shape& s) {
+  const int64_t n = (s.units * GROUP8_PIECES + A8_SPAN - 1) / A8_SPAN;
+  return dim3((unsigned)(n < A8_GRID ? n : A8_GRID));
 }
 
 template <bool GELU>
@@ -137,13 +181,16 @@ int pack_call(const void* x, void* a, int8_t* q, float* scale, int64_t rows, int
   const int rc = check8(rows, d, xs, dtype);
   if (rc != GMDN_OK || rows == 0) return rc;
   if (!x || !q || !scale || (GELU && !a)) return GMDN_ERR_ARG;
-  const int64_t units = rows * groups8(d);
-  if (dtype == GMDN_DTYPE_BF16)
-    hipLaunchKernelGGL((pack<bf16, GELU>), grid8(units), dim3(A8_THREADS), 0, (hipStream_t)stream, (const bf16*)x,
-                       (bf16*)a, q, scale, units, d, xs);
+  const Shape s = shape_of(rows, d, xs);
+  if (dtype == GMDN_DTYPE_BF16 && rows * d * 2 >= FAR_BYTES)
+    hipLaunchKernelGGL((pack<bf16, GELU, true>), grid8(s), dim3(A8_THREADS), 0, (hipStream_t)stream, (const bf16*)x,
+                       (bf16*)a, q, scale, s, xs);
+  else if (dtype == GMDN_DTYPE_BF16)
+    hipLaunchKernelGGL((pack<bf16, GELU, false>), grid8(s), dim3(A8_THREADS), 0, (hipStream_t)stream, (const bf16*)x,
+                       (bf16*)a, q, scale, s, xs);
   else
-    hipLaunchKernelGGL((pack<float, GELU>), grid8(units), dim3(A8_THREADS), 0, (hipStream_t)stream, (const float*)x,
-                       (float*)a, q, scale, units, d, xs);
+    hipLaunchKernelGGL((pack<float, GELU, false>), grid8(s), dim3(A8_THREADS), 0, (hipStream_t)stream, (const float*)x,
+                       (float*)a, q, scale, s, xs);
   return launched();
 }
 template <bool UNPACK>
@@ -152,13 +199,16 @@ int unpack_call(const int8_t* q, const float* scale, const void* da, int64_t das
   const int rc = check8(rows, d, das, dtype);
   if (rc != GMDN_OK || rows == 0) return rc;
   if (!q || !scale || (UNPACK ? !a : !da || !dh)) return GMDN_ERR_ARG;
-  const int64_t units = rows * groups8(d);
-  if (dtype == GMDN_DTYPE_BF16)
-    hipLaunchKernelGGL((unpack<bf16, UNPACK>), grid8(units), dim3(A8_THREADS), 0, (hipStream_t)stream, q, scale,
-                       (const bf16*)da, das, (bf16*)dh, (bf16*)a, units, d);
+  const Shape s = shape_of(rows, d, das);
+  if (!UNPACK && dtype == GMDN_DTYPE_BF16 && rows * d * 2 >= FAR_BYTES)
+    hipLaunchKernelGGL((unpack<bf16, UNPACK, !UNPACK>), grid8(s), dim3(A8_THREADS), 0, (hipStream_t)stream, q, scale,
+                       (const bf16*)da, das, (bf16*)dh, (bf16*)a, s);
+  else if (dtype == GMDN_DTYPE_BF16)
+    hipLaunchKernelGGL((unpack<bf16, UNPACK, false>), grid8(s), dim3(A8_THREADS), 0, (hipStream_t)stream, q, scale,
+                       (const bf16*)da, das, (bf16*)dh, (bf16*)a, s);
   else
-    hipLaunchKernelGGL((unpack<float, UNPACK>), grid8(units), dim3(A8_THREADS), 0, (hipStream_t)stream, q, scale,
-                       (const float*)da, das, (float*)dh, (float*)a, units, d);
+    hipLaunchKernelGGL((unpack<float, UNPACK, false>), grid8(s), dim3(A8_THREADS), 0, (hipStream_t)stream, q, scale,
+                       (const float*)da, das, (float*)dh, (float*)a, s);
   return launched();
 }
 
@@ -178,7 +228,7 @@ int gmdn_act8_pack(const void* x, int8_t* q, float* scale, int64_t rows, int64_t
 
 int gmdn_act8_unpack(const int8_t* q, const float* scale, void* x, int64_t rows, int64_t d, int32_t dtype,
                      void* stream) {
-  return unpack_call<true>(q, scale, nullptr, 0, nullptr, x, rows, d, dtype, stream);
+  return unpack_call<true>(q, scale, nullptr, d, nullptr, x, rows, d, dtype, stream);
 }
 
 int gmdn_gelu8_fwd(const void* h, void* a, int8_t* q, float* scale, int64_t rows, int64_t d, int64_t h_stride,

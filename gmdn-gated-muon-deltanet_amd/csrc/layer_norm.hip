@@ -14,7 +14,7 @@ namespace {
 
 constexpr int LN_THREADS = 512;      // threads of a workgroup, or a row's if more
 constexpr int LN_MAX_D = 16384;
-constexpr int LN_FWD_BLOCKS = 1024;
+constexpr int LN_FWD_BLOCKS = 512;
 constexpr int LN_BWD_BLOCKS = 256;   // of the backward: each writes 2 d partial sums
 
 constexpr int ln_threads(int tpr) { return tpr > LN_THREADS ? tpr : LN_THREADS; }
@@ -38,6 +38,23 @@ GMDN_DEV float row_sum(float x, float (*red)[16], int& slot) {
   return x;
 }
 
+// A thread's columns of weight and bias (1 and 0 without).
+template <int TPR, int NV>
+GMDN_DEV void load_weights(const void* w, const void* b, bool w16, int d, int t, float (&wv)[NV][8],
+                           float (&bv)[NV][8]) {
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = 8 * (i * TPR + t);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      wv[i][j] = 1.f;
+      bv[i][j] = 0.f;
+    }
+    if (c < d && w) load8_weight(w, w16, c, d - c, wv[i]);
+    if (c < d && b) load8_weight(b, w16, c, d - c, bv[i]);
+  }
+}
+
 // A row is TPR threads with NV pieces each, piece i of thread t at
 // i TPR + t; a workgroup takes its threads / TPR rows at a time.
 template <typename TX, typename TY, int TPR, int NV, bool PACK>
@@ -50,17 +67,7 @@ ln_fwd(const TX* __restrict__ x, const void* __restrict__ w, const void* __restr
   const int lr = threadIdx.x / TPR, t = threadIdx.x % TPR;
   int slot = 0;
   float wv[NV][8], bv[NV][8];
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int c = 8 * (i * TPR + t);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      wv[i][j] = 1.f;
-      bv[i][j] = 0.f;
-    }
-    if (c < d && w) load8_weight(w, w16, c, d - c, wv[i]);
-    if (c < d && b) load8_weight(b, w16, c, d - c, bv[i]);
-  }
+  load_weights<TPR, NV>(w, b, w16, d, t, wv, bv);
   // the next row's pieces are loaded before this row's sums
   Raw8<TX> raw[NV];
   auto fetch = [&](int64_t r) {
@@ -113,7 +120,7 @@ ln_fwd(const TX* __restrict__ x, const void* __restrict__ w, const void* __restr
       const int c = 8 * (i * TPR + t);
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[i][j] = (v[i][j] - m) * rs * wv[i][j] + bv[i][j];
-      if (live && c < d) store8(y + r * d + c, d - c, v[i]);
+      if (live && c < d) stream8(y + r * d + c, d - c, v[i]);
     }
     if (live && t == 0) {
       mean[r] = m;
@@ -220,7 +227,7 @@ ln_bwd(Src src, const TY* __restrict__ dy, int64_t ds, const void* __restrict__ 
       const int c = 8 * (i * TPR + t);
 #pragma unroll
       for (int j = 0; j < 8; ++j) g[i][j] = rs * (g[i][j] - mg - v[i][j] * mx);
-      if (live && c < d) store8(dx + r * d + c, d - c, g[i]);
+      if (live && c < d) stream8(dx + r * d + c, d - c, g[i]);
     }
   }
   if (!w) return;
@@ -305,31 +312,43 @@ ln_sums(const float* __restrict__ part, void* __restrict__ dw, void* __restrict_
   }
 }
 
-// y again from the checkpoint and the saved statistics; one piece a thread.
-template <typename TY>
-__global__ void __launch_bounds__(256)
+// y again from the checkpoint and the saved statistics.
+template <typename TY, int TPR, int NV>
+__global__ void __launch_bounds__(ln_threads(TPR))
 ln_rebuild(From8 src, const void* __restrict__ w, const void* __restrict__ b, bool w16,
            const float* __restrict__ mean, const float* __restrict__ rstd, TY* __restrict__ y, int64_t rows, int d) {
-  const int pieces = (d + 7) / 8;
-  const int64_t total = rows * pieces;
-  for (int64_t p = (int64_t)blockIdx.x * 256 + threadIdx.x; p < total; p += (int64_t)gridDim.x * 256) {
-    const int64_t r = p / pieces;
-    const int c = 8 * (int)(p - r * pieces);
-    float v[8], wv[8], bv[8];
-    From8::Raw raw;
-    raw.load(src, r, c, d - c, d);
-    raw.get(v);
-    const float m = mean[r], rs = rstd[r];
+  constexpr int RPB = ln_threads(TPR) / TPR;
+  const int lr = threadIdx.x / TPR, t = threadIdx.x % TPR;
+  float wv[NV][8], bv[NV][8];
+  load_weights<TPR, NV>(w, b, w16, d, t, wv, bv);
+  From8::Raw raw[NV];
+  float mr, rr;
+  auto fetch = [&](int64_t r) {
+    const bool live = r < rows;
+    mr = live ? mean[r] : 0.f;
+    rr = live ? rstd[r] : 0.f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      wv[j] = 1.f;
-      bv[j] = 0.f;
+    for (int i = 0; i < NV; ++i) {
+      const int c = 8 * (i * TPR + t);
+      raw[i].load(src, r, c, live ? d - c : 0, d);
     }
-    if (w) load8_weight(w, w16, c, d - c, wv);
-    if (b) load8_weight(b, w16, c, d - c, bv);
+  };
+  const int64_t step = (int64_t)gridDim.x * RPB;
+  int64_t r = (int64_t)blockIdx.x * RPB + lr;
+  fetch(r);
+  for (; r < rows; r += step) {
+    float v[NV][8];
+    const float m = mr, rs = rr;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = (v[j] - m) * rs * wv[j] + bv[j];
-    store8(y + r * d + c, d - c, v);
+    for (int i = 0; i < NV; ++i) raw[i].get(v[i]);
+    fetch(r + step);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = 8 * (i * TPR + t);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[i][j] = (v[i][j] - m) * rs * wv[i][j] + bv[i][j];
+      if (c < d) stream8(y + r * d + c, d - c, v[i]);
+    }
   }
 }
 
@@ -441,7 +460,7 @@ int gmdn_layer_norm_bwd(const void* dy, const void* x, const int8_t* q, const fl
       with_shape(d, [&](auto s) {
         using S = decltype(s);
         const dim3 grid((unsigned)nb), block(ln_threads(S::TPR));
-        if (q)
+              if (q)
           hipLaunchKernelGGL((ln_bwd<From8, TX, TY, S::TPR, S::NV>), grid, block, 0, st, From8{q, scale},
                              (const TY*)dy, dy_stride, weight, w16, mean, rstd, (TX*)dx, workspace, rows, (int)d);
         else
@@ -467,15 +486,18 @@ int gmdn_layer_norm8_rebuild(const int8_t* q, const float* scale, const void* we
   if (bias && !weight) return GMDN_ERR_ARG;
   if (rows == 0) return GMDN_OK;
   if (!q || !scale || !mean || !rstd || !y) return GMDN_ERR_ARG;
-  const int64_t blocks = (rows * ((d + 7) / 8) + 255) / 256;
-  const dim3 grid((unsigned)(blocks < (1 << 20) ? blocks : (1 << 20)));
+  const dim3 grid((unsigned)ln_blocks(rows, d, LN_FWD_BLOCKS));
   const bool w16 = w_type == GMDN_DTYPE_BF16;
-  if (y_type == GMDN_DTYPE_BF16)
-    hipLaunchKernelGGL(ln_rebuild<bf16>, grid, dim3(256), 0, (hipStream_t)stream, From8{q, scale}, weight, bias, w16,
-                       mean, rstd, (bf16*)y, rows, (int)d);
-  else
-    hipLaunchKernelGGL(ln_rebuild<float>, grid, dim3(256), 0, (hipStream_t)stream, From8{q, scale}, weight, bias, w16,
-                       mean, rstd, (float*)y, rows, (int)d);
+  with_shape(d, [&](auto s) {
+    using S = decltype(s);
+    const dim3 block(ln_threads(S::TPR));
+    if (y_type == GMDN_DTYPE_BF16)
+      hipLaunchKernelGGL((ln_rebuild<bf16, S::TPR, S::NV>), grid, block, 0, (hipStream_t)stream, From8{q, scale}, weight,
+                         bias, w16, mean, rstd, (bf16*)y, rows, (int)d);
+    else
+      hipLaunchKernelGGL((ln_rebuild<float, S::TPR, S::NV>), grid, block, 0, (hipStream_t)stream, From8{q, scale}, weight,
+                         bias, w16, mean, rstd, (float*)y, rows, (int)d);
+  });
   return launched();
 }
 

@@ -59,33 +59,31 @@ GMDN_DEV void add8(Sums& a, const float (&x)[8], float most) {
 }
 GMDN_DEV void add8(Sums& a, const float (&x)[8]) { add8(a, x, max8(x)); }
 
-// The row's sums from its threads': the maximum of all, then s and w at it.
-// A row of one wave needs no LDS.
+// The sums of N lanes' Sums, in each of them.
+template <int N>
+GMDN_DEV Sums join_lanes(Sums a) {
+  rescale(a, lanes_max<N>(a.m));
+  a.s = lanes_sum<N>(a.s);
+  a.w = lanes_sum<N>(a.w);
+  return a;
+}
+// The first wave's sums from the waves', in each of its lanes.
+template <int W>
+GMDN_DEV Sums join_waves(const Sums* waves) {
+  const Sums a = join_lanes<16>(lane_id() < W ? waves[lane_id()] : no_sums());
+  auto first = [](float x) { return float_of(__builtin_amdgcn_readfirstlane(bits_of(x))); };
+  return {first(a.m), first(a.s), first(a.w)};
+}
+// The sums of a row's NT threads, in its first wave: each wave its own, then
+// the first wave all of them (the work is small beside that of 16 waves doing
+// it side by side).  `waves` is LDS for a wave's each.
 template <int NT>
-GMDN_DEV Sums join(Sums a, float (*red)[16]) {
-  constexpr int W = NT / 64;
-  float m = lanes_max<64>(a.m);
-  if constexpr (W > 1) {
-    if (lane_id() == 0) red[0][wave_id()] = m;
+GMDN_DEV Sums join(Sums a, Sums* waves) {
+  a = join_lanes<64>(a);
+  if constexpr (NT > 64) {
+    if (lane_id() == 0) waves[wave_id()] = a;
     __syncthreads();
-#pragma unroll
-    for (int i = 0; i < W; ++i) m = fmaxf(m, red[0][i]);
-  }
-  rescale(a, m);
-  a.s = lanes_sum<64>(a.s);
-  a.w = lanes_sum<64>(a.w);
-  if constexpr (W > 1) {
-    if (lane_id() == 0) {
-      red[1][wave_id()] = a.s;
-      red[2][wave_id()] = a.w;
-    }
-    __syncthreads();
-    a.s = a.w = 0.f;
-#pragma unroll
-    for (int i = 0; i < W; ++i) {
-      a.s += red[1][i];
-      a.w += red[2][i];
-    }
+    if (wave_id() == 0) a = join_waves<NT / 64>(waves);
   }
   return a;
 }
@@ -136,14 +134,14 @@ struct Parts {
 };
 
 // The sums of columns first .. last - 1 of a row by NT threads.
-template <typename T, int NT>
+template <typename T, int NT, bool FAR>
 GMDN_DEV Sums sums_of(const T* x, int first, int last, int t) {
   Sums a = no_sums();
   int c0 = first + 8 * t;
   for (; c0 + 8 * NT * (PIECES - 1) + 8 <= last; c0 += 8 * NT * PIECES) {
     Raw8<T> raw[PIECES];
 #pragma unroll
-    for (int i = 0; i < PIECES; ++i) raw[i].stream(x + c0 + 8 * NT * i);
+    for (int i = 0; i < PIECES; ++i) raw[i].template load<FAR>(x + c0 + 8 * NT * i, 8);
 #pragma unroll
     for (int i = 0; i < PIECES; ++i) {
       float v[8];
@@ -161,10 +159,10 @@ GMDN_DEV Sums sums_of(const T* x, int first, int last, int t) {
 
 // A row is TPR threads of the workgroup's 256 (SPLIT: 256 for a part of it).
 constexpr int LP_THREADS = 256;
-template <typename T, int TPR, bool SPLIT>
+template <typename T, int TPR, bool SPLIT, bool FAR>
 __global__ void __launch_bounds__(LP_THREADS)
 lp_fwd(const T* __restrict__ logits, int64_t stride, int64_t rows, Out out, Parts parts) {
-  __shared__ float red[3][16];
+  __shared__ Sums waves[LP_THREADS / 64];
   const int64_t item = (int64_t)blockIdx.x * (LP_THREADS / TPR) + threadIdx.x / TPR;
   const int t = threadIdx.x % TPR;
   if (item >= rows * (SPLIT ? parts.parts : 1)) return;  // whole waves, and of rows of one wave only
@@ -172,7 +170,7 @@ lp_fwd(const T* __restrict__ logits, int64_t stride, int64_t rows, Out out, Part
   const int first = SPLIT ? (int)(item - row * parts.parts) * parts.span : 0;
   const int last = SPLIT && first + parts.span < out.V ? first + parts.span : out.V;
   const T* x = logits + row * stride;
-  const Sums a = join<TPR>(sums_of<T, TPR>(x, first, last, t), red);
+  const Sums a = join<TPR>(sums_of<T, TPR, FAR>(x, first, last, t), waves);
   if (t != 0) return;
   if constexpr (SPLIT)
     parts.sums[item] = a;
@@ -211,15 +209,18 @@ GMDN_DEV uint64_t lanes_max64(uint64_t x) {
 
 constexpr int TOP_MAX = 32;
 constexpr int TOP_LIST = 1024;  // candidates of a tile
+constexpr int TOP_PIECES = 256;  // and pieces that they come from
 
 struct TopLds {
+  float piece[TOP_PIECES][8];
+  int column[TOP_PIECES];
   uint64_t groups[64];
   uint64_t list[TOP_LIST + TOP_MAX];
   uint64_t run[TOP_MAX];  // the best so far, in order
   uint64_t bound;
   uint64_t red64[16];
-  float red[3][16];
-  int count;
+  Sums waves[16];
+  int pieces, count, nan;
 };
 
 // The n keys of the list by rank into run: a key's rank is the number of
@@ -268,7 +269,8 @@ GMDN_DEV void slow_top(const T* x, int first, int last, int top, TopLds& lds) {
 // better logit of that value exceeds: equal logits, masked ones above all,
 // stay out of the list by their index.  Those that reach the bound join the best
 // of the tiles before in the list, which is ranked.  A tile that gives more
-// than the list holds, or a NaN, is left to slow_top.
+// than LDS holds, or a NaN, is left to slow_top.  The sums are returned in the
+// first wave.
 template <typename T, int NT>
 GMDN_DEV Sums top_of(const T* x, int first, int last, int top, TopLds& lds, int& have) {
   const int tid = threadIdx.x;
@@ -276,7 +278,7 @@ GMDN_DEV Sums top_of(const T* x, int first, int last, int top, TopLds& lds, int&
   have = 0;
   bool over = false;
   if (tid < 64) lds.groups[tid] = 0;
-  if (tid == 0) lds.count = 0;
+  if (tid == 0) lds.pieces = lds.count = lds.nan = 0;
   __syncthreads();
   for (int c0 = first; c0 < last; c0 += 8 * NT * PIECES) {
     Raw8<T> raw[PIECES];
@@ -284,10 +286,7 @@ GMDN_DEV Sums top_of(const T* x, int first, int last, int top, TopLds& lds, int&
 #pragma unroll
     for (int i = 0; i < PIECES; ++i) {
       const int c = c0 + 8 * (i * NT + tid);
-      if (c + 8 <= last)
-        raw[i].stream(x + c);
-      else
-        raw[i].load(x + c, last - c, -INFINITY);
+      raw[i].load(x + c, last - c, -INFINITY);
     }
     // the thread's best: its value, and the first piece that has it
     float bv = -INFINITY;
@@ -321,52 +320,41 @@ GMDN_DEV Sums top_of(const T* x, int first, int last, int top, TopLds& lds, int&
     }
     __syncthreads();
     if (tid < 64) lds.groups[tid] = 0;
-    // candidates: by value first, then by key; places in the list by one
-    // addition a wave
+    // the pieces that hold candidates go to LDS, where each of their values is
+    // a thread's: by value, and for the bound's own value by index
     const uint64_t least = lds.bound;
     const float lv = value_of(least);
-    uint32_t found = 0;
+    const int upto = least ? index_of(least) : 0x7fffffff;
 #pragma unroll
     for (int i = 0; i < PIECES; ++i) {
-      if (!(most[i] >= lv)) continue;
-      float v[8];
-      raw[i].get(v);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int c = c0 + 8 * (i * NT + tid) + j;
-        if (c < last && key_of(v[j], c) >= least) found |= 1u << (8 * i + j);
+      const int c = c0 + 8 * (i * NT + tid);
+      if ((most[i] > lv || (most[i] == lv && c <= upto)) && c < last) {
+        const int at = atomicAdd(&lds.pieces, 1);
+        if (at < TOP_PIECES) {
+          float v[8];
+          raw[i].get(v);
+          *reinterpret_cast<f32x4*>(&lds.piece[at][0]) = f32x4{v[0], v[1], v[2], v[3]};
+          *reinterpret_cast<f32x4*>(&lds.piece[at][4]) = f32x4{v[4], v[5], v[6], v[7]};
+          lds.column[at] = c;
+        }
       }
     }
-    if (__ballot(found != 0)) {
-      const int mine = __popc(found);
-      int upto = mine;  // of lanes up to this one
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const int y = __shfl_up(upto, o, 64);
-        if (lane_id() >= o) upto += y;
-      }
-      int at = 0;
-      if (lane_id() == 63) at = atomicAdd(&lds.count, upto);
-      at = __shfl(at, 63, 64) + upto - mine;
-#pragma unroll
-      for (int i = 0; i < PIECES; ++i) {
-        if (!(found >> (8 * i) & 0xff)) continue;
-        float v[8];
-        raw[i].get(v);
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (found >> (8 * i + j) & 1) {
-            if (at < TOP_LIST) lds.list[at] = key_of(v[j], c0 + 8 * (i * NT + tid) + j);
-            ++at;
-          }
+    __syncthreads();
+    const int np = lds.pieces;
+    for (int e = tid; e < 8 * np && np <= TOP_PIECES; e += NT) {
+      const float v = lds.piece[e / 8][e % 8];
+      const int c = lds.column[e / 8] + e % 8;
+      if ((v > lv || (v == lv && c <= upto)) && c < last) {
+        const int at = atomicAdd(&lds.count, 1);
+        if (at < TOP_LIST) lds.list[at] = key_of(v, c);
       }
     }
     __syncthreads();
     int n = lds.count;
-    over = n > TOP_LIST;
+    over = n > TOP_LIST || np > TOP_PIECES;
     if (!over && tid < have) lds.list[n + tid] = lds.run[tid];
     __syncthreads();
-    if (tid == 0) lds.count = 0;
+    if (tid == 0) lds.pieces = lds.count = 0;
     if (!over) {
       n += have;
       rank_list<NT>(lds, n, top);
@@ -374,12 +362,17 @@ GMDN_DEV Sums top_of(const T* x, int first, int last, int top, TopLds& lds, int&
     }
     __syncthreads();
   }
-  a = join<NT>(a, lds.red);
-  if (over || a.s != a.s) {
-    slow_top<T, NT>(x, first, last, top < last - first ? top : last - first, lds);
-    have = top < last - first ? top : last - first;
+  a = join_lanes<64>(a);
+  if (lane_id() == 0) {
+    lds.waves[wave_id()] = a;
+    if (a.s != a.s) lds.nan = 1;
   }
-  return a;
+  __syncthreads();
+  if (over || lds.nan) {
+    have = top < last - first ? top : last - first;
+    slow_top<T, NT>(x, first, last, have, lds);
+  }
+  return join_waves<NT / 64>(lds.waves);
 }
 
 template <typename T, int NT, bool SPLIT>
@@ -392,6 +385,7 @@ lp_top(const T* __restrict__ logits, int64_t stride, Out out, Parts parts) {
   const T* x = logits + row * stride;
   int have;
   const Sums a = top_of<T, NT>(x, first, last, out.top, lds, have);
+  if (wave_id() > 0) return;
   const int i = threadIdx.x;
   if constexpr (SPLIT) {
     if (i == 0) parts.sums[item] = a;
@@ -405,22 +399,24 @@ lp_top(const T* __restrict__ logits, int64_t stride, Out out, Parts parts) {
 
 // A row's outputs from its parts.
 constexpr int MAX_PARTS = 32;
+constexpr int JOIN_THREADS = 1024;
 template <typename T>
-__global__ void __launch_bounds__(LP_THREADS)
+__global__ void __launch_bounds__(JOIN_THREADS)
 lp_join(const T* __restrict__ logits, int64_t stride, Out out, Parts parts) {
   static_assert(MAX_PARTS * TOP_MAX <= TOP_LIST, "the parts' best fit the list");
   __shared__ TopLds lds;
   const int64_t row = blockIdx.x;
   const T* x = logits + row * stride;
   const int n = parts.parts * out.top;
-  for (int i = threadIdx.x; i < n; i += LP_THREADS) lds.list[i] = parts.best[row * n + i];
+  for (int i = threadIdx.x; i < n; i += JOIN_THREADS) lds.list[i] = parts.best[row * n + i];
   Sums a = no_sums();
   if ((int)threadIdx.x < parts.parts) a = parts.sums[row * parts.parts + threadIdx.x];
-  const Row r = row_of(join<LP_THREADS>(a, lds.red));
-  if (threadIdx.x == 0) out.row(row, r, x);
-  if (n == 0) return;
-  rank_list<LP_THREADS>(lds, n, out.top);
+  a = join<JOIN_THREADS>(a, lds.waves);
+  rank_list<JOIN_THREADS>(lds, n, out.top);
   __syncthreads();
+  if (wave_id() > 0) return;
+  const Row r = row_of(a);
+  if (threadIdx.x == 0) out.row(row, r, x);
   if ((int)threadIdx.x < out.top) out.alternative(row, threadIdx.x, index_of(lds.run[threadIdx.x]), r, x);
 }
 
@@ -469,13 +465,13 @@ lp_bwd(const T* __restrict__ logits, int64_t stride, int64_t rows, const int64_t
   for (; c0 + 8 * TPR * (PIECES - 1) + 8 <= last; c0 += 8 * TPR * PIECES) {
     Raw8<T> raw[PIECES];
 #pragma unroll
-    for (int i = 0; i < PIECES; ++i) raw[i].stream(x + c0 + 8 * TPR * i);
+    for (int i = 0; i < PIECES; ++i) raw[i].load(x + c0 + 8 * TPR * i, 8);
 #pragma unroll
     for (int i = 0; i < PIECES; ++i) {
       float v[8];
       raw[i].get(v);
       grad8(v, c0 + 8 * TPR * i);
-      stream8(out + c0 + 8 * TPR * i, v);
+      stream8(out + c0 + 8 * TPR * i, 8, v);
     }
   }
   for (; c0 < last; c0 += 8 * TPR) {
@@ -524,18 +520,22 @@ void fwd_launch(const T* x, int64_t stride, int64_t rows, const Out& out, Parts 
   if (out.top > 0) {
     if (split)
       hipLaunchKernelGGL((lp_top<T, 1024, true>), grid, dim3(1024), 0, st, x, stride, out, p);
-    else if (out.V <= 8 * 256 * PIECES || rows > 256)
-      hipLaunchKernelGGL((lp_top<T, 256, false>), grid, block, 0, st, x, stride, out, p);
+    else if (out.V <= 8 * 256 * PIECES)
+      hipLaunchKernelGGL((lp_top<T, 256, false>), grid, dim3(256), 0, st, x, stride, out, p);
+    else if (rows > 256)
+      hipLaunchKernelGGL((lp_top<T, 512, false>), grid, dim3(512), 0, st, x, stride, out, p);
     else
       hipLaunchKernelGGL((lp_top<T, 1024, false>), grid, dim3(1024), 0, st, x, stride, out, p);
   } else if (split) {
-    hipLaunchKernelGGL((lp_fwd<T, 256, true>), grid, block, 0, st, x, stride, rows, out, p);
+    hipLaunchKernelGGL((lp_fwd<T, 256, true, false>), grid, block, 0, st, x, stride, rows, out, p);
   } else if (out.V <= ONE_WAVE) {
-    hipLaunchKernelGGL((lp_fwd<T, 64, false>), dim3((unsigned)((rows + 3) / 4)), block, 0, st, x, stride, rows, out, p);
+    hipLaunchKernelGGL((lp_fwd<T, 64, false, false>), dim3((unsigned)((rows + 3) / 4)), block, 0, st, x, stride, rows, out, p);
+  } else if (sizeof(T) == 2 && rows * out.V * 2 >= FAR_BYTES) {
+    hipLaunchKernelGGL((lp_fwd<T, 256, false, sizeof(T) == 2>), grid, block, 0, st, x, stride, rows, out, p);
   } else {
-    hipLaunchKernelGGL((lp_fwd<T, 256, false>), grid, block, 0, st, x, stride, rows, out, p);
+    hipLaunchKernelGGL((lp_fwd<T, 256, false, false>), grid, block, 0, st, x, stride, rows, out, p);
   }
-  if (split) hipLaunchKernelGGL((lp_join<T>), dim3((unsigned)rows), block, 0, st, x, stride, out, p);
+  if (split) hipLaunchKernelGGL((lp_join<T>), dim3((unsigned)rows), dim3(JOIN_THREADS), 0, st, x, stride, out, p);
 }
 
 template <typename T>

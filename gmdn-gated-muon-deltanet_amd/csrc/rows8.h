@@ -53,16 +53,6 @@ GMDN_DEV void store8(bf16* p, int n, const float (&x)[8]) {
       if (j < n) p[j] = v[j];
   }
 }
-// The same for a whole piece that is not read again soon (nontemporal).
-GMDN_DEV void stream8(bf16* p, const float (&x)[8]) {
-  const bf16x8_any v = cat8(to_bf16x4(f32x4{x[0], x[1], x[2], x[3]}), to_bf16x4(f32x4{x[4], x[5], x[6], x[7]}));
-  __builtin_nontemporal_store(v, reinterpret_cast<bf16x8_any*>(p));
-}
-GMDN_DEV void stream8(float* p, const float (&x)[8]) {
-  f32x4_any* q = reinterpret_cast<f32x4_any*>(p);
-  __builtin_nontemporal_store(f32x4_any{x[0], x[1], x[2], x[3]}, q);
-  __builtin_nontemporal_store(f32x4_any{x[4], x[5], x[6], x[7]}, q + 1);
-}
 GMDN_DEV void store8(float* p, int n, const float (&x)[8]) {
   if (n >= 8) {
     *reinterpret_cast<f32x4_any*>(p) = f32x4{x[0], x[1], x[2], x[3]};
@@ -73,20 +63,40 @@ GMDN_DEV void store8(float* p, int n, const float (&x)[8]) {
       if (j < n) p[j] = x[j];
   }
 }
+// The same past the caches (nontemporal) for outputs that a kernel does not
+// read again.  bf16 only: a wave's pieces fill whole lines in one instruction.  The
+// two halves of float32 pieces do not, and went slower so (a layer norm's dx
+// at 16384 x 2048: 89 us, with plain stores 80; bf16 at 16384 x 1024: 35 and 39).
+GMDN_DEV void stream8(bf16* p, int n, const float (&x)[8]) {
+  if (n >= 8) {
+    const bf16x8_any v = cat8(to_bf16x4(f32x4{x[0], x[1], x[2], x[3]}), to_bf16x4(f32x4{x[4], x[5], x[6], x[7]}));
+    __builtin_nontemporal_store(v, reinterpret_cast<bf16x8_any*>(p));
+  } else {
+    store8(p, n, x);
+  }
+}
+GMDN_DEV void stream8(float* p, int n, const float (&x)[8]) { store8(p, n, x); }
+
 // A piece as it lies in memory, for loads that are to be in flight over other
-// work; values from n on are `pad` (0 or an infinity).  `stream` loads a whole piece that is not
-// wanted again soon (nontemporal).
+// work; values from n on are `pad` (0 or an infinity).  FAR: whole bf16 pieces are
+// loaded past the caches (nontemporal), for matrices of at least FAR_BYTES:
+// what the last kernel left in the 256 MB cache is then little of them, and
+// the outputs keep it.  GELU's backward at 16384 x 4096 takes 76 us so and 83 us
+// without; at 16384 x 1024, 24 and 21.
+constexpr int64_t FAR_BYTES = 96 << 20;
 template <typename T>
 struct Raw8;
 template <>
 struct Raw8<bf16> {
   u32x4 v;
-  GMDN_DEV void stream(const bf16* p) {
-    v = __builtin_nontemporal_load(reinterpret_cast<const u32x4_any*>(p));
-  }
+  template <bool FAR = false>
   GMDN_DEV void load(const bf16* p, int n, float pad = 0.f) {
+    const u32x4_any* q = reinterpret_cast<const u32x4_any*>(p);
     if (n >= 8) {
-      v = *reinterpret_cast<const u32x4_any*>(p);
+      if constexpr (FAR)
+        v = __builtin_nontemporal_load(q);
+      else
+        v = *q;
     } else {
       const uint32_t bits = __builtin_bit_cast(uint32_t, pad) >> 16;
       const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
@@ -106,16 +116,10 @@ struct Raw8<bf16> {
 template <>
 struct Raw8<float> {
   float v[8];
-  GMDN_DEV void stream(const float* p) {
-    const f32x4_any* q = reinterpret_cast<const f32x4_any*>(p);
-    const f32x4_any a = __builtin_nontemporal_load(q), b = __builtin_nontemporal_load(q + 1);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      v[j] = a[j];
-      v[4 + j] = b[j];
-    }
+  template <bool FAR = false>
+  GMDN_DEV void load(const float* p, int n, float pad = 0.f) {
+    load8(p, n, v, pad);
   }
-  GMDN_DEV void load(const float* p, int n, float pad = 0.f) { load8(p, n, v, pad); }
   GMDN_DEV void get(float (&x)[8]) const {
 #pragma unroll
     for (int j = 0; j < 8; ++j) x[j] = v[j];
@@ -213,27 +217,43 @@ GMDN_DEV u32x2_any load_q8(const int8_t* p, int n) {
 }
 
 // ------------------------------------------------- over the threads of a row
-// Sum over aligned groups of N lanes (N a power of two up to 64).
-template <int N>
-GMDN_DEV float lanes_sum(float x) {
-#pragma unroll
-  for (int o = 1; o < N; o <<= 1) x += __shfl_xor(x, o, 64);
-  return x;
+// Over aligned groups of N lanes (N a power of two up to 64), the result in
+// each of them: within 16 lanes by DPP (the quad's neighbours, then mirrors of 8 and
+// 16: once a quad agrees, a mirror pairs it with another), the rows of 16 of a
+// wave through scalar registers.  A butterfly of LDS permutes instead costs its
+// latency at every step: in a workgroup of 16 waves the three reductions of a
+// row of logits took 6400 cycles so.
+template <int CTRL>
+GMDN_DEV uint32_t dpp(uint32_t x) {
+  return (uint32_t)__builtin_amdgcn_update_dpp((int)x, (int)x, CTRL, 0xf, 0xf, false);
 }
-template <int N>
-GMDN_DEV uint32_t lanes_max(uint32_t x) {
-#pragma unroll
-  for (int o = 1; o < N; o <<= 1) {
-    const uint32_t y = (uint32_t)__shfl_xor((int)x, o, 64);
-    x = y > x ? y : x;
+template <int N, class F>
+GMDN_DEV uint32_t lanes_fold(uint32_t x, F&& f) {
+  if constexpr (N > 1) x = f(x, dpp<0xb1>(x));   // quad_perm 1 0 3 2
+  if constexpr (N > 2) x = f(x, dpp<0x4e>(x));   // quad_perm 2 3 0 1
+  if constexpr (N > 4) x = f(x, dpp<0x141>(x));  // row_half_mirror
+  if constexpr (N > 8) x = f(x, dpp<0x140>(x));  // row_mirror
+  if constexpr (N == 32) x = f(x, (uint32_t)__shfl_xor((int)x, 16, 64));
+  if constexpr (N == 64) {
+    const uint32_t a = __builtin_amdgcn_readlane(x, 0), b = __builtin_amdgcn_readlane(x, 16),
+                   c = __builtin_amdgcn_readlane(x, 32), d = __builtin_amdgcn_readlane(x, 48);
+    x = f(f(a, b), f(c, d));
   }
   return x;
 }
+GMDN_DEV uint32_t bits_of(float x) { return __builtin_bit_cast(uint32_t, x); }
+GMDN_DEV float float_of(uint32_t x) { return __builtin_bit_cast(float, x); }
+template <int N>
+GMDN_DEV float lanes_sum(float x) {
+  return float_of(lanes_fold<N>(bits_of(x), [](uint32_t a, uint32_t b) { return bits_of(float_of(a) + float_of(b)); }));
+}
+template <int N>
+GMDN_DEV uint32_t lanes_max(uint32_t x) {
+  return lanes_fold<N>(x, [](uint32_t a, uint32_t b) { return b > a ? b : a; });
+}
 template <int N>
 GMDN_DEV float lanes_max(float x) {
-#pragma unroll
-  for (int o = 1; o < N; o <<= 1) x = fmaxf(x, __shfl_xor(x, o, 64));
-  return x;
+  return float_of(lanes_fold<N>(bits_of(x), [](uint32_t a, uint32_t b) { return bits_of(fmaxf(float_of(a), float_of(b))); }));
 }
 
 // Element type codes of the C-ABI.
