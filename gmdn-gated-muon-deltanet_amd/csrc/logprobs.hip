@@ -44,20 +44,18 @@ GMDN_DEV float max3(float a, float b, float c) {
   asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
   return r;
 }
-GMDN_DEV float max8(const float (&x)[8]) {
-  return max3(max3(x[0], x[1], x[2]), max3(x[3], x[4], x[5]), fmaxf(x[6], x[7]));
+GMDN_DEV float max8(const float (&x)[8], float m) {
+  return max3(max3(x[0], x[1], x[2]), max3(x[3], x[4], x[5]), max3(x[6], x[7], m));
 }
-GMDN_DEV void add8(Sums& a, const float (&x)[8], float most) {
-  const float m = fmaxf(a.m, most);
-  rescale(a, m);
+// The terms of a piece at the maximum that `a` has.
+GMDN_DEV void terms8(Sums& a, const float (&x)[8]) {
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    const float u = x[j] - m, e = exp_of(u);
+    const float u = x[j] - a.m, e = exp_of(u);
     a.s += e;
     a.w += e * fmaxf(u, FAR);
   }
 }
-GMDN_DEV void add8(Sums& a, const float (&x)[8]) { add8(a, x, max8(x)); }
 
 // The sums of N lanes' Sums, in each of them.
 template <int N>
@@ -79,7 +77,7 @@ GMDN_DEV Sums join_waves(const Sums* waves) {
 // it side by side).  `waves` is LDS for a wave's each.
 template <int NT>
 GMDN_DEV Sums join(Sums a, Sums* waves) {
-  a = join_lanes<64>(a);
+  a = join_lanes<(NT < 64 ? NT : 64)>(a);
   if constexpr (NT > 64) {
     if (lane_id() == 0) waves[wave_id()] = a;
     __syncthreads();
@@ -142,17 +140,21 @@ GMDN_DEV Sums sums_of(const T* x, int first, int last, int t) {
     Raw8<T> raw[PIECES];
 #pragma unroll
     for (int i = 0; i < PIECES; ++i) raw[i].template load<FAR>(x + c0 + 8 * NT * i, 8);
+    float v[PIECES][8], m = a.m;
 #pragma unroll
     for (int i = 0; i < PIECES; ++i) {
-      float v[8];
-      raw[i].get(v);
-      add8(a, v);
+      raw[i].get(v[i]);
+      m = max8(v[i], m);
     }
+    rescale(a, m);  // once for all of them
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) terms8(a, v[i]);
   }
   for (; c0 < last; c0 += 8 * NT) {
     float v[8];
     load8(x + c0, last - c0, v, -INFINITY);
-    add8(a, v);
+    rescale(a, max8(v, a.m));
+    terms8(a, v);
   }
   return a;
 }
@@ -165,7 +167,7 @@ lp_fwd(const T* __restrict__ logits, int64_t stride, int64_t rows, Out out, Part
   __shared__ Sums waves[LP_THREADS / 64];
   const int64_t item = (int64_t)blockIdx.x * (LP_THREADS / TPR) + threadIdx.x / TPR;
   const int t = threadIdx.x % TPR;
-  if (item >= rows * (SPLIT ? parts.parts : 1)) return;  // whole waves, and of rows of one wave only
+  if (item >= rows * (SPLIT ? parts.parts : 1)) return;  // rows of no more than a wave only
   const int64_t row = SPLIT ? item / parts.parts : item;
   const int first = SPLIT ? (int)(item - row * parts.parts) * parts.span : 0;
   const int last = SPLIT && first + parts.span < out.V ? first + parts.span : out.V;
@@ -295,8 +297,9 @@ GMDN_DEV Sums top_of(const T* x, int first, int last, int top, TopLds& lds, int&
     for (int i = 0; i < PIECES; ++i) {
       float v[8];
       raw[i].get(v);
-      most[i] = max8(v);
-      add8(a, v, most[i]);
+      most[i] = max8(v, -INFINITY);
+      rescale(a, max3(a.m, most[i], most[i]));
+      terms8(a, v);
       if (most[i] > bv) {
         bv = most[i];
         bp = i;
@@ -432,7 +435,7 @@ lp_bwd(const T* __restrict__ logits, int64_t stride, int64_t rows, const int64_t
        T* __restrict__ dx, int V, int top, int64_t ignore, int span, int parts) {
   const int64_t item = (int64_t)blockIdx.x * (NT / TPR) + threadIdx.x / TPR;
   const int t = threadIdx.x % TPR;
-  if (item >= rows * parts) return;  // rows of one wave only
+  if (item >= rows * parts) return;  // rows of no more than a wave only
   const int64_t row = item / parts;
   const int first = (int)(item - row * parts) * span, last = first + span < V ? first + span : V;
   const T* x = logits + row * stride;
@@ -505,7 +508,7 @@ int check_lp(int64_t rows, int64_t V, int64_t stride, int32_t top, int32_t dtype
 
 // Workgroups of a row in the forward.
 constexpr int64_t SPLIT_GRID = 512, SPLIT_SPAN = 16384;
-constexpr int64_t ONE_WAVE = 2048;  // rows of at most so many logits are a wave's
+constexpr int64_t SMALL_ROW = 512, ONE_WAVE = 4096;  // rows of at most so many logits are 16 lanes', a wave's
 int parts_of(int64_t rows, int64_t V) {
   const int64_t room = SPLIT_GRID / rows, most = V / SPLIT_SPAN;
   const int64_t n = room < most ? room : most;
@@ -528,6 +531,9 @@ void fwd_launch(const T* x, int64_t stride, int64_t rows, const Out& out, Parts 
       hipLaunchKernelGGL((lp_top<T, 1024, false>), grid, dim3(1024), 0, st, x, stride, out, p);
   } else if (split) {
     hipLaunchKernelGGL((lp_fwd<T, 256, true, false>), grid, block, 0, st, x, stride, rows, out, p);
+  } else if (out.V <= SMALL_ROW) {
+    hipLaunchKernelGGL((lp_fwd<T, 16, false, false>), dim3((unsigned)((rows + 15) / 16)), block, 0, st, x, stride, rows,
+                       out, p);
   } else if (out.V <= ONE_WAVE) {
     hipLaunchKernelGGL((lp_fwd<T, 64, false, false>), dim3((unsigned)((rows + 3) / 4)), block, 0, st, x, stride, rows, out, p);
   } else if (sizeof(T) == 2 && rows * out.V * 2 >= FAR_BYTES) {
@@ -555,6 +561,8 @@ void bwd_launch(const T* x, int64_t stride, int64_t rows, const int64_t* tokens,
                      ignore, span, (int)parts)
   if (alternatives)
     GMDN_LP_BWD(256, 256, true);
+  else if (V <= SMALL_ROW)
+    GMDN_LP_BWD(256, 16, false);
   else if (V <= ONE_WAVE)
     GMDN_LP_BWD(256, 64, false);
   else if (V <= 8 * 256 * PIECES)

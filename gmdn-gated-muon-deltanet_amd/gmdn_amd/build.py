@@ -75,7 +75,7 @@ def _link_ops(objs: list[str], verbose: bool) -> None:
     lib = os.path.join(os.path.dirname(torch.__file__), "lib")
     tmp = OPS_OUT + ".tmp"
     _run([os.environ.get("CXX", "g++"), "-shared", *objs, "-o", tmp, "-L", lib, "-ltorch", "-ltorch_cpu", "-lc10",
-          "-lc10_hip", "-L", HERE, "-lgmdn_scan", "-Wl,-rpath,$ORIGIN"], "linking the torch operators", verbose)
+          "-lc10_hip", "-ltorch_hip", "-L", HERE, "-lgmdn_scan", "-Wl,-rpath,$ORIGIN"], "linking the torch operators", verbose)
     os.replace(tmp, OPS_OUT)
 
 

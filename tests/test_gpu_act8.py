@@ -183,6 +183,23 @@ def test_gelu_derivative_against_differences():
     assert ((dh.double() - d1).abs() <= (d2 - d1).abs() + rounding).all()
 
 
+def test_large_matrices_equal_their_parts():
+    """Beyond 96 MB activations are loaded past the caches: the same bits."""
+    dev = _dev()
+    gen = torch.Generator(device=dev).manual_seed(4)
+    h = torch.randn(13000, 4000, generator=gen, device=dev).bfloat16()
+    dy = torch.randn(13000, 4000, generator=gen, device=dev).bfloat16()
+
+    def both(h, dy):
+        a, q, s = torch.ops.gmdn.gelu8_fwd(h)
+        return (a, q, s, *torch.ops.gmdn.act8_pack(h), *torch.ops.gmdn.gelu8_bwd(dy, q, s, True))
+
+    whole = both(h, dy)
+    for a in (0, 12000):
+        part = both(h[a:a + 1000], dy[a:a + 1000])
+        assert all(torch.equal(w[a:a + 1000], p) for w, p in zip(whole, part))
+
+
 def test_deterministic_and_on_another_stream():
     dev = _dev()
     h, dy = values((3000, 1000), 1, torch.bfloat16).to(dev), values((3000, 1000), 2, torch.bfloat16).to(dev)

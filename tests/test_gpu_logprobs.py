@@ -178,6 +178,24 @@ def test_ties_and_orders(V):
         check(x.bfloat16(), tokens, top)
 
 
+@pytest.mark.parametrize("rows,V,top", [(300, 9001, 5), (300, 40000, 32), (700, 300, 0), (300, 5000, 20)])
+def test_many_rows(rows, V, top):
+    """Row counts that take other shapes of workgroup than a few rows do."""
+    check(*logits((rows, V), rows + V, torch.bfloat16), top)
+
+
+def test_large_matrices_equal_their_parts():
+    """Beyond 96 MB logits are loaded past the caches: the same bits."""
+    dev = _dev()
+    gen = torch.Generator(device=dev).manual_seed(4)
+    x = (3 * torch.randn(1700, 32000, generator=gen, device=dev)).bfloat16()
+    tokens = torch.randint(32000, (1700,), generator=gen, device=dev)
+    got = lp.token_logprobs(x, tokens)
+    for a in (0, 1500):
+        part = lp.token_logprobs(x[a:a + 200], tokens[a:a + 200])
+        assert torch.equal(got.logprob[a:a + 200], part.logprob) and torch.equal(got.entropy[a:a + 200], part.entropy)
+
+
 def test_large_and_peaked_logits():
     """Logits far from zero, and a token with nearly all the probability: its
     log probability keeps relative accuracy to float32's resolution of 1."""
