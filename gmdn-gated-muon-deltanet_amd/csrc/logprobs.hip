@@ -210,14 +210,16 @@ GMDN_DEV uint64_t lanes_max64(uint64_t x) {
 }
 
 constexpr int TOP_MAX = 32;
-constexpr int TOP_LIST = 1024;  // candidates of a tile
-constexpr int TOP_PIECES = 256;  // and pieces that they come from
 
+// A workgroup's LDS: at most LIST candidates of a tile, from at most PIECES_
+// pieces; less for a workgroup of one wave, so that a CU holds 28 of them.
+template <int NT>
 struct TopLds {
-  float piece[TOP_PIECES][8];
-  int column[TOP_PIECES];
+  static constexpr int LIST = NT > 64 ? 1024 : 256, PIECES_ = NT > 64 ? 256 : 64;
+  float piece[PIECES_][8];
+  int column[PIECES_];
   uint64_t groups[64];
-  uint64_t list[TOP_LIST + TOP_MAX];
+  uint64_t list[LIST + TOP_MAX];
   uint64_t run[TOP_MAX];  // the best so far, in order
   uint64_t bound;
   uint64_t red64[16];
@@ -228,7 +230,7 @@ struct TopLds {
 // The n keys of the list by rank into run: a key's rank is the number of
 // better ones, counted over 64 lanes at a time; a wave ranks every W-th key.
 template <int NT>
-GMDN_DEV void rank_list(TopLds& lds, int n, int top) {
+GMDN_DEV void rank_list(TopLds<NT>& lds, int n, int top) {
   const int lane = lane_id();
   const uint64_t a = lane < n ? lds.list[lane] : 0, b = 64 + lane < n ? lds.list[64 + lane] : 0;
   for (int i = wave_id(); i < n; i += NT / 64) {
@@ -239,10 +241,29 @@ GMDN_DEV void rank_list(TopLds& lds, int n, int top) {
   }
 }
 
+// The top-th largest of a wave's 64 keys (0: fewer are there), bit by bit:
+// first of their values, then, where several keys have that value, of their
+// indexes.
+GMDN_DEV uint64_t kth(uint64_t key, int top) {
+  const uint32_t value = (uint32_t)(key >> 32), index = (uint32_t)key;
+  uint32_t v = 0;
+#pragma unroll
+  for (int b = 31; b >= 0; --b)
+    if (__popcll(__ballot(value >= (v | 1u << b))) >= top) v |= 1u << b;
+  if (v == 0) return 0;
+  const int need = top - __popcll(__ballot(value > v));
+  const uint64_t ties = __ballot(value == v);
+  if (__popcll(ties) == 1) return lane_key(key, __ffsll((long long)ties) - 1);
+  uint32_t x = 0;
+  for (int b = 31; b >= 0; --b)
+    if (__popcll(__ballot(value == v && index >= (x | 1u << b))) >= need) x |= 1u << b;
+  return (uint64_t)v << 32 | x;
+}
+
 // The best `top` of columns first .. last - 1 by one logit a round: for rows
 // that the tiles below give up on.
 template <typename T, int NT>
-GMDN_DEV void slow_top(const T* x, int first, int last, int top, TopLds& lds) {
+GMDN_DEV void slow_top(const T* x, int first, int last, int top, TopLds<NT>& lds) {
   uint64_t prev = ~0ull;
   for (int k = 0; k < top; ++k) {
     uint64_t best = 0;
@@ -274,7 +295,7 @@ GMDN_DEV void slow_top(const T* x, int first, int last, int top, TopLds& lds) {
 // than LDS holds, or a NaN, is left to slow_top.  The sums are returned in the
 // first wave.
 template <typename T, int NT>
-GMDN_DEV Sums top_of(const T* x, int first, int last, int top, TopLds& lds, int& have) {
+GMDN_DEV Sums top_of(const T* x, int first, int last, int top, TopLds<NT>& lds, int& have) {
   const int tid = threadIdx.x;
   Sums a = no_sums();
   have = 0;
@@ -311,7 +332,14 @@ GMDN_DEV Sums top_of(const T* x, int first, int last, int top, TopLds& lds, int&
       atomicMax((unsigned long long*)&lds.groups[lane_id()],
                 (unsigned long long)key_of(bv, c0 + 8 * (bp * NT + tid) + 7));
     __syncthreads();
-    {
+    // the groups' top-th best, or the best so far's: found by the first wave
+    // where that is not many waves' wait, else shared
+    if constexpr (NT <= 256) {
+      if (wave_id() == 0) {
+        const uint64_t k = kth(lds.groups[lane_id()], top);
+        if (lane_id() == 0) lds.bound = have == top && lds.run[top - 1] > k ? lds.run[top - 1] : k;
+      }
+    } else {
       // a wave ranks its share of the groups against all 64; equal only where there is none
       const uint64_t mine = lds.groups[lane_id()];
       constexpr int SHARE = 64 / (NT / 64);
@@ -333,7 +361,7 @@ GMDN_DEV Sums top_of(const T* x, int first, int last, int top, TopLds& lds, int&
       const int c = c0 + 8 * (i * NT + tid);
       if ((most[i] > lv || (most[i] == lv && c <= upto)) && c < last) {
         const int at = atomicAdd(&lds.pieces, 1);
-        if (at < TOP_PIECES) {
+        if (at < TopLds<NT>::PIECES_) {
           float v[8];
           raw[i].get(v);
           *reinterpret_cast<f32x4*>(&lds.piece[at][0]) = f32x4{v[0], v[1], v[2], v[3]};
@@ -344,17 +372,17 @@ GMDN_DEV Sums top_of(const T* x, int first, int last, int top, TopLds& lds, int&
     }
     __syncthreads();
     const int np = lds.pieces;
-    for (int e = tid; e < 8 * np && np <= TOP_PIECES; e += NT) {
+    for (int e = tid; e < 8 * np && np <= TopLds<NT>::PIECES_; e += NT) {
       const float v = lds.piece[e / 8][e % 8];
       const int c = lds.column[e / 8] + e % 8;
       if ((v > lv || (v == lv && c <= upto)) && c < last) {
         const int at = atomicAdd(&lds.count, 1);
-        if (at < TOP_LIST) lds.list[at] = key_of(v, c);
+        if (at < TopLds<NT>::LIST) lds.list[at] = key_of(v, c);
       }
     }
     __syncthreads();
     int n = lds.count;
-    over = n > TOP_LIST || np > TOP_PIECES;
+    over = n > TopLds<NT>::LIST || np > TopLds<NT>::PIECES_;
     if (!over && tid < have) lds.list[n + tid] = lds.run[tid];
     __syncthreads();
     if (tid == 0) lds.pieces = lds.count = 0;
@@ -379,9 +407,9 @@ GMDN_DEV Sums top_of(const T* x, int first, int last, int top, TopLds& lds, int&
 }
 
 template <typename T, int NT, bool SPLIT>
-__global__ void __launch_bounds__(NT, 8)
+__global__ void __launch_bounds__(NT, NT > 64 ? 8 : 6)
 lp_top(const T* __restrict__ logits, int64_t stride, Out out, Parts parts) {
-  __shared__ TopLds lds;
+  __shared__ TopLds<NT> lds;
   const int64_t item = blockIdx.x, row = SPLIT ? item / parts.parts : item;
   const int first = SPLIT ? (int)(item - row * parts.parts) * parts.span : 0;
   const int last = SPLIT && first + parts.span < out.V ? first + parts.span : out.V;
@@ -406,8 +434,8 @@ constexpr int JOIN_THREADS = 1024;
 template <typename T>
 __global__ void __launch_bounds__(JOIN_THREADS)
 lp_join(const T* __restrict__ logits, int64_t stride, Out out, Parts parts) {
-  static_assert(MAX_PARTS * TOP_MAX <= TOP_LIST, "the parts' best fit the list");
-  __shared__ TopLds lds;
+  static_assert(MAX_PARTS * TOP_MAX <= TopLds<JOIN_THREADS>::LIST, "the parts' best fit the list");
+  __shared__ TopLds<JOIN_THREADS> lds;
   const int64_t row = blockIdx.x;
   const T* x = logits + row * stride;
   const int n = parts.parts * out.top;
@@ -523,6 +551,8 @@ void fwd_launch(const T* x, int64_t stride, int64_t rows, const Out& out, Parts 
   if (out.top > 0) {
     if (split)
       hipLaunchKernelGGL((lp_top<T, 1024, true>), grid, dim3(1024), 0, st, x, stride, out, p);
+    else if (out.V <= 8 * 64 * PIECES && rows >= 1024)
+      hipLaunchKernelGGL((lp_top<T, 64, false>), grid, dim3(64), 0, st, x, stride, out, p);
     else if (out.V <= 8 * 256 * PIECES)
       hipLaunchKernelGGL((lp_top<T, 256, false>), grid, dim3(256), 0, st, x, stride, out, p);
     else if (rows > 256)

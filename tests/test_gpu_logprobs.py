@@ -178,10 +178,27 @@ def test_ties_and_orders(V):
         check(x.bfloat16(), tokens, top)
 
 
-@pytest.mark.parametrize("rows,V,top", [(300, 9001, 5), (300, 40000, 32), (700, 300, 0), (300, 5000, 20)])
+@pytest.mark.parametrize("rows,V,top", [(300, 9001, 5), (300, 40000, 32), (700, 300, 0), (300, 5000, 20),
+                                        (1100, 257, 20), (1030, 2047, 32), (1024, 8, 8)])
 def test_many_rows(rows, V, top):
     """Row counts that take other shapes of workgroup than a few rows do."""
     check(*logits((rows, V), rows + V, torch.bfloat16), top)
+
+
+def test_ties_in_many_short_rows():
+    """Equal logits, sorted rows and masks where a row is one wave's."""
+    V, gen = 1500, torch.Generator().manual_seed(7)
+    x = torch.randn(1200, V, generator=gen)
+    x[::7] = 0.0
+    x[1::7] = torch.arange(V).float()
+    x[2::7] = -torch.arange(V).float()
+    x[3::7, 9:] = -math.inf
+    x[4::7] = torch.randint(2, (172, V), generator=gen).float()[:x[4::7].shape[0]]
+    x[5::7] = torch.where((torch.arange(V) // 8) % 64 < 31, 1.0 + torch.rand(V, generator=gen), 0.0)
+    x[6] = -math.inf
+    tokens = torch.randint(V, (1200,), generator=gen)
+    for top in (1, 20, 32):
+        check(x, tokens, top)
 
 
 def test_large_matrices_equal_their_parts():
