@@ -3,14 +3,20 @@
 //
 // All four kernels stream: a group of 128 values is 16 lanes of one piece
 // each, its amax a butterfly over them; nothing is shared between groups.
+// Memory bound (GELU's forward nearly by its vector instructions too: they are
+// active in 98 % of its cycles; fewer of them gained nothing).  At 16384 x 4096 bf16:
+// pack 35 us (5.8 TB/s), unpack 29 us (6.9), GELU 59 us (5.7), its backward with
+// the output again 76 us (6.2); a 1 GiB copy reaches 5.1 TB/s.
 #include "../../include/gmdn_lm.h"
 #include "rows8.h"
 
 namespace gmdn {
 namespace {
 
+// Threads, and pieces a thread has in flight, A8_THREADS apart.  GELU's backward at
+// 16384 x 4096: 256 x 2 76 us, 256 x 4 79, 1024 x 4 90; at 256 x 512 4, 6 and 12 us.
 constexpr int A8_THREADS = 256;
-constexpr int A8_PIECES = 2;  // pieces a thread has in flight, A8_THREADS apart
+constexpr int A8_PIECES = 2;
 constexpr int A8_SPAN = A8_THREADS * A8_PIECES;
 constexpr int64_t A8_GRID = 1 << 20;
 

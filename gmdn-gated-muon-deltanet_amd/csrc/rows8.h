@@ -5,8 +5,9 @@
 // A piece is 8 consecutive values of a row (16 bytes of bf16, 32 of float32).
 // Rows of odd widths start at any element, so the vector types below promise
 // element alignment only; gfx950 loads and stores them by one instruction all
-// the same (measured at 16384 x 1001 beside 16384 x 1024).  Only the short
-// last piece of a row is read and written by elements.
+// the same (packing 16384 x 4095 bf16 takes 44 us, 16384 x 4096 35 us: the
+// pieces cross cache lines).  Only the short last piece of a row is read and
+// written by elements.
 #pragma once
 #include "../../include/gmdn_scan.h"
 #include "tile.h"

@@ -16,7 +16,7 @@ import threading
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libgmdn_scan.so")
-OPS_PATH = os.path.join(HERE, "libgmdn_ops.so")  # the torch operators over it (csrc/torch_ops.cpp)
+OPS_PATH = os.path.join(HERE, "libgmdn_ops.so")  # the torch operators over it (csrc/torch_ops*.cpp)
 
 GMDN_OK = 0
 PREC_TF32 = 0

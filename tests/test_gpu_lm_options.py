@@ -139,3 +139,93 @@ def test_graph_replays_match_eager():
         torch.cuda.synchronize()
         for k, (a, b) in enumerate(zip(outs, ref)):
             assert torch.equal(a, b), f"replay {rep}: output {k} differs"
+
+
+def test_loss_graph_replays_match_eager():
+    """The mean loss over many tokens, forward and backward, in one graph."""
+    dev = _dev()
+    gen = torch.Generator(device=dev).manual_seed(0)
+    x = torch.randn(20000, 96, generator=gen, device=dev, dtype=torch.bfloat16).requires_grad_(True)
+    targets = torch.randint(96, (20000,), generator=gen, device=dev)
+    targets[::17] = logprobs.IGNORE
+
+    def step():
+        loss = logprobs.cross_entropy(x, targets)
+        return loss, *torch.autograd.grad(loss, x)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step()
+    torch.cuda.synchronize()
+    ref = [t.detach().clone() for t in step()]
+    for rep in range(4):
+        step()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        for k, (a, b) in enumerate(zip(outs, ref)):
+            assert torch.equal(a, b), f"replay {rep}: output {k} differs"
+
+
+def _op_calls(dev):
+    gen = torch.Generator(device=dev).manual_seed(0)
+    x = torch.randn(6, 5, 200, generator=gen, device=dev).requires_grad_(True)
+    w, b = (torch.randn(200, generator=gen, device=dev).requires_grad_(True) for _ in range(2))
+    tokens = torch.randint(200, (6, 5), generator=gen, device=dev)
+    plain = x.detach()
+    with torch.no_grad():
+        y, mean, rstd, q, scale = torch.ops.gmdn.layer_norm_fwd(plain, w, b, 1e-5, torch.float32, True)
+        _, h, _, top, stats = torch.ops.gmdn.logprobs_fwd(plain, tokens, 3, -100)
+    wd, bd = w.detach(), b.detach()
+    return {
+        "layer_norm_fwd": (x, w, b, 1e-5, torch.bfloat16, False),
+        "layer_norm_bwd": (y, plain, wd, mean, rstd),
+        "layer_norm8_bwd": (y, q, scale, wd, mean, rstd, torch.float32),
+        "layer_norm8_rebuild": (q, scale, wd, bd, mean, rstd, torch.bfloat16),
+        "act8_pack": (plain,),
+        "act8_unpack": (q, scale, torch.bfloat16),
+        "gelu8_fwd": (x,),
+        "gelu8_bwd": (y, q, scale, True),
+        "logprobs_fwd": (x, tokens, 3, -100),
+        "logprobs_bwd": (plain, tokens, stats, h, top, h, None, None, -100),
+    }
+
+
+@pytest.mark.parametrize("name", ["layer_norm_fwd", "layer_norm_bwd", "layer_norm8_bwd", "layer_norm8_rebuild",
+                                  "act8_pack", "act8_unpack", "gelu8_fwd", "gelu8_bwd", "logprobs_fwd", "logprobs_bwd"])
+def test_opcheck(name):
+    dev = _dev()
+    torch.library.opcheck(getattr(torch.ops.gmdn, name).default, _op_calls(dev)[name])
+
+
+def test_compiled_step_matches_eager():
+    """torch.compile over norm, MLP and loss with 8-bit checkpoints: the eager
+    call's loss and gradients."""
+    dev = _dev()
+    torch.manual_seed(0)
+    x = torch.randn(4, 60, 64, device=dev, requires_grad=True)
+    nw, nb = torch.rand(64, device=dev).requires_grad_(True), torch.zeros(64, device=dev, requires_grad=True)
+    w1 = (torch.randn(256, 64, device=dev) / 8).requires_grad_(True)
+    w2 = (torch.randn(64, 256, device=dev) / 16).requires_grad_(True)
+    tokens = torch.randint(64, (4, 60), device=dev)
+    leaves = (x, nw, nb, w1, w2)
+
+    def fn(x, nw, nb, w1, w2):
+        y = x + act8.norm_mlp(x, nw, nb, w1, w2)
+        return logprobs.cross_entropy(layer_norm.layer_norm(y, nw, nb, checkpoint="int8"), tokens)
+
+    eager = fn(*leaves)
+    want = torch.autograd.grad(eager, leaves)
+    torch._dynamo.reset()
+    loss = torch.compile(fn, backend="aot_eager", fullgraph=True)(*leaves)
+    got = torch.autograd.grad(loss, leaves)
+    assert torch.allclose(loss, eager, rtol=1e-6)
+    for a, b in zip(got, want):
+        assert _moved(a, b) < 1e-5
