@@ -11,9 +11,9 @@
 // matrix is read and written once; the deviation is a second sum over the
 // centred registers (a sum of squares would cancel for rows far from zero).
 // At 5.1 TB/s (what a 1 GiB copy reaches):
-//   16384 x 1024, float32 in, bf16 out   forward 17 us (floor 20; outputs stay in the cache),
-//                                        backward 34 + 4 us (33)
-//   8192 x 8192 bf16                     forward 48 us (53), backward 72 + 7 us (79)
+//   16384 x 1024, float32 in, bf16 out   forward 19 us (floor 20), backward 29 + 5 us (33)
+//   8192 x 8192 bf16                     forward 49 us (53), backward 65 + 6 us (79)
+// (in brackets the floor: the outputs stay in the cache in part).
 #include "../../include/gmdn_lm.h"
 #include <type_traits>
 #include "rows8.h"
@@ -26,7 +26,7 @@ constexpr int LN_MAX_D = 16384;
 // Workgroups of a launch at most; each takes rows in turn.  Forward: 1024 took
 // 55 us where 512 take 48 at 8192 x 8192, and the same at 16384 x 1024.
 // Backward: each writes 2 d partial sums, at 8192 x 8192 with 1024 of them a sixth
-// of all bytes (94 + 17 us, with 256 72 + 7).
+// of all bytes (94 + 17 us, with 256 65 + 6).
 constexpr int LN_FWD_BLOCKS = 512;
 constexpr int LN_BWD_BLOCKS = 256;
 
@@ -280,7 +280,7 @@ ln_bwd(Src src, const TY* __restrict__ dy, int64_t ds, const void* __restrict__ 
 // dweight and dbias from the workgroups' sums: a workgroup takes 32 columns
 // of (2, d) -- 8 lanes of 4 -- and 128 lane groups every 128th partial row, four
 // of them in flight; joined in a wave, then over the waves in LDS.  The order
-// is fixed: the same bits on every run.  Bound by latency: 4 us for 256 rows of
+// is fixed: the same bits on every run.  Bound by latency: 4 to 5 us for 256 rows of
 // 2 x 1024 (12 us when a thread added 128 rows one after the other).
 constexpr int LN_COLS = 32;
 constexpr int LN_SUM_THREADS = 1024;
