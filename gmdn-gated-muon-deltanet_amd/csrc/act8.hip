@@ -169,7 +169,7 @@ unpack(const int8_t* __restrict__ q, const float* __restrict__ scale, const T* _
 int check8(int64_t rows, int64_t d, int64_t stride, int32_t dtype) {
   if (rows < 0 || d <= 0 || stride < 0) return GMDN_ERR_ARG;
   if (!type_ok(dtype)) return GMDN_ERR_UNSUPPORTED;
-  if (d >= ((int64_t)1 << 31) || rows > ((int64_t)1 << 40)) return GMDN_ERR_ARG;
+  if (d >= ((int64_t)1 << 31) || rows > ((int64_t)1 << 48) / d) return GMDN_ERR_ARG;
   return GMDN_OK;
 }
 Shape shape_of(int64_t rows, int64_t d, int64_t stride) {

@@ -242,6 +242,13 @@ template <int NT>
 GMDN_DEV void rank_list(TopLds<NT>& lds, int n, int top) {
   const int lane = lane_id();
   const uint64_t a = lane < n ? lds.list[lane] : 0, b = 64 + lane < n ? lds.list[64 + lane] : 0;
+  if (NT == 64 && n <= 64) {  // alone: each lane its own key, against each of the others
+    int rank = 0;
+#pragma unroll 4
+    for (int i = 0; i < n; ++i) rank += lane_key(a, i) > a;
+    if (lane < n && rank < top) lds.run[rank] = a;
+    return;
+  }
   for (int i = wave_id(); i < n; i += NT / 64) {
     const uint64_t k = i < 64 ? lane_key(a, i) : i < 128 ? lane_key(b, i - 64) : lds.list[i];
     int rank = __popcll(__ballot(a > k)) + __popcll(__ballot(b > k));
@@ -558,7 +565,7 @@ int parts_of(int64_t rows, int64_t V) {
 }
 int span_of(int64_t V, int parts) { return (int)(((V + parts - 1) / parts + 7) / 8 * 8); }
 
-// With alternatives: a wave a row for many short rows (8192 x 2000: 19 us, 256
+// With alternatives: a wave a row for many short rows (8192 x 2000: 17 us, 256
 // threads 42; 64 x 2000: 10 and 7), 256 threads while a row is one tile of theirs,
 // 512 for many rows (16384 x 32000: 276 us, 1024 threads 312), 1024 for few (8 x
 // 32000: 8 us, 512 threads 11).
