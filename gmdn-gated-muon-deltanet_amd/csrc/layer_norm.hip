@@ -11,8 +11,8 @@
 // matrix is read and written once; the deviation is a second sum over the
 // centred registers (a sum of squares would cancel for rows far from zero).
 // At 5.1 TB/s (what a 1 GiB copy reaches):
-//   16384 x 1024, float32 in, bf16 out   forward 19 us (floor 20), backward 29 + 5 us (33)
-//   8192 x 8192 bf16                     forward 49 us (53), backward 65 + 6 us (79)
+//   16384 x 1024, float32 in, bf16 out   forward 19 us (floor 20), backward 27 + 5 us (33)
+//   8192 x 8192 bf16                     forward 49 us (53), backward 63 + 6 us (79)
 // (in brackets the floor: the outputs stay in the cache in part).
 #include "../../include/gmdn_lm.h"
 #include <type_traits>
@@ -149,8 +149,9 @@ struct FromX {
   const TX* x;
   int64_t stride;
   struct Raw : Raw8<TX> {
+    template <bool FAR = false>
     GMDN_DEV void load(const FromX& src, int64_t r, int c, int n, int) {
-      Raw8<TX>::load(src.x + r * src.stride + c, n);
+      Raw8<TX>::template load<FAR>(src.x + r * src.stride + c, n);
     }
   };
 };
@@ -160,6 +161,7 @@ struct From8 {
   struct Raw {
     u32x2_any v;
     float s;
+    template <bool FAR = false>
     GMDN_DEV void load(const From8& src, int64_t r, int c, int n, int d) {
       v = load_q8(src.q + r * d + c, n);
       s = n > 0 ? src.scale[r * groups8(d) + c / GROUP8] : 0.f;
@@ -172,12 +174,14 @@ struct From8 {
 // (workgroups, 2, d).  A thread's columns are the same in every row, so the
 // sums stay in its registers; the rows a workgroup takes side by side are
 // added in LDS at the end, in a fixed order.  No atomics: they would add in
-// another order on every run.
+// another order on every run.  `large`: the matrix is FAR_BYTES or more; rows of
+// several waves are then loaded past the caches (8192 x 8192: 80 -> 78 us; from
+// 8 bits at 16384 x 4096: 66 -> 58).
 template <typename Src, typename TX, typename TY, int TPR, int NV>
 __global__ void __launch_bounds__(ln_threads(TPR))
 ln_bwd(Src src, const TY* __restrict__ dy, int64_t ds, const void* __restrict__ w, bool w16,
        const float* __restrict__ mean, const float* __restrict__ rstd, TX* __restrict__ dx,
-       float* __restrict__ part, int64_t rows, int d) {
+       float* __restrict__ part, int64_t rows, int d, bool large) {
   constexpr int RPB = ln_threads(TPR) / TPR;
   // a row's loads before the last row's work (8192 x 8192: 103 -> 88 us), where
   // the registers hold them: 1024 threads have 128 each, and spilled
@@ -199,15 +203,25 @@ ln_bwd(Src src, const TY* __restrict__ dy, int64_t ds, const void* __restrict__ 
   typename Src::Raw xr[NV];
   Raw8<TY> gr[NV];
   float mr, rr;
+  auto pieces = [&](int64_t r, auto far) {
+    const bool live = r < rows;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = 8 * (i * TPR + t);
+      xr[i].template load<decltype(far)::value>(src, r, c, live ? d - c : 0, d);
+      gr[i].template load<decltype(far)::value>(dy + r * ds + c, live ? d - c : 0);
+    }
+  };
   auto fetch = [&](int64_t r) {
     const bool live = r < rows;
     mr = live ? mean[r] : 0.f;
     rr = live ? rstd[r] : 0.f;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = 8 * (i * TPR + t);
-      xr[i].load(src, r, c, live ? d - c : 0, d);
-      gr[i].load(dy + r * ds + c, live ? d - c : 0);
+    if (TPR > 64 && sizeof(TY) == 2 && large) {
+      apart();
+      pieces(r, std::true_type{});
+      apart();
+    } else {
+      pieces(r, std::false_type{});
     }
   };
   const int64_t step = (int64_t)gridDim.x * RPB;
@@ -240,11 +254,23 @@ ln_bwd(Src src, const TY* __restrict__ dy, int64_t ds, const void* __restrict__ 
     const float mg = row_sum<TPR>(s0, red, slot) / (float)d;
     const float mx = row_sum<TPR>(s1, red, slot) / (float)d;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = 8 * (i * TPR + t);
+    for (int i = 0; i < NV; ++i)
 #pragma unroll
       for (int j = 0; j < 8; ++j) g[i][j] = rs * (g[i][j] - mg - v[i][j] * mx);
-      if (live && c < d) stream8(dx + r * d + c, d - c, g[i]);
+    if (sizeof(TX) == 4 && !large) {
+      apart();
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int c = 8 * (i * TPR + t);
+        if (live && c < d) stream8_f32(dx + r * d + c, d - c, g[i]);
+      }
+      apart();
+    } else {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int c = 8 * (i * TPR + t);
+        if (live && c < d) stream8(dx + r * d + c, d - c, g[i]);
+      }
     }
   }
   if (!w) return;
@@ -475,6 +501,7 @@ int gmdn_layer_norm_bwd(const void* dy, const void* x, const int8_t* q, const fl
     if (!dy || (!x && !q) || (x && q) || !mean || !rstd || !dx) return GMDN_ERR_ARG;
     nb = ln_blocks(rows, d, LN_BWD_BLOCKS);
     if (weight && (!workspace || workspace_floats < (size_t)(nb * 2 * d))) return GMDN_ERR_WORKSPACE;
+    const bool large = rows * d * (x_type == GMDN_DTYPE_F32 ? 4 : 2) >= FAR_BYTES;
     with_types(x_type, y_type, [&](auto tx, auto ty) {
       using TX = decltype(tx);
       using TY = decltype(ty);
@@ -483,11 +510,11 @@ int gmdn_layer_norm_bwd(const void* dy, const void* x, const int8_t* q, const fl
         const dim3 grid((unsigned)nb), block(ln_threads(S::TPR));
               if (q)
           hipLaunchKernelGGL((ln_bwd<From8, TX, TY, S::TPR, S::NV>), grid, block, 0, st, From8{q, scale},
-                             (const TY*)dy, dy_stride, weight, w16, mean, rstd, (TX*)dx, workspace, rows, (int)d);
+                             (const TY*)dy, dy_stride, weight, w16, mean, rstd, (TX*)dx, workspace, rows, (int)d, large);
         else
           hipLaunchKernelGGL((ln_bwd<FromX<TX>, TX, TY, S::TPR, S::NV>), grid, block, 0, st,
                              FromX<TX>{(const TX*)x, x_stride}, (const TY*)dy, dy_stride, weight, w16, mean, rstd,
-                             (TX*)dx, workspace, rows, (int)d);
+                             (TX*)dx, workspace, rows, (int)d, large);
       });
     });
     if (hipGetLastError() != hipSuccess) return GMDN_ERR_LAUNCH;

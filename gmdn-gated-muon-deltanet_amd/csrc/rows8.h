@@ -77,6 +77,21 @@ GMDN_DEV void stream8(bf16* p, int n, const float (&x)[8]) {
   }
 }
 GMDN_DEV void stream8(float* p, int n, const float (&x)[8]) { store8(p, n, x); }
+// float32 past the caches all the same: faster while the whole matrix would fit
+// them (a norm's dx at 16384 x 1024: 37 us, plain 39; 16384 x 2048 above).
+GMDN_DEV void stream8_f32(float* p, int n, const float (&x)[8]) {
+  if (n >= 8) {
+    f32x4_any* q = reinterpret_cast<f32x4_any*>(p);
+    __builtin_nontemporal_store(f32x4_any{x[0], x[1], x[2], x[3]}, q);
+    __builtin_nontemporal_store(f32x4_any{x[4], x[5], x[6], x[7]}, q + 1);
+  } else {
+    store8(p, n, x);
+  }
+}
+GMDN_DEV void stream8_f32(bf16* p, int n, const float (&x)[8]) { stream8(p, n, x); }
+// At both ends of one side of a branch whose sides differ in their caching
+// only: the compiler would join them into one, without the difference.
+GMDN_DEV void apart() { asm volatile(""); }
 
 // A piece as it lies in memory, for loads that are to be in flight over other
 // work; values from n on are `pad` (0 or an infinity).  FAR: whole bf16 pieces are

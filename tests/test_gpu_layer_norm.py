@@ -230,6 +230,29 @@ def test_from_checkpoint(rows, d, x_dtype, y_dtype):
     assert_close(again, *ref["y"], "rebuilt")
 
 
+@pytest.mark.parametrize("dtype,rows,d", [(torch.bfloat16, 13000, 4000), (torch.float32, 13000, 2048),
+                                          (torch.float32, 3000, 1024)])
+def test_large_matrices_equal_their_parts(dtype, rows, d):
+    """From 96 MB on a matrix goes past the caches, below it a float32 dx does:
+    the same bits as its parts, which are on the other side or the same."""
+    dev = _dev()
+    gen = torch.Generator(device=dev).manual_seed(4)
+    x = torch.randn(rows, d, generator=gen, device=dev).to(dtype)
+    dy = torch.randn(rows, d, generator=gen, device=dev).to(dtype)
+    w, b = torch.randn(d, generator=gen, device=dev), torch.randn(d, generator=gen, device=dev)
+
+    def rows_of(x, dy):
+        y, mean, rstd, q, scale = torch.ops.gmdn.layer_norm_fwd(x, w, b, 1e-5, dtype, True)
+        return (y, mean, rstd, q, scale, torch.ops.gmdn.layer_norm_bwd(dy, x, w, mean, rstd)[0],
+                torch.ops.gmdn.layer_norm8_bwd(dy, q, scale, w, mean, rstd, dtype)[0],
+                torch.ops.gmdn.layer_norm8_rebuild(q, scale, w, b, mean, rstd, dtype))
+
+    whole = rows_of(x, dy)
+    for a in (0, rows - 500):
+        part = rows_of(x[a:a + 500], dy[a:a + 500])
+        assert all(torch.equal(o[a:a + 500], p) for o, p in zip(whole, part))
+
+
 def test_deterministic_and_on_another_stream():
     dev = _dev()
     x, w, b, dy = (t.to(dev) for t in data(5000, 1024, 2, torch.float32, torch.bfloat16))
