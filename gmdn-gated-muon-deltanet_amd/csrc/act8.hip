@@ -87,6 +87,7 @@ GMDN_DEV void gelu(float h, float& a, float& slope) {
   slope = __builtin_fmaf(h * (0.39894228040143268f * half), half, cdf);
 }
 
+// The checkpoint of x; GELU: and a = GELU(x), or that alone (q null).
 template <typename T, bool GELU, bool FAR>
 __global__ void __launch_bounds__(A8_THREADS)
 pack(const T* __restrict__ x, T* __restrict__ a, int8_t* __restrict__ q, float* __restrict__ scale, Shape s,
@@ -106,11 +107,13 @@ pack(const T* __restrict__ x, T* __restrict__ a, int8_t* __restrict__ q, float* 
       const Place p = place(piece, s);
       float v[8];
       raw[i].get(v);
-      const Scale8 sc = scale8(lanes_max<GROUP8_PIECES>(amax_bits(v)));
-      if (!p.n) continue;
-      if (piece % GROUP8_PIECES == 0) scale[p.unit] = sc.scale;
       const int64_t at = offset(p, piece, s, s.d);
-      store_q8(q + at, p.n, quant8(v, sc.inverse));
+      if (!GELU || q) {
+        const Scale8 sc = scale8(lanes_max<GROUP8_PIECES>(amax_bits(v)));
+        if (p.n && piece % GROUP8_PIECES == 0) scale[p.unit] = sc.scale;
+        if (p.n) store_q8(q + at, p.n, quant8(v, sc.inverse));
+      }
+      if (!p.n) continue;
       if constexpr (GELU) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = gelu(v[j]);
@@ -186,7 +189,7 @@ int pack_call(const void* x, void* a, int8_t* q, float* scale, int64_t rows, int
               void* stream) {
   const int rc = check8(rows, d, xs, dtype);
   if (rc != GMDN_OK || rows == 0) return rc;
-  if (!x || !q || !scale || (GELU && !a)) return GMDN_ERR_ARG;
+  if (!x || !q != !scale || (GELU ? !a : !q)) return GMDN_ERR_ARG;
   const Shape s = shape_of(rows, d, xs);
   if (dtype == GMDN_DTYPE_BF16 && rows * d * 2 >= FAR_BYTES)
     hipLaunchKernelGGL((pack<bf16, GELU, true>), grid8(s), dim3(A8_THREADS), 0, (hipStream_t)stream, (const bf16*)x,

@@ -112,6 +112,11 @@ std::pair<Tensor, Tensor> new_kept(const Tensor& x) {
           fresh(x, with_last(lead(x), gmdn_act8_groups(x.size(-1))))};
 }
 
+std::pair<Tensor, Tensor> kept_or_none(const Tensor& x, bool pack) {
+  if (pack) return new_kept(x);
+  return {fresh(x, {0}, at::kChar), fresh(x, {0})};
+}
+
 // ---------------------------------------------------------------- layer norm
 using Norm = std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor>;
 Norm layer_norm_fwd(const Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps, ScalarType dtype,
@@ -121,7 +126,7 @@ Norm layer_norm_fwd(const Tensor& x, const OptTensor& weight, const OptTensor& b
   const Rows r = rows_of(x, "x");
   const Weights w = weights_of(weight, bias, x, r.d);
   Tensor y = fresh(x, x.sizes(), dtype), mean = fresh(x, lead(x)), rstd = fresh(x, lead(x));
-  auto [q, scale] = pack ? new_kept(x) : std::pair(fresh(x, {0}, at::kChar), fresh(x, {0}));
+  auto [q, scale] = kept_or_none(x, pack);
   if (r.rows)
     check(gmdn_layer_norm_fwd(r.ptr(), ptr(w.w), ptr(w.b), y.data_ptr(), fp(mean), fp(rstd),
                               pack ? q.data_ptr<int8_t>() : nullptr, pack ? fp(scale) : nullptr, r.rows, r.d, r.stride,
@@ -203,15 +208,15 @@ Tensor act8_unpack(const Tensor& q, const Tensor& scale, ScalarType dtype) {
           "gmdn_act8_unpack");
   return x;
 }
-std::tuple<Tensor, Tensor, Tensor> gelu8_fwd(const Tensor& h) {
+std::tuple<Tensor, Tensor, Tensor> gelu8_fwd(const Tensor& h, bool pack) {
   const c10::DeviceGuard guard(h.device());
   const int32_t code = type_code(h.scalar_type(), "h");
   const Rows r = rows_of(h, "h");
   Tensor a = fresh(h, h.sizes(), h.scalar_type());
-  auto [q, scale] = new_kept(h);
+  auto [q, scale] = kept_or_none(h, pack);
   if (r.rows)
-    check(gmdn_gelu8_fwd(r.ptr(), a.data_ptr(), q.data_ptr<int8_t>(), fp(scale), r.rows, r.d, r.stride, code,
-                         stream_of(h)),
+    check(gmdn_gelu8_fwd(r.ptr(), a.data_ptr(), pack ? q.data_ptr<int8_t>() : nullptr, pack ? fp(scale) : nullptr,
+                         r.rows, r.d, r.stride, code, stream_of(h)),
           "gmdn_gelu8_fwd");
   return {a, q, scale};
 }
@@ -335,7 +340,7 @@ struct Gelu8Fwd : torch::autograd::Function<Gelu8Fwd> {
   static constexpr bool is_traceable = true;
   static Tensor forward(AutogradContext* ctx, const Tensor& h, std::pair<Tensor, Tensor>* kept) {
     at::AutoDispatchBelowADInplaceOrView below;
-    auto [a, q, scale] = GMDN_OP(gelu8_fwd).call(h);
+    auto [a, q, scale] = GMDN_OP(gelu8_fwd).call(h, true);
     *kept = {q, scale};
     ctx->set_materialize_grads(false);
     ctx->save_for_backward({q, scale});
@@ -347,11 +352,12 @@ struct Gelu8Fwd : torch::autograd::Function<Gelu8Fwd> {
     return {std::get<0>(GMDN_OP(gelu8_bwd).call(g[0], s[0], s[1], false)), Tensor()};
   }
 };
-std::tuple<Tensor, Tensor, Tensor> gelu8_fwd_ad(const Tensor& h) {
+std::tuple<Tensor, Tensor, Tensor> gelu8_fwd_ad(const Tensor& h, bool pack) {
   if (!wants_grad({&h})) {
     at::AutoDispatchBelowADInplaceOrView below;
-    return GMDN_OP(gelu8_fwd).call(h);
+    return GMDN_OP(gelu8_fwd).call(h, pack);
   }
+  TORCH_CHECK(pack, "gelu8_fwd without its checkpoint has no backward");
   std::pair<Tensor, Tensor> kept;
   Tensor a = Gelu8Fwd::apply(h, &kept);
   return {a, kept.first, kept.second};
@@ -404,7 +410,7 @@ TORCH_LIBRARY_FRAGMENT(gmdn, m) {
         "ScalarType dtype) -> Tensor", PT2);
   m.def("act8_pack(Tensor x) -> (Tensor, Tensor)", PT2);
   m.def("act8_unpack(Tensor q, Tensor scale, ScalarType dtype) -> Tensor", PT2);
-  m.def("gelu8_fwd(Tensor h) -> (Tensor, Tensor, Tensor)", PT2);
+  m.def("gelu8_fwd(Tensor h, bool pack=True) -> (Tensor, Tensor, Tensor)", PT2);
   m.def("gelu8_bwd(Tensor da, Tensor q, Tensor scale, bool with_output) -> (Tensor, Tensor)", PT2);
   m.def("logprobs_fwd(Tensor logits, Tensor tokens, SymInt top, SymInt ignore_index) -> "
         "(Tensor, Tensor, Tensor, Tensor, Tensor)", PT2);

@@ -11,7 +11,7 @@ group below 2^-100 reads back as zeros; one that holds an infinity or a NaN
 reads back as NaN.
 
 The forward's outputs are computed from the activations themselves; only the
-backward sees the checkpoints.
+backward sees the checkpoints, and a call without gradients makes none.
 
 * ``pack`` / ``unpack`` -- a checkpoint of any tensor.
 * ``gelu``     -- GELU that keeps its input in 8 bits.
@@ -57,7 +57,7 @@ def gelu(h: Tensor) -> Tensor:
     """GELU (``h`` times the normal distribution function of ``h``), keeping
     ``h`` in 8 bits for the backward."""
     ops.ensure()
-    return torch.ops.gmdn.gelu8_fwd(h)[0]
+    return torch.ops.gmdn.gelu8_fwd(h, ops.wants_grad(h))[0]
 
 
 def _cast(*tensors: Tensor | None):
@@ -99,17 +99,20 @@ class _Linear(torch.autograd.Function):
 def linear(x: Tensor, weight: Tensor, bias: Tensor | None = None) -> Tensor:
     """``F.linear`` that keeps ``x`` in 8 bits for the weight's gradient."""
     ops.ensure()
-    return _Linear.apply(*_cast(x, weight, bias))
+    x, weight, bias = _cast(x, weight, bias)
+    if not ops.wants_grad(x, weight, bias):
+        return F.linear(x, weight, bias)
+    return _Linear.apply(x, weight, bias)
 
 
-def _mlp_forward(ctx, y, w1, w2):
+def _mlp_forward(y, w1, w2, pack=True):
     """linear, GELU, linear; returns the output and the hidden checkpoint."""
     h = F.linear(y, w1)
-    a, qh, sh = torch.ops.gmdn.gelu8_fwd(h)
+    a, qh, sh = torch.ops.gmdn.gelu8_fwd(h, pack)
     return F.linear(a, w2), qh, sh
 
 
-def _mlp_backward(ctx, dout, qh, sh, w1, w2, need1, need2, input_again):
+def _mlp_backward(dout, qh, sh, w1, w2, need1, need2, input_again):
     """(dy, dw1, dw2) of linear, GELU, linear; ``input_again`` gives the input
     from its checkpoint, where the first weight wants its gradient."""
     da = dout @ w2
@@ -124,7 +127,7 @@ def _mlp_backward(ctx, dout, qh, sh, w1, w2, need1, need2, input_again):
 class _Mlp(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w1, w2):
-        out, qh, sh = _mlp_forward(ctx, x, w1, w2)
+        out, qh, sh = _mlp_forward(x, w1, w2)
         ctx.save_for_backward(*torch.ops.gmdn.act8_pack(x), qh, sh, w1, w2)
         return out
 
@@ -132,7 +135,7 @@ class _Mlp(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
         q, scale, qh, sh, w1, w2 = ctx.saved_tensors
-        return _mlp_backward(ctx, dout, qh, sh, w1, w2, *ctx.needs_input_grad[1:3],
+        return _mlp_backward(dout, qh, sh, w1, w2, *ctx.needs_input_grad[1:3],
                              lambda: torch.ops.gmdn.act8_unpack(q, scale, dout.dtype))
 
 
@@ -140,14 +143,17 @@ def mlp(x: Tensor, w1: Tensor, w2: Tensor) -> Tensor:
     """``F.linear(F.gelu(F.linear(x, w1)), w2)``, keeping ``x`` and the hidden
     layer in 8 bits."""
     ops.ensure()
-    return _Mlp.apply(*_cast(x, w1, w2))
+    x, w1, w2 = _cast(x, w1, w2)
+    if not ops.wants_grad(x, w1, w2):
+        return _mlp_forward(x, w1, w2, False)[0]
+    return _Mlp.apply(x, w1, w2)
 
 
 class _NormMlp(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, w1, w2, eps):
         y, mean, rstd, q, scale = torch.ops.gmdn.layer_norm_fwd(x, weight, bias, eps, w1.dtype, True)
-        out, qh, sh = _mlp_forward(ctx, y, w1, w2)
+        out, qh, sh = _mlp_forward(y, w1, w2)
         ctx.save_for_backward(q, scale, mean, rstd, qh, sh, weight, bias, w1, w2)
         ctx.x_dtype = x.dtype
         return out
@@ -157,7 +163,7 @@ class _NormMlp(torch.autograd.Function):
     def backward(ctx, dout):
         q, scale, mean, rstd, qh, sh, weight, bias, w1, w2 = ctx.saved_tensors
         dy, dw1, dw2 = _mlp_backward(
-            ctx, dout, qh, sh, w1, w2, *ctx.needs_input_grad[3:5],
+            dout, qh, sh, w1, w2, *ctx.needs_input_grad[3:5],
             lambda: torch.ops.gmdn.layer_norm8_rebuild(q, scale, weight, bias, mean, rstd, dout.dtype))
         dx, dweight, dbias = torch.ops.gmdn.layer_norm8_bwd(dy, q, scale, weight, mean, rstd, ctx.x_dtype)
         return (dx, dweight if weight is not None else None, dbias if bias is not None else None, dw1, dw2, None)
@@ -168,4 +174,6 @@ def norm_mlp(x: Tensor, weight: Tensor | None, bias: Tensor | None, w1: Tensor, 
     hidden layer in 8 bits."""
     ops.ensure()
     w1, w2 = _cast(w1, w2)
+    if not ops.wants_grad(x, weight, bias, w1, w2):
+        return _mlp_forward(torch.ops.gmdn.layer_norm_fwd(x, weight, bias, eps, w1.dtype, False)[0], w1, w2, False)[0]
     return _NormMlp.apply(x, weight, bias, w1, w2, eps)

@@ -36,7 +36,8 @@ def layer_norm(x: Tensor, weight: Tensor | None = None, bias: Tensor | None = No
     of its group's largest magnitude.
     """
     ops.ensure()
-    return torch.ops.gmdn.layer_norm_fwd(x, weight, bias, eps, dtype or x.dtype, checked_checkpoint(checkpoint))[0]
+    pack = checked_checkpoint(checkpoint) and ops.wants_grad(x, weight, bias)
+    return torch.ops.gmdn.layer_norm_fwd(x, weight, bias, eps, dtype or x.dtype, pack)[0]
 
 
 class LayerNorm(nn.LayerNorm):

@@ -34,7 +34,7 @@ its model, train_ablation.py:420-422):
   dweight, dbias)``; ``gmdn::layer_norm8_rebuild(q, scale, weight, bias, mean,
   rstd, dtype) -> y`` (gmdn_amd.layer_norm).
 * ``gmdn::act8_pack(x) -> (q, scale)``, ``gmdn::act8_unpack(q, scale, dtype)
-  -> x`` -- 8-bit activation checkpoints; ``gmdn::gelu8_fwd(h) -> (a, q,
+  -> x`` -- 8-bit activation checkpoints; ``gmdn::gelu8_fwd(h, pack) -> (a, q,
   scale)`` and ``gmdn::gelu8_bwd(da, q, scale, with_output) -> (dh, a)`` --
   GELU that keeps its input in one (gmdn_amd.act8).
 * ``gmdn::logprobs_fwd(logits, tokens, top, ignore_index) -> (logprob, entropy,
@@ -197,10 +197,13 @@ def _act8_fakes(x):
             x.new_empty((*x.shape[:-1], (x.shape[-1] + 127) // 128), dtype=torch.float32))
 
 
+def _act8_fakes_if(x, pack):
+    return _act8_fakes(x) if pack else (x.new_empty((0,), dtype=torch.int8), _empty(x))
+
+
 def _layer_norm_fwd_fake(x, weight, bias, eps, dtype, pack):
     stats = [x.new_empty(x.shape[:-1], dtype=torch.float32) for _ in range(2)]
-    kept = _act8_fakes(x) if pack else (x.new_empty((0,), dtype=torch.int8), _empty(x))
-    return x.new_empty(x.shape, dtype=dtype), *stats, *kept
+    return x.new_empty(x.shape, dtype=dtype), *stats, *_act8_fakes_if(x, pack)
 
 
 def _layer_norm_bwd_fake(dy, x, weight, mean, rstd):
@@ -220,8 +223,8 @@ def _act8_unpack_fake(q, scale, dtype):
     return q.new_empty(q.shape, dtype=dtype)
 
 
-def _gelu8_fwd_fake(h):
-    return h.new_empty(h.shape), *_act8_fakes(h)
+def _gelu8_fwd_fake(h, pack=True):
+    return h.new_empty(h.shape), *_act8_fakes_if(h, pack)
 
 
 def _gelu8_bwd_fake(da, q, scale, with_output):
@@ -285,6 +288,11 @@ def ensure() -> None:
     have been built after this module's import)."""
     if not REGISTERED:
         nat.load()
+
+
+def wants_grad(*tensors: Tensor | None) -> bool:
+    """Whether a call on these tensors is recorded for a backward."""
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
 def __getattr__(name: str):

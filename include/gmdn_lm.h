@@ -64,7 +64,7 @@ int gmdn_act8_unpack(const int8_t* q, const float* scale, void* x, int64_t rows,
                      void* stream);
 
 /* a = GELU(h) = h Phi(h) (Phi the normal distribution function), and h's
- * checkpoint. */
+ * checkpoint (none where q and scale are NULL). */
 int gmdn_gelu8_fwd(const void* h, void* a, int8_t* q, float* scale, int64_t rows, int64_t d, int64_t h_stride,
                    int32_t dtype, void* stream);
 

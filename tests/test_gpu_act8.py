@@ -294,6 +294,31 @@ def test_mlp_keeps_less_memory():
     assert held <= rows * d * 5 * (1 + 4 / 128) + (1 << 16), held / (rows * d)
 
 
+def test_without_gradients_nothing_is_packed():
+    """Under no_grad, and where nothing wants a gradient, the outputs are the
+    same and no checkpoint is made."""
+    dev = _dev()
+    torch.manual_seed(0)
+    x = torch.randn(5, 40, 128, device=dev)
+    nw, w1, w2 = torch.rand(128, device=dev), torch.randn(256, 128, device=dev), torch.randn(128, 256, device=dev)
+
+    def calls():
+        return (act8.gelu(x), act8.linear(x, w1), act8.mlp(x, w1, w2), act8.norm_mlp(x, nw, None, w1, w2))
+
+    with torch.no_grad():
+        plain = calls()
+    x.requires_grad_(True)
+    kept = calls()
+    with torch.no_grad():
+        again = calls()
+    for a, b, c in zip(plain, kept, again):
+        assert torch.equal(a, b) and torch.equal(a, c) and b.requires_grad and not c.requires_grad
+    a, q, scale = torch.ops.gmdn.gelu8_fwd(x.detach(), False)
+    assert q.numel() == scale.numel() == 0 and torch.equal(a, plain[0])
+    with pytest.raises(RuntimeError, match="no backward"):
+        torch.ops.gmdn.gelu8_fwd(x, False)
+
+
 def test_frozen_weights():
     dev = _dev()
     x = torch.randn(20, 64, device=dev, requires_grad=True)

@@ -60,6 +60,7 @@ def test_act8_argument_checks():
     assert lib.gmdn_act8_pack(None, None, None, 0, 64, 64, BF16, None) == 0
     assert lib.gmdn_act8_unpack(P, P, None, 4, 64, BF16, None) == 1
     assert lib.gmdn_gelu8_fwd(P, None, P, P, 4, 64, 64, BF16, None) == 1
+    assert lib.gmdn_gelu8_fwd(P, P, P, None, 4, 64, 64, BF16, None) == 1
     assert lib.gmdn_gelu8_bwd(None, P, P, P, None, 4, 64, 64, BF16, None) == 1
     assert lib.gmdn_gelu8_bwd(None, None, None, None, None, 0, 64, 64, F32, None) == 0
 
