@@ -450,15 +450,32 @@ constexpr int JOIN_THREADS = 1024;
 template <typename T>
 __global__ void __launch_bounds__(JOIN_THREADS)
 lp_join(const T* __restrict__ logits, int64_t stride, Out out, Parts parts) {
-  static_assert(MAX_PARTS * TOP_MAX <= TopLds<JOIN_THREADS>::LIST, "the parts' best fit the list");
+  static_assert(MAX_PARTS * TOP_MAX <= JOIN_THREADS && JOIN_THREADS <= TopLds<JOIN_THREADS>::LIST, "a key a thread");
   __shared__ TopLds<JOIN_THREADS> lds;
   const int64_t row = blockIdx.x;
   const T* x = logits + row * stride;
-  const int n = parts.parts * out.top;
-  for (int i = threadIdx.x; i < n; i += JOIN_THREADS) lds.list[i] = parts.best[row * n + i];
+  int n = parts.parts * out.top;
+  const int i = threadIdx.x;
+  const uint64_t key = i < n ? parts.best[row * n + i] : 0;
+  if (i < n) lds.list[i] = key;
+  if (i == 0) lds.count = 0;
   Sums a = no_sums();
-  if ((int)threadIdx.x < parts.parts) a = parts.sums[row * parts.parts + threadIdx.x];
+  if (i < parts.parts) a = parts.sums[row * parts.parts + i];
   a = join<JOIN_THREADS>(a, lds.waves);
+  if (n > 128) {
+    // ranking them all would be n^2 (1 x 262144, 20 alternatives: 21 us, so 11.5);
+    // as in a tile, few reach the top-th best of 64 lanes' bests
+    if (wave_id() == 0) {
+      uint64_t best = 0;
+      for (int k = lane_id(); k < n; k += 64) best = lds.list[k] > best ? lds.list[k] : best;
+      best = kth(best, out.top);
+      if (i == 0) lds.bound = best;
+    }
+    __syncthreads();
+    if (i < n && key >= lds.bound) lds.list[atomicAdd(&lds.count, 1)] = key;
+    __syncthreads();
+    n = lds.count;
+  }
   rank_list<JOIN_THREADS>(lds, n, out.top);
   __syncthreads();
   if (wave_id() > 0) return;
@@ -554,12 +571,12 @@ int check_lp(int64_t rows, int64_t V, int64_t stride, int32_t top, int32_t dtype
 
 // Workgroups of a row in the forward: more than one where rows alone leave the
 // chip idle and a row is long enough to pay for the second launch that joins
-// them (1 x 131072 float32: 7.5 us, one workgroup 19; with 20 alternatives 13.5 and 29.
-// Parts of 8192 logits made 8 x 32000 slower: 15.6 us, whole rows 8 to 11).
+// them (1 x 131072 float32: 7.5 us, one workgroup 19; with 20 alternatives 11 and
+// 29.  8 x 32000 bf16, 20 alternatives: two parts 10.6 us, a whole row 8.2).
 constexpr int64_t SPLIT_GRID = 512, SPLIT_SPAN = 16384;
 constexpr int64_t SMALL_ROW = 512, ONE_WAVE = 4096;  // see lp_fwd
 int parts_of(int64_t rows, int64_t V) {
-  const int64_t room = SPLIT_GRID / rows, most = V / SPLIT_SPAN;
+  const int64_t room = SPLIT_GRID / rows, most = V <= 2 * SPLIT_SPAN ? 1 : (V + SPLIT_SPAN - 1) / SPLIT_SPAN;
   const int64_t n = room < most ? room : most;
   return n < 2 ? 1 : (int)(n < MAX_PARTS ? n : MAX_PARTS);
 }
@@ -568,13 +585,17 @@ int span_of(int64_t V, int parts) { return (int)(((V + parts - 1) / parts + 7) /
 // With alternatives: a wave a row for many short rows (8192 x 2000: 17 us, 256
 // threads 42; 64 x 2000: 10 and 7), 256 threads while a row is one tile of theirs,
 // 512 for many rows (16384 x 32000: 276 us, 1024 threads 312), 1024 for few (8 x
-// 32000: 8 us, 512 threads 11).
+// 32000: 8 us, 512 threads 11).  A part: 512 threads while it is one tile of theirs
+// (16 x 131072, 5 alternatives: 9.9 us, 1024 threads 11.5), 1024 past that (1 x
+// 50000 in three parts of 16672: 11.4 us, 512 threads 14.3).
 template <typename T>
 void fwd_launch(const T* x, int64_t stride, int64_t rows, const Out& out, Parts p, hipStream_t st) {
   const dim3 grid((unsigned)(rows * p.parts)), block(LP_THREADS);
   const bool split = p.parts > 1;
   if (out.top > 0) {
-    if (split)
+    if (split && p.span <= 8 * 512 * PIECES)
+      hipLaunchKernelGGL((lp_top<T, 512, true>), grid, dim3(512), 0, st, x, stride, out, p);
+    else if (split)
       hipLaunchKernelGGL((lp_top<T, 1024, true>), grid, dim3(1024), 0, st, x, stride, out, p);
     else if (out.V <= 8 * 64 * PIECES && rows >= 1024)
       hipLaunchKernelGGL((lp_top<T, 64, false>), grid, dim3(64), 0, st, x, stride, out, p);

@@ -113,7 +113,8 @@ def logits(shape, seed, dtype, spread=3.0):
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("rows,V,top", [(1, 1, 1), (3, 2, 2), (4, 7, 3), (5, 8, 8), (3, 64, 32), (4, 65, 5),
                                         (9, 257, 20), (300, 1000, 0), (5, 4099, 32), (3, 8192, 20), (3, 8193, 20),
-                                        (4, 32000, 20), (2, 32768, 32), (2, 32769, 7), (2, 70001, 20), (2, 131072, 0)])
+                                        (4, 32000, 20), (2, 32768, 32), (2, 32769, 7), (2, 70001, 20), (2, 131072, 0),
+                                        (1, 300001, 32), (1, 600000, 32)])
 def test_values_and_gradient(rows, V, top, dtype):
     check(*logits((rows, V), V + rows, dtype), top)
 
@@ -158,7 +159,7 @@ def test_masks(V, dtype):
     check(x, tokens, 0)
 
 
-@pytest.mark.parametrize("V", [600, 20000, 50000])
+@pytest.mark.parametrize("V", [600, 20000, 50000, 150000])
 def test_ties_and_orders(V):
     """Equal logits go by index, whatever their number; rising, falling and
     blockwise rows; a row whose likely tokens crowd a few groups (more
