@@ -174,14 +174,16 @@ struct From8 {
 // (workgroups, 2, d).  A thread's columns are the same in every row, so the
 // sums stay in its registers; the rows a workgroup takes side by side are
 // added in LDS at the end, in a fixed order.  No atomics: they would add in
-// another order on every run.  `large`: the matrix is FAR_BYTES or more; rows of
+// another order on every run.  A workgroup alone (see bwd_blocks) has the whole sums
+// and writes them to dweight and dbias, which are null otherwise.  `large`: the matrix is FAR_BYTES or more; rows of
 // several waves are then loaded past the caches (8192 x 8192: 80 -> 78 us; from
 // 8 bits at 16384 x 4096: 66 -> 58).
 template <typename Src, typename TX, typename TY, int TPR, int NV>
 __global__ void __launch_bounds__(ln_threads(TPR))
 ln_bwd(Src src, const TY* __restrict__ dy, int64_t ds, const void* __restrict__ w, bool w16,
        const float* __restrict__ mean, const float* __restrict__ rstd, TX* __restrict__ dx,
-       float* __restrict__ part, int64_t rows, int d, bool large) {
+       float* __restrict__ part, void* __restrict__ dweight, void* __restrict__ dbias, int64_t rows, int d,
+       bool large) {
   constexpr int RPB = ln_threads(TPR) / TPR;
   // a row's loads before the last row's work (8192 x 8192: 103 -> 88 us), where
   // the registers hold them: 1024 threads have 128 each, and spilled
@@ -274,14 +276,20 @@ ln_bwd(Src src, const TY* __restrict__ dy, int64_t ds, const void* __restrict__ 
     }
   }
   if (!w) return;
-  float* out = part + (int64_t)blockIdx.x * 2 * d;
+  const bool narrow = dweight && w16;
+  float* first = dweight ? reinterpret_cast<float*>(dweight) : part + (int64_t)blockIdx.x * 2 * d;
+  float* second = dweight ? reinterpret_cast<float*>(dbias) : first + d;
   if constexpr (RPB == 1) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = 8 * (i * TPR + t);
-      if (c < d) {
-        store8(out + c, d - c, dw[i]);
-        store8(out + d + c, d - c, db[i]);
+      if (c >= d) continue;
+      if (narrow) {
+        store8(reinterpret_cast<bf16*>(dweight) + c, d - c, dw[i]);
+        store8(reinterpret_cast<bf16*>(dbias) + c, d - c, db[i]);
+      } else {
+        store8(first + c, d - c, dw[i]);
+        store8(second + c, d - c, db[i]);
       }
     }
   } else {
@@ -297,7 +305,10 @@ ln_bwd(Src src, const TY* __restrict__ dy, int64_t ds, const void* __restrict__ 
         float s = sums[0][c];
 #pragma unroll
         for (int i = 1; i < RPB; ++i) s += sums[i][c];
-        out[which * d + c] = s;
+        if (narrow)
+          reinterpret_cast<bf16*>(which ? dbias : dweight)[c] = (bf16)s;
+        else
+          (which ? second : first)[c] = s;
       }
     }
   }
@@ -428,6 +439,16 @@ int64_t ln_blocks(int64_t rows, int64_t d, int64_t most) {
   return n < most ? n : most;
 }
 
+// The backward's workgroups.  One alone does without the partial sums' launch:
+// 5.5 us instead of 8.5 for 128 x 128 bf16, and 4 us of the caller's.  Past its
+// first few rows it loses that again (32 x 1024: 8.3 us, with partial sums
+// 8.6; 64 x 1024: 12.7 and 8.7).  Narrow rows take less each (152 x 112, five
+// turns: 7.9 and 8.7; 512 x 128, sixteen: 13.4 and 9.1).
+int64_t bwd_blocks(int64_t rows, int64_t d) {
+  const int64_t alone = d <= 256 ? 8 : 4;
+  return ln_blocks(rows, d, alone + 1) <= alone ? 1 : ln_blocks(rows, d, LN_BWD_BLOCKS);
+}
+
 // The built pairs of types: (bf16, bf16), (float32, float32) and a float32
 // input beside a bf16 output.
 bool pair_ok(int32_t xt, int32_t yt) {
@@ -482,7 +503,8 @@ int gmdn_layer_norm_fwd(const void* x, const void* weight, const void* bias, voi
 
 size_t gmdn_layer_norm_bwd_workspace_floats(int64_t rows, int64_t d) {
   if (rows <= 0 || check_dims(rows, d) != GMDN_OK) return 0;
-  return (size_t)(ln_blocks(rows, d, LN_BWD_BLOCKS) * 2 * d);
+  const int64_t nb = bwd_blocks(rows, d);
+  return nb == 1 ? 0 : (size_t)(nb * 2 * d);
 }
 
 int gmdn_layer_norm_bwd(const void* dy, const void* x, const int8_t* q, const float* scale, const void* weight,
@@ -499,8 +521,9 @@ int gmdn_layer_norm_bwd(const void* dy, const void* x, const int8_t* q, const fl
   int64_t nb = 0;
   if (rows > 0) {
     if (!dy || (!x && !q) || (x && q) || !mean || !rstd || !dx) return GMDN_ERR_ARG;
-    nb = ln_blocks(rows, d, LN_BWD_BLOCKS);
-    if (weight && (!workspace || workspace_floats < (size_t)(nb * 2 * d))) return GMDN_ERR_WORKSPACE;
+    nb = bwd_blocks(rows, d);
+    if (weight && nb > 1 && (!workspace || workspace_floats < (size_t)(nb * 2 * d))) return GMDN_ERR_WORKSPACE;
+    void *const dw = nb == 1 ? dweight : nullptr, *const db = nb == 1 ? dbias : nullptr;
     const bool large = rows * d * (x_type == GMDN_DTYPE_F32 ? 4 : 2) >= FAR_BYTES;
     with_types(x_type, y_type, [&](auto tx, auto ty) {
       using TX = decltype(tx);
@@ -508,18 +531,20 @@ int gmdn_layer_norm_bwd(const void* dy, const void* x, const int8_t* q, const fl
       with_shape(d, [&](auto s) {
         using S = decltype(s);
         const dim3 grid((unsigned)nb), block(ln_threads(S::TPR));
-              if (q)
+        if (q)
           hipLaunchKernelGGL((ln_bwd<From8, TX, TY, S::TPR, S::NV>), grid, block, 0, st, From8{q, scale},
-                             (const TY*)dy, dy_stride, weight, w16, mean, rstd, (TX*)dx, workspace, rows, (int)d, large);
+                             (const TY*)dy, dy_stride, weight, w16, mean, rstd, (TX*)dx, workspace, dw, db, rows,
+                             (int)d, large);
         else
           hipLaunchKernelGGL((ln_bwd<FromX<TX>, TX, TY, S::TPR, S::NV>), grid, block, 0, st,
                              FromX<TX>{(const TX*)x, x_stride}, (const TY*)dy, dy_stride, weight, w16, mean, rstd,
-                             (TX*)dx, workspace, rows, (int)d, large);
+                             (TX*)dx, workspace, dw, db, rows,
+                             (int)d, large);
       });
     });
     if (hipGetLastError() != hipSuccess) return GMDN_ERR_LAUNCH;
   }
-  if (!weight) return GMDN_OK;
+  if (!weight || nb == 1) return GMDN_OK;
   hipLaunchKernelGGL(ln_sums, dim3((unsigned)((2 * d + LN_COLS - 1) / LN_COLS)), dim3(LN_SUM_THREADS), 0, st, workspace,
                      dweight, dbias, w16, (int)d, (int)nb);
   return launched();

@@ -153,12 +153,12 @@ Grads3 norm_bwd(const Tensor& dy, const Tensor* x, const Kept* k, const OptTenso
   Tensor dx = fresh(dy, dy.sizes(), x_dtype);
   Tensor dw = w.w ? at::empty_like(*w.w) : fresh(dy, {0}), db = w.w ? at::empty_like(*w.w) : fresh(dy, {0});
   const size_t need = w.w ? gmdn_layer_norm_bwd_workspace_floats(g.rows, g.d) : 0;
-  Tensor ws = fresh(dy, {(int64_t)need});
+  const Tensor ws = need ? fresh(dy, {(int64_t)need}) : Tensor();
   if (g.rows || w.w)
     check(gmdn_layer_norm_bwd(g.ptr(), x ? r.ptr() : nullptr, x ? nullptr : k->q.data_ptr<int8_t>(),
                               x ? nullptr : fp(k->scale), ptr(w.w), fp(mean), fp(rstd), dx.data_ptr(),
-                              w.w ? dw.data_ptr() : nullptr, w.w ? db.data_ptr() : nullptr, fp(ws), need, g.rows, g.d,
-                              g.stride, x ? r.stride : 0, xc, yc, w.code, stream_of(dy)),
+                              w.w ? dw.data_ptr() : nullptr, w.w ? db.data_ptr() : nullptr, need ? fp(ws) : nullptr, need, g.rows,
+                              g.d, g.stride, x ? r.stride : 0, xc, yc, w.code, stream_of(dy)),
           "gmdn_layer_norm_bwd");
   return {dx, dw, db};
 }

@@ -38,7 +38,8 @@ int gmdn_layer_norm_fwd(const void* x, const void* weight, const void* bias, voi
                         int8_t* q, float* scale, int64_t rows, int64_t d, int64_t x_stride, float eps,
                         int32_t x_type, int32_t y_type, int32_t w_type, void* stream);
 
-/* Floats of the backward's workspace (sums of the weight's gradient). */
+/* Floats of the backward's workspace (sums of the weight's gradient); 0 for few
+ * rows. */
 size_t gmdn_layer_norm_bwd_workspace_floats(int64_t rows, int64_t d);
 
 /* dx (x_type), dweight and dbias (w_type; where weight is given) from dy

@@ -109,6 +109,23 @@ def test_optional_and_bfloat16_weights(which, w_dtype):
     assert all(g.dtype == w_dtype for g in grads[1:])
 
 
+@pytest.mark.parametrize("w_dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,d", [(1, 200), (16, 200), (128, 200), (129, 200), (32, 1000), (33, 1000), (16, 1500),
+                                    (4, 5001), (5, 5001), (4, 16384)])
+def test_weight_gradients_of_few_rows(rows, d, w_dtype):
+    """One workgroup writes them itself up to a number of rows; past it their
+    sums go through memory."""
+    dev = _dev()
+    x, w, b, dy = data(rows, d, rows + d, torch.float32, torch.bfloat16, w_dtype)
+    ref = reference(x.double(), w.double(), b.double(), dy.double(), 1e-5)
+    args = [t.to(dev) for t in (x, w, b)]
+    _, mean, rstd, _, _ = torch.ops.gmdn.layer_norm_fwd(*args, 1e-5, torch.bfloat16, False)
+    grads = torch.ops.gmdn.layer_norm_bwd(dy.to(dev), args[0], args[1], mean, rstd)
+    for name, got in zip(("dx", "dw", "db"), grads):
+        assert_close(got, *ref[name], name)
+    assert grads[1].dtype == grads[2].dtype == w_dtype
+
+
 def test_strided_rows_and_gradients():
     """A slice of a wider tensor at an odd offset, a transposed batch and a
     broadcast cotangent give what their contiguous copies give."""
