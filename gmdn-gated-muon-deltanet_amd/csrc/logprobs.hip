@@ -112,6 +112,10 @@ struct Out {
   float *lp, *entropy, *stats, *top_lp;
   int64_t* top_tokens;
   int V, top;
+  Out from(int64_t row) const {
+    return {tokens + row, ignore, lp + row, entropy + row, stats + 2 * row, top ? top_lp + row * top : nullptr,
+            top ? top_tokens + row * top : nullptr, V, top};
+  }
   template <typename T>
   GMDN_DEV void row(int64_t row, const Row& r, const T* x) const {
     const int64_t token = tokens[row];
@@ -588,6 +592,10 @@ int span_of(int64_t V, int parts) { return (int)(((V + parts - 1) / parts + 7) /
 // 32000: 8 us, 512 threads 11).  A part: 512 threads while it is one tile of theirs
 // (16 x 131072, 5 alternatives: 9.9 us, 1024 threads 11.5), 1024 past that (1 x
 // 50000 in three parts of 16672: 11.4 us, 512 threads 14.3).
+//
+// A launch has fewer than 2^32 threads, so more rows than these go in several
+// (1024 threads a row at most).
+constexpr int64_t LAUNCH_ROWS = 1 << 21;
 template <typename T>
 void fwd_launch(const T* x, int64_t stride, int64_t rows, const Out& out, Parts p, hipStream_t st) {
   const dim3 grid((unsigned)(rows * p.parts)), block(LP_THREADS);
@@ -675,10 +683,13 @@ int gmdn_logprobs_fwd(const void* logits, const int64_t* tokens, float* logprob,
   // the keys first: 8-byte values at the workspace's start, the sums behind them
   uint64_t* best = static_cast<uint64_t*>(workspace);
   const Parts p{need ? reinterpret_cast<Sums*>(best + rows * parts * top) : nullptr, best, parts, span_of(vocab, parts)};
-  if (dtype == GMDN_DTYPE_BF16)
-    fwd_launch((const bf16*)logits, stride, rows, out, p, (hipStream_t)stream);
-  else
-    fwd_launch((const float*)logits, stride, rows, out, p, (hipStream_t)stream);
+  for (int64_t r = 0; r < rows; r += LAUNCH_ROWS) {
+    const int64_t n = rows - r < LAUNCH_ROWS ? rows - r : LAUNCH_ROWS;
+    if (dtype == GMDN_DTYPE_BF16)
+      fwd_launch((const bf16*)logits + r * stride, stride, n, out.from(r), p, (hipStream_t)stream);
+    else
+      fwd_launch((const float*)logits + r * stride, stride, n, out.from(r), p, (hipStream_t)stream);
+  }
   return launched();
 }
 
@@ -689,12 +700,19 @@ int gmdn_logprobs_bwd(const void* logits, const int64_t* tokens, const float* st
   const int rc = check_lp(rows, vocab, stride, top, dtype);
   if (rc != GMDN_OK || rows == 0) return rc;
   if (!logits || !tokens || !stats || !entropy || !dlogits || (dtop && top && !top_tokens)) return GMDN_ERR_ARG;
-  if (dtype == GMDN_DTYPE_BF16)
-    bwd_launch((const bf16*)logits, stride, rows, tokens, stats, entropy, top_tokens, dlogprob, dentropy, dtop,
-               (bf16*)dlogits, vocab, top, ignore_index, (hipStream_t)stream);
-  else
-    bwd_launch((const float*)logits, stride, rows, tokens, stats, entropy, top_tokens, dlogprob, dentropy, dtop,
-               (float*)dlogits, vocab, top, ignore_index, (hipStream_t)stream);
+  auto launch = [&](auto* x, auto* dx, int64_t r, int64_t n) {
+    bwd_launch(x + r * stride, stride, n, tokens + r, stats + 2 * r, entropy + r,
+               top_tokens ? top_tokens + r * top : nullptr, dlogprob ? dlogprob + r : nullptr,
+               dentropy ? dentropy + r : nullptr, dtop ? dtop + r * top : nullptr, dx + r * vocab, vocab, top,
+               ignore_index, (hipStream_t)stream);
+  };
+  for (int64_t r = 0; r < rows; r += LAUNCH_ROWS) {
+    const int64_t n = rows - r < LAUNCH_ROWS ? rows - r : LAUNCH_ROWS;
+    if (dtype == GMDN_DTYPE_BF16)
+      launch((const bf16*)logits, (bf16*)dlogits, r, n);
+    else
+      launch((const float*)logits, (float*)dlogits, r, n);
+  }
   return launched();
 }
 

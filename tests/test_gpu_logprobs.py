@@ -214,6 +214,28 @@ def test_large_matrices_equal_their_parts():
         assert torch.equal(got.logprob[a:a + 200], part.logprob) and torch.equal(got.entropy[a:a + 200], part.entropy)
 
 
+@pytest.mark.parametrize("top", [0, 2])
+def test_many_short_rows(top):
+    """More rows than a launch has threads for, a workgroup a row: the bits of
+    their parts."""
+    dev = _dev()
+    rows, V = (1 << 24) + 5, 5
+    gen = torch.Generator(device=dev).manual_seed(6)
+    x = torch.randn(rows, V, generator=gen, device=dev).bfloat16()
+    tokens = torch.randint(V, (rows,), generator=gen, device=dev)
+    g = torch.randn(rows, generator=gen, device=dev)
+
+    def run(a, b):
+        out = torch.ops.gmdn.logprobs_fwd(x[a:b], tokens[a:b], top, -100)
+        dtop = g[a:b, None].expand(b - a, top).contiguous() if top else None
+        return (*out, torch.ops.gmdn.logprobs_bwd(x[a:b], tokens[a:b], out[4], out[1], out[3], g[a:b], None, dtop, -100))
+
+    got = run(0, rows)
+    for a in (0, (1 << 21) - 700, (1 << 23) - 700, rows - 1500):
+        for whole, part in zip(got, run(a, a + 1500)):
+            assert torch.equal(whole[a:a + 1500], part)
+
+
 def test_large_and_peaked_logits():
     """Logits far from zero, and a token with nearly all the probability: its
     log probability keeps relative accuracy to float32's resolution of 1."""
