@@ -53,6 +53,13 @@ GMDN_DEV float max3(float a, float b, float c) {
 GMDN_DEV float max8(const float (&x)[8], float m) {
   return max3(max3(x[0], x[1], x[2]), max3(x[3], x[4], x[5]), max3(x[6], x[7], m));
 }
+GMDN_DEV float min8(const float (&x)[8]) {
+  float r, s;
+  asm("v_min3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(x[0]), "v"(x[1]), "v"(x[2]));
+  asm("v_min3_f32 %0, %1, %2, %3" : "=v"(s) : "v"(x[3]), "v"(x[4]), "v"(x[5]));
+  asm("v_min3_f32 %0, %0, %1, %2" : "+v"(r) : "v"(x[6]), "v"(x[7]));
+  return fminf(r, s);
+}
 // The terms of a piece at the maximum that `a` has.
 GMDN_DEV void terms8(Sums& a, const float (&x)[8]) {
 #pragma unroll
@@ -310,7 +317,11 @@ GMDN_DEV void slow_top(const T* x, int first, int last, int top, TopLds<NT>& lds
 // 512 apart, so that neighbours do not share a group).  A group's best is its
 // largest value with the last index of the first piece that has it, which no
 // better logit of that value exceeds: equal logits, masked ones above all,
-// stay out of the list by their index.  Those that reach the bound join the best
+// stay out of the list by their index.  In a row with fewer allowed
+// tokens than are wanted the bound is the masks' value, and of the first wave's
+// pieces of nothing else only those with the first `top` logits go on (4816 x 1220
+// float32, five allowed of each, 32 wanted: 128 -> 24 us).  With 512 threads that is
+// done for -inf alone: to know other values cost 5 to 10 % of every row.  Those that reach the bound join the best
 // of the tiles before in the list, which is ranked.  A tile that gives more
 // than LDS holds, or a NaN, is left to slow_top.  The sums are returned in the
 // first wave.
@@ -334,11 +345,13 @@ GMDN_DEV Sums top_of(const T* x, int first, int last, int top, TopLds<NT>& lds, 
     // the thread's best: its value, and the first piece that has it
     float bv = -INFINITY;
     int bp = 0;
+    [[maybe_unused]] uint64_t flat = 0;  // the wave's first pieces of one value
 #pragma unroll
     for (int i = 0; i < PIECES; ++i) {
       float v[8];
       raw[i].get(v);
       most[i] = max8(v, -INFINITY);
+      if (NT <= 256 && i == 0) flat = __ballot(min8(v) == most[0]);
       rescale(a, max3(a.m, most[i], most[i]));
       terms8(a, v);
       if (most[i] > bv) {
@@ -376,10 +389,18 @@ GMDN_DEV Sums top_of(const T* x, int first, int last, int top, TopLds<NT>& lds, 
     const uint64_t least = lds.bound;
     const float lv = value_of(least);
     const int upto = least ? index_of(least) : 0x7fffffff;
+    int upto0 = upto;  // in a thread's first piece
+    if (tid < 64 && (NT <= 256 || lv == -INFINITY)) {
+      uint64_t equal = __ballot(most[0] == lv && c0 + 8 * tid + 8 <= last);
+      if constexpr (NT <= 256) equal &= flat;
+      for (int k = 8; k < top; k += 8) equal &= equal - 1;
+      const int enough = c0 + 8 * (__ffsll((long long)equal) - 1);
+      if (equal && enough < upto) upto0 = enough;
+    }
 #pragma unroll
     for (int i = 0; i < PIECES; ++i) {
       const int c = c0 + 8 * (i * NT + tid);
-      if ((most[i] > lv || (most[i] == lv && c <= upto)) && c < last) {
+      if ((most[i] > lv || (most[i] == lv && c <= (i == 0 ? upto0 : upto))) && c < last) {
         const int at = atomicAdd(&lds.pieces, 1);
         if (at < TopLds<NT>::PIECES_) {
           float v[8];

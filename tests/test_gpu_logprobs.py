@@ -159,6 +159,23 @@ def test_masks(V, dtype):
     check(x, tokens, 0)
 
 
+@pytest.mark.parametrize("mask", [-math.inf, -1e30, -3.0])
+@pytest.mark.parametrize("rows,V", [(24, 600), (1030, 1220), (24, 7681), (24, 20000), (260, 9001), (3, 140000)])
+def test_handfuls(rows, V, mask):
+    """Rows with 0 to 40 logits beside the masks, one piece of them, and one in
+    each of the first columns' pieces."""
+    gen = torch.Generator().manual_seed(V)
+    x = torch.full((rows, V), mask)
+    for r in range(min(rows, 24)):
+        at = torch.randperm(V, generator=gen)[:2 * r if r < 21 else 8]
+        at = at if r < 21 else torch.arange(8) + 16 if r == 21 else 8 * torch.arange(8) + r
+        x[r, at] = torch.randn(len(at), generator=gen)
+    x[24:] = x[:24].repeat(rows // 24 + 1, 1)[24:rows]
+    tokens = torch.randint(V, (rows,), generator=gen)
+    for top in (1, 8, 32):
+        check(x, tokens, top)
+
+
 @pytest.mark.parametrize("V", [600, 20000, 50000, 150000])
 def test_ties_and_orders(V):
     """Equal logits go by index, whatever their number; rising, falling and
