@@ -60,6 +60,13 @@ inline bool wants_grad(std::initializer_list<const Tensor*> ts) {
     if (t->defined() && t->requires_grad()) return true;
   return false;
 }
+// Refuses inputs that carry a forward-mode tangent: calls below autograd would
+// return outputs without one, and no error.
+inline void refuse_tangents(const char* name, std::initializer_list<const Tensor*> ts) {
+  for (const Tensor* t : ts)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(/*level=*/0).defined(), "gmdn::", name,
+                                " has no forward-mode derivative (jvp)");
+}
 inline Tensor opt(const OptTensor& t) { return t ? *t : Tensor(); }
 inline OptTensor opt(const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
 

@@ -327,6 +327,7 @@ struct LayerNormFwd : torch::autograd::Function<LayerNormFwd> {
 Norm layer_norm_fwd_ad(const Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps, ScalarType dtype,
                        bool pack) {
   const Tensor w = opt(weight), b = opt(bias);
+  refuse_tangents("layer_norm_fwd", {&x, &w, &b});
   if (!wants_grad({&x, &w, &b})) {
     at::AutoDispatchBelowADInplaceOrView below;
     return GMDN_OP(layer_norm_fwd).call(x, weight, bias, eps, dtype, pack);
@@ -353,6 +354,7 @@ struct Gelu8Fwd : torch::autograd::Function<Gelu8Fwd> {
   }
 };
 std::tuple<Tensor, Tensor, Tensor> gelu8_fwd_ad(const Tensor& h, bool pack) {
+  refuse_tangents("gelu8_fwd", {&h});
   if (!wants_grad({&h})) {
     at::AutoDispatchBelowADInplaceOrView below;
     return GMDN_OP(gelu8_fwd).call(h, pack);
@@ -387,6 +389,7 @@ struct LogprobsFwd : torch::autograd::Function<LogprobsFwd> {
 };
 std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> logprobs_fwd_ad(const Tensor& logits, const Tensor& tokens,
                                                                    c10::SymInt top, c10::SymInt ignore_index) {
+  refuse_tangents("logprobs_fwd", {&logits});
   if (!wants_grad({&logits})) {
     at::AutoDispatchBelowADInplaceOrView below;
     return GMDN_OP(logprobs_fwd).call(logits, tokens, top, ignore_index);
