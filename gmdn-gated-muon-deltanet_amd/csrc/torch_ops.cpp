@@ -367,6 +367,7 @@ struct StateScan : torch::autograd::Function<StateScan> {
 std::tuple<Tensor, Tensor, Tensor> state_scan_ad(const Tensor& U, const Tensor& K, const Tensor& a, const Tensor& b,
                                                  const Tensor& m, const Tensor& n, c10::SymInt rule, c10::SymInt ns,
                                                  c10::SymInt precision, bool save) {
+  refuse_tangents("state_scan", {&U, &K, &a, &b, &m, &n});
   if (!wants_grad({&U, &K, &a, &b, &m, &n})) {
     at::AutoDispatchBelowADInplaceOrView below;
     return GMDN_OP(state_scan).call(U, K, a, b, m, n, rule, ns, precision, save);
@@ -417,6 +418,7 @@ std::tuple<Tensor, Tensor> chunk_fwd_ad(const Tensor& q, const Tensor& k, const 
                                         const Tensor& g, const OptTensor& gmu, const OptTensor& gnu, c10::SymInt rule,
                                         c10::SymInt ns, double eps, bool record) {
   const Tensor m = opt(gmu), n = opt(gnu);
+  refuse_tangents("chunk_fwd", {&q, &k, &v, &beta, &g, &m, &n});
   if (!wants_grad({&q, &k, &v, &beta, &g, &m, &n})) {
     at::AutoDispatchBelowADInplaceOrView below;
     return GMDN_OP(chunk_fwd).call(q, k, v, beta, g, gmu, gnu, rule, ns, eps, record);
@@ -448,6 +450,7 @@ struct WyFwd : torch::autograd::Function<WyFwd> {
 };
 std::tuple<Tensor, Tensor> wy_fwd_ad(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& beta,
                                      const Tensor& g, bool record) {
+  refuse_tangents("wy_fwd", {&q, &k, &v, &beta, &g});
   if (!wants_grad({&q, &k, &v, &beta, &g})) {
     at::AutoDispatchBelowADInplaceOrView below;
     return GMDN_OP(wy_fwd).call(q, k, v, beta, g, record);
@@ -475,6 +478,7 @@ struct FrontFwd : torch::autograd::Function<FrontFwd> {
 };
 std::tuple<Tensor, Tensor, Tensor> front_fwd_ad(const Tensor& y, const Tensor& weight, const Tensor& bias,
                                                 c10::SymInt dh) {
+  refuse_tangents("front_fwd", {&y, &weight, &bias});
   if (!wants_grad({&y, &weight, &bias})) {
     at::AutoDispatchBelowADInplaceOrView below;
     return GMDN_OP(front_fwd).call(y, weight, bias, dh);
@@ -499,6 +503,7 @@ struct GatesFwd : torch::autograd::Function<GatesFwd> {
   }
 };
 Tensor gates_fwd_ad(const Tensor& y, c10::SymInt heads, c10::SymInt n_gates) {
+  refuse_tangents("gates_fwd", {&y});
   if (!wants_grad({&y})) {
     at::AutoDispatchBelowADInplaceOrView below;
     return GMDN_OP(gates_fwd).call(y, heads, n_gates);
@@ -524,6 +529,7 @@ struct HeadNorm : torch::autograd::Function<HeadNorm> {
   }
 };
 std::tuple<Tensor, Tensor> head_norm_fwd_ad(const Tensor& x, const Tensor& weight, double eps) {
+  refuse_tangents("head_norm_fwd", {&x, &weight});
   if (!wants_grad({&x, &weight})) {
     at::AutoDispatchBelowADInplaceOrView below;
     return GMDN_OP(head_norm_fwd).call(x, weight, eps);

@@ -8,6 +8,7 @@ from torch._subclasses.fake_tensor import FakeTensorMode
 
 from gmdn_amd import act8, layer_norm, logprobs
 from gmdn_amd import ops  # noqa: F401
+from test_ops import _meta_ops
 
 
 def _lm_calls():
@@ -67,3 +68,9 @@ def test_products_behind_them_keep_theirs():
 
         assert fwd.unpack_dual(act8.mlp(x, w1, dual(w2))).tangent is not None
         assert fwd.unpack_dual(act8.linear(dual(x), w1)).tangent is not None
+
+
+@pytest.mark.parametrize("name", [x[0] for x in _meta_ops()])
+def test_mixer_operators_refuse_tangents(name):
+    _, call, inputs = next(x for x in _meta_ops() if x[0] == name)
+    _refuses(call, [t.detach() for t in inputs])
