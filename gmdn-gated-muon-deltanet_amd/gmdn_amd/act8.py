@@ -11,7 +11,8 @@ group below 2^-100 reads back as zeros; one that holds an infinity or a NaN
 reads back as NaN.
 
 The forward's outputs are computed from the activations themselves; only the
-backward sees the checkpoints, and a call without gradients makes none.
+backward sees the checkpoints.  A call without gradients makes none, and one
+with frozen weights none that only they would want.
 
 * ``pack`` / ``unpack`` -- a checkpoint of any tensor.
 * ``gelu``     -- GELU that keeps its input in 8 bits.
@@ -74,10 +75,15 @@ def _flat(t: Tensor) -> Tensor:
     return t.reshape(-1, t.shape[-1])
 
 
+def _kept(x: Tensor, wanted: bool):
+    """The checkpoint of a product's input, where the weight wants its gradient."""
+    return torch.ops.gmdn.act8_pack(x) if wanted else (None, None)
+
+
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias):
-        ctx.save_for_backward(*torch.ops.gmdn.act8_pack(x), weight)
+        ctx.save_for_backward(*_kept(x, ctx.needs_input_grad[1]), weight)
         ctx.has_bias = bias is not None
         return F.linear(x, weight, bias)
 
@@ -112,30 +118,31 @@ def _mlp_forward(y, w1, w2, pack=True):
     return F.linear(a, w2), qh, sh
 
 
-def _mlp_backward(dout, qh, sh, w1, w2, need1, need2, input_again):
-    """(dy, dw1, dw2) of linear, GELU, linear; ``input_again`` gives the input
-    from its checkpoint, where the first weight wants its gradient."""
+def _mlp_backward(dout, qh, sh, w1, w2, need_y, need1, need2, input_again):
+    """(dy, dw1, dw2) of linear, GELU, linear, None where not needed;
+    ``input_again`` gives the input from its checkpoint, where the first weight
+    wants its gradient."""
     da = dout @ w2
     dh, a = torch.ops.gmdn.gelu8_bwd(da, qh, sh, need2)
     del da
     dw2 = _flat(dout).t() @ _flat(a) if need2 else None
     del a
     dw1 = _flat(dh).t() @ _flat(input_again()) if need1 else None
-    return dh @ w1, dw1, dw2
+    return dh @ w1 if need_y else None, dw1, dw2
 
 
 class _Mlp(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w1, w2):
         out, qh, sh = _mlp_forward(x, w1, w2)
-        ctx.save_for_backward(*torch.ops.gmdn.act8_pack(x), qh, sh, w1, w2)
+        ctx.save_for_backward(*_kept(x, ctx.needs_input_grad[1]), qh, sh, w1, w2)
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
         q, scale, qh, sh, w1, w2 = ctx.saved_tensors
-        return _mlp_backward(dout, qh, sh, w1, w2, *ctx.needs_input_grad[1:3],
+        return _mlp_backward(dout, qh, sh, w1, w2, *ctx.needs_input_grad,
                              lambda: torch.ops.gmdn.act8_unpack(q, scale, dout.dtype))
 
 
@@ -152,9 +159,11 @@ def mlp(x: Tensor, w1: Tensor, w2: Tensor) -> Tensor:
 class _NormMlp(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, w1, w2, eps):
-        y, mean, rstd, q, scale = torch.ops.gmdn.layer_norm_fwd(x, weight, bias, eps, w1.dtype, True)
+        # all but the second weight's gradient want the norm's input again
+        pack = any(ctx.needs_input_grad[:4])
+        y, mean, rstd, q, scale = torch.ops.gmdn.layer_norm_fwd(x, weight, bias, eps, w1.dtype, pack)
         out, qh, sh = _mlp_forward(y, w1, w2)
-        ctx.save_for_backward(q, scale, mean, rstd, qh, sh, weight, bias, w1, w2)
+        ctx.save_for_backward(*((q, scale, mean, rstd) if pack else (None,) * 4), qh, sh, weight, bias, w1, w2)
         ctx.x_dtype = x.dtype
         return out
 
@@ -162,9 +171,12 @@ class _NormMlp(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
         q, scale, mean, rstd, qh, sh, weight, bias, w1, w2 = ctx.saved_tensors
+        need_norm = any(ctx.needs_input_grad[:3])
         dy, dw1, dw2 = _mlp_backward(
-            dout, qh, sh, w1, w2, *ctx.needs_input_grad[3:5],
+            dout, qh, sh, w1, w2, need_norm, *ctx.needs_input_grad[3:5],
             lambda: torch.ops.gmdn.layer_norm8_rebuild(q, scale, weight, bias, mean, rstd, dout.dtype))
+        if not need_norm:
+            return None, None, None, dw1, dw2, None
         dx, dweight, dbias = torch.ops.gmdn.layer_norm8_bwd(dy, q, scale, weight, mean, rstd, ctx.x_dtype)
         return (dx, dweight if weight is not None else None, dbias if bias is not None else None, dw1, dw2, None)
 
