@@ -243,9 +243,18 @@ ln_bwd(Src src, const TY* __restrict__ dy, int64_t ds, const void* __restrict__ 
     if constexpr (AHEAD) fetch(r + step);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
+      const int c = 8 * (i * TPR + t);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[i][j] = (v[i][j] - m) * rs;  // xh
+      if (c + 8 > d) {  // past the row's end g is 0, but -m rs may be infinite
+        int end = d;
+        asm volatile("" : "+s"(end));  // compared here: sixteen masks kept over the loop spill
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (c + j >= end) v[i][j] = 0.f;
+      }
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        v[i][j] = (v[i][j] - m) * rs;  // xh; a dead lane's g is 0
         dw[i][j] += g[i][j] * v[i][j];
         db[i][j] += g[i][j];
         g[i][j] *= wv[i][j];
