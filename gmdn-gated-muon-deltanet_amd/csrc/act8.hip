@@ -5,7 +5,7 @@
 // each, its amax a butterfly over them; nothing is shared between groups.
 // Memory bound (GELU's forward nearly by its vector instructions too: they are
 // active in 98 % of its cycles; fewer of them gained nothing).  At 16384 x 4096 bf16:
-// pack 35 us (5.8 TB/s), unpack 29 us (6.9), GELU 59 us (5.7), its backward with
+// pack 35 us (5.8 TB/s), unpack 29 us (6.9), GELU 61 us (5.5), its backward with
 // the output again 76 us (6.2); a 1 GiB copy reaches 5.1 TB/s.
 #include "../../include/gmdn_lm.h"
 #include "rows8.h"

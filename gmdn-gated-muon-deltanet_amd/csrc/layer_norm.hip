@@ -11,8 +11,8 @@
 // matrix is read and written once; the deviation is a second sum over the
 // centred registers (a sum of squares would cancel for rows far from zero).
 // At 5.1 TB/s (what a 1 GiB copy reaches):
-//   16384 x 1024, float32 in, bf16 out   forward 19 us (floor 20), backward 27 + 5 us (33)
-//   8192 x 8192 bf16                     forward 49 us (53), backward 63 + 6 us (79)
+//   16384 x 1024, float32 in, bf16 out   forward 19 us (floor 20), backward 31 + 5 us (33)
+//   8192 x 8192 bf16                     forward 48 us (53), backward 64 + 6 us (79)
 // (in brackets the floor: the outputs stay in the cache in part).
 #include "../../include/gmdn_lm.h"
 #include <type_traits>

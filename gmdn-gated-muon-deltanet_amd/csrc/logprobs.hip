@@ -13,8 +13,8 @@
 // The forward reads the logits once; nothing of their size is written.  It is
 // near both bounds: 10.6 instruction slots a logit (the exponential takes four)
 // keep the vector units busy in 91 % of its cycles, and 16384 x 32000 bf16 logits go by
-// in 160 us, 6.6 TB/s (172 between backward passes; a kernel that only reads
-// reaches 7.0).  The backward reads and writes once: 332 us, 6.3 TB/s (a copy 5.1).
+// in 163 us, 6.4 TB/s (172 between backward passes; a kernel that only reads
+// reaches 7.0).  The backward reads and writes once: 333 us, 6.3 TB/s (a copy 5.1).
 #include "../../include/gmdn_lm.h"
 #include <float.h>
 #include "rows8.h"
@@ -178,8 +178,8 @@ GMDN_DEV Sums sums_of(const T* x, int first, int last, int t) {
 }
 
 // A row is TPR threads of the workgroup's 256 (SPLIT: 256 for a part of it): 16
-// up to 512 logits (65536 x 257 float32: 14 us, a wave each 22, 256 threads each 63),
-// a wave up to 4096 (16384 x 4096 bf16: 26 us, 256 threads 33; x 8000: 52 and 50).
+// up to 512 logits (65536 x 257 float32: 14 us, a wave each 23, 256 threads each 53),
+// a wave up to 4096 (16384 x 4096 bf16: 26 us, 256 threads 37; x 8000: 54 and 53).
 constexpr int LP_THREADS = 256;
 template <typename T, int TPR, bool SPLIT, bool FAR>
 __global__ void __launch_bounds__(LP_THREADS)
@@ -513,8 +513,11 @@ lp_join(const T* __restrict__ logits, int64_t stride, Out out, Parts parts) {
 // TPR threads take `span` columns of a row; a workgroup NT / TPR rows.  The
 // token's term goes to its column where that is computed.  TOP: the columns of
 // token and alternatives are written again with their terms at the end.
-// Rows of 1024 threads from 8192 logits on (16384 x 32000 bf16: 333 us, of 256
-// threads 372; x 4096: 86 and 44).
+// Rows of 1024 threads past 8192 logits (16384 x 32000 bf16: 337 us, of 256
+// threads 403; x 8000: 112 and 90, x 9000 still 130 and 109), of a wave up to 4096
+// (x 4096: 47 and 46), of 16 up to 512 (65536 x 257 float32: 28 us, of a wave 32,
+// of 256 threads 54).  With alternatives' terms always of 256, also where that is
+// far off: 16384 x 257 float32 with 20 takes 71 us, without them 8.7.
 template <typename T, int NT, int TPR, bool TOP>
 __global__ void __launch_bounds__(NT)
 lp_bwd(const T* __restrict__ logits, int64_t stride, int64_t rows, const int64_t* __restrict__ tokens,
@@ -596,8 +599,8 @@ int check_lp(int64_t rows, int64_t V, int64_t stride, int32_t top, int32_t dtype
 
 // Workgroups of a row in the forward: more than one where rows alone leave the
 // chip idle and a row is long enough to pay for the second launch that joins
-// them (1 x 131072 float32: 7.5 us, one workgroup 19; with 20 alternatives 11 and
-// 29.  8 x 32000 bf16, 20 alternatives: two parts 10.6 us, a whole row 8.2).
+// them (1 x 131072 float32: 7.8 us, one workgroup 11; with 20 alternatives 11 and
+// 22.  8 x 32000 bf16, 20 alternatives: two parts 10.5 us, a whole row 8.1).
 constexpr int64_t SPLIT_GRID = 512, SPLIT_SPAN = 16384;
 constexpr int64_t SMALL_ROW = 512, ONE_WAVE = 4096;  // see lp_fwd
 int parts_of(int64_t rows, int64_t V) {
@@ -607,12 +610,15 @@ int parts_of(int64_t rows, int64_t V) {
 }
 int span_of(int64_t V, int parts) { return (int)(((V + parts - 1) / parts + 7) / 8 * 8); }
 
-// With alternatives: a wave a row for many short rows (8192 x 2000: 17 us, 256
-// threads 42; 64 x 2000: 10 and 7), 256 threads while a row is one tile of theirs,
-// 512 for many rows (16384 x 32000: 276 us, 1024 threads 312), 1024 for few (8 x
-// 32000: 8 us, 512 threads 11).  A part: 512 threads while it is one tile of theirs
-// (16 x 131072, 5 alternatives: 9.9 us, 1024 threads 11.5), 1024 past that (1 x
-// 50000 in three parts of 16672: 11.4 us, 512 threads 14.3).
+// With alternatives (20 of bf16 rows here): a wave a row for many short rows (8192 x
+// 2000: 22 us, 256 threads 44; 64 x 2000: 7.8 and 7.6), 256 threads while a row is
+// one tile of theirs (2048 x 8000: 17 us, 512 threads 24; x 9000: 27 and 24), 512
+// for many rows (16384 x 32000: 279 us, 1024 threads 365), 1024 for few (256 x
+// 32000: 9.8 us, 512 threads 12.4; 8 x 32000: 8.1 and 11.3).  A part: 512 threads
+// while it is one tile of theirs (16 x 131072, 5 alternatives: 10.2 us, 1024 threads
+// 11.4), 1024 past that, where rows or parts are too many for more of them (100 x
+// 100000 in 5 parts of 20000: 18.6 us, 512 threads 21.2; 1 x 1000000 in 32: 13.3
+// and 16.6).
 //
 // A launch has fewer than 2^32 threads, so more rows than these go in several
 // (1024 threads a row at most).
