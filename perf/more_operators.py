@@ -186,7 +186,7 @@ def _run_own(s):
         if not train:
             return {"r": r, "z": z}
         dx, dy, dw, dpost, dgate, dscale = op.residual_norm_bwd(s["dr"], s["dz"], r, s["y"], *parts, rstd, post_rstd)
-        out = {"r": r, "z": z, "dx": dx, "dy": dy, "dweight": dw}
+        out = {"r": r, "z": z, "dx": dx, "dy": dy if dy.numel() else dx, "dweight": dw}
         if s["post"] is not None:
             out.update(dpost=dpost, dscale=dscale)
         return dict(out, dgate=dgate) if s["gate"] is not None else out
