@@ -16,33 +16,13 @@
 // in 163 us, 6.4 TB/s (172 between backward passes; a kernel that only reads
 // reaches 7.0).  The backward reads and writes once: 333 us, 6.3 TB/s (a copy 5.1).
 #include "../../include/gmdn_lm.h"
-#include <float.h>
-#include "rows8.h"
+#include "logsums.h"
 
 namespace gmdn {
 namespace {
 
-constexpr float LOG2E = 1.44269504088896340736f;
-// Differences of logits are clamped here where they multiply a sum: e^-200
-// is 0 in float32, and 0 times the clamped value is 0, not NaN.
-constexpr float FAR = -200.f;
 constexpr int PIECES = 4;  // pieces a thread loads before it works on them
 
-GMDN_DEV float exp_of(float x) { return __builtin_amdgcn_exp2f(x * LOG2E); }
-
-struct Sums {
-  float m, s, w;
-};
-GMDN_DEV Sums no_sums() { return {-FLT_MAX, 0.f, 0.f}; }
-
-// Rescale to the maximum m >= a.m.  NaN stays in s; an infinite m makes its
-// own terms NaN.
-GMDN_DEV void rescale(Sums& a, float m) {
-  const float u = fmaxf(a.m - m, FAR), k = exp_of(u);
-  a.w = k * (a.w + u * a.s);
-  a.s *= k;
-  a.m = m;
-}
 // The instruction by name: for fmaxf of loaded values the compiler first
 // quiets each one, which costs as much again.  A NaN gives way to the others.
 GMDN_DEV float max3(float a, float b, float c) {
@@ -70,14 +50,6 @@ GMDN_DEV void terms8(Sums& a, const float (&x)[8]) {
   }
 }
 
-// The sums of N lanes' Sums, in each of them.
-template <int N>
-GMDN_DEV Sums join_lanes(Sums a) {
-  rescale(a, lanes_max<N>(a.m));
-  a.s = lanes_sum<N>(a.s);
-  a.w = lanes_sum<N>(a.w);
-  return a;
-}
 // The first wave's sums from the waves', in each of its lanes.
 template <int W>
 GMDN_DEV Sums join_waves(const Sums* waves) {
@@ -97,19 +69,6 @@ GMDN_DEV Sums join(Sums a, Sums* waves) {
     if (wave_id() == 0) a = join_waves<NT / 64>(waves);
   }
   return a;
-}
-
-// What a row's sums say.  No logit above -inf: s = 0, and the row's
-// distribution is empty (stats -inf, 0).
-struct Row {
-  float m, logs, entropy;
-  bool empty;
-  GMDN_DEV float logprob(float x) const { return empty ? -INFINITY : x - m - logs; }
-};
-GMDN_DEV Row row_of(const Sums& a) {
-  if (a.s == 0.f) return {-INFINITY, 0.f, 0.f, true};
-  const float logs = logf(a.s), h = logs - a.w / a.s;
-  return {a.m, logs, h < 0.f ? 0.f : h, false};
 }
 
 // The outputs of a call, and its tokens.
