@@ -1,0 +1,433 @@
+// Token embedding and its gradient (include/gmdn_lm.h).
+//
+//   y_i = s W[t_i],     dW[v] = s sum over the i with t_i = v of dy_i
+//
+// Memory bound both ways.  The forward copies rows.  The gradient is a sum by
+// token in a fixed order, without atomics on values: the positions are sorted
+// by token (a stable radix sort, so equal tokens keep their order), blocks of
+// the sorted positions add the rows of dy they name, and a token whose run
+// crosses blocks is joined from their partial sums, in order.  Rows of dW that
+// no token names are zeroed beside the sums, in the same launch.
+#include "../../include/gmdn_lm.h"
+#include "rows8.h"
+
+namespace gmdn {
+namespace {
+
+// ------------------------------------------------------------------ forward
+constexpr int EM_THREADS = 256;
+
+// A thread for each piece of eight values of y.
+template <typename T>
+__global__ void __launch_bounds__(EM_THREADS)
+em_gather(const T* __restrict__ w, const int64_t* __restrict__ tokens, T* __restrict__ y, int64_t pieces, int per_row,
+          int d, int64_t vocab, int64_t ws, float scale) {
+  const int64_t i = (int64_t)blockIdx.x * EM_THREADS + threadIdx.x;
+  if (i >= pieces) return;
+  const int64_t row = i / per_row;
+  const int c = 8 * (int)(i - row * per_row);
+  const int64_t token = tokens[row];
+  float v[8];
+  if (token >= 0 && token < vocab) {
+    load8(w + token * ws + c, d - c, v);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] *= scale;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = __builtin_nanf("");
+  }
+  store8(y + row * d + c, d - c, v);
+}
+
+// ---------------------------------------------------- positions by token
+// Least significant digit first, up to 9 bits a pass.  A workgroup moves one
+// tile of consecutive positions; where they go follows from how often each
+// digit comes in all tiles and in the earlier ones.  Tokens outside the vocabulary
+// and the padding token get the key `vocab`, behind all others.
+constexpr int SORT_THREADS = 1024;
+constexpr int SORT_WAVES = SORT_THREADS / 64;
+constexpr int SORT_BITS = 9;
+constexpr int SORT_BINS = 1 << SORT_BITS;
+constexpr int SORT_TILES = 256;          // at most; a tile is a multiple of SORT_THREADS
+constexpr int64_t SORT_SELF = 32768;     // up to here each workgroup counts all digits itself
+
+struct SortInput {
+  const int64_t* tokens;  // the first pass's, else null
+  const uint32_t *keys, *at;
+  int64_t n, vocab, padding;
+  GMDN_DEV uint32_t key(int64_t i) const {
+    if (!tokens) return keys[i];
+    const int64_t t = tokens[i];
+    return (uint32_t)(t >= 0 && t < vocab && t != padding ? t : vocab);
+  }
+  GMDN_DEV uint32_t position(int64_t i) const { return tokens ? (uint32_t)i : at[i]; }
+};
+
+// The lanes of the wave that hold the same digit (none for a lane that is not live).
+GMDN_DEV uint64_t same_digit(uint32_t digit, bool live, int bits) {
+  uint64_t m = __ballot(live);
+  for (int b = 0; b < bits; ++b) {
+    const bool set = (digit >> b) & 1;
+    const uint64_t with = __ballot(set);
+    m &= set ? with : ~with;
+  }
+  return live ? m : 0;
+}
+
+// counts[digit * tiles + tile]
+__global__ void __launch_bounds__(SORT_THREADS)
+em_count(SortInput in, uint32_t* __restrict__ counts, int64_t tile, int shift, int bits) {
+  __shared__ uint32_t bins[SORT_BINS];
+  const int t = threadIdx.x;
+  if (t < SORT_BINS) bins[t] = 0;
+  __syncthreads();
+  const int64_t first = blockIdx.x * tile;
+  for (int64_t i0 = first; i0 < first + tile && i0 < in.n; i0 += SORT_THREADS) {
+    const int64_t i = i0 + t;
+    const bool live = i < in.n;
+    const uint32_t digit = live ? (in.key(i) >> shift) & ((1u << bits) - 1) : 0;
+    const uint64_t peers = same_digit(digit, live, bits);
+    if (live && (peers & ((1ull << lane_id()) - 1)) == 0) atomicAdd(&bins[digit], (uint32_t)__popcll(peers));
+  }
+  __syncthreads();
+  if (t < SORT_BINS) counts[(int64_t)t * gridDim.x + blockIdx.x] = bins[t];
+}
+
+__global__ void __launch_bounds__(SORT_THREADS)
+em_scatter(SortInput in, const uint32_t* __restrict__ counts, uint32_t* __restrict__ keys, uint32_t* __restrict__ at,
+           int64_t tile, int shift, int bits) {
+  __shared__ uint32_t total[SORT_BINS], below[SORT_BINS];
+  __shared__ uint32_t waves[SORT_WAVES][SORT_BINS];
+  __shared__ uint32_t sums[SORT_BINS / 64];
+  const int t = threadIdx.x, w = wave_id();
+  const uint64_t before = (1ull << lane_id()) - 1;
+  const int64_t first = blockIdx.x * tile;
+  auto digit_of = [&](uint32_t key) { return (key >> shift) & ((1u << bits) - 1); };
+  if (t < SORT_BINS) total[t] = below[t] = 0;
+  __syncthreads();
+  if (counts) {
+    if (t < SORT_BINS) {
+      uint32_t all = 0, less = 0;
+      for (unsigned i = 0; i < gridDim.x; ++i) {
+        const uint32_t c = counts[(int64_t)t * gridDim.x + i];
+        all += c;
+        less += i < blockIdx.x ? c : 0;
+      }
+      total[t] = all;
+      below[t] = less;
+    }
+  } else {
+    for (int64_t i0 = 0; i0 < in.n; i0 += SORT_THREADS) {
+      const int64_t i = i0 + t;
+      const bool live = i < in.n;
+      const uint32_t digit = live ? digit_of(in.key(i)) : 0;
+      const uint64_t peers = same_digit(digit, live, bits);
+      if (live && (peers & before) == 0) {
+        atomicAdd(&total[digit], (uint32_t)__popcll(peers));
+        if (i0 < first) atomicAdd(&below[digit], (uint32_t)__popcll(peers));
+      }
+    }
+  }
+  __syncthreads();
+  // where each digit of this tile starts: the smaller digits, and its own in earlier tiles
+  uint32_t mine = 0, run = 0;
+  if (t < SORT_BINS) {
+    mine = run = total[t];
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const uint32_t u = (uint32_t)__shfl_up((int)run, o, 64);
+      if (lane_id() >= o) run += u;
+    }
+    if (lane_id() == 63) sums[w] = run;
+  }
+  __syncthreads();
+  uint32_t base = 0;
+  if (t < SORT_BINS) {
+    for (int i = 0; i < w; ++i) base += sums[i];
+    base += run - mine + below[t];
+  }
+  for (int64_t i0 = first; i0 < first + tile && i0 < in.n; i0 += SORT_THREADS) {
+    for (int i = t; i < SORT_WAVES * SORT_BINS; i += SORT_THREADS) (&waves[0][0])[i] = 0;
+    __syncthreads();
+    const int64_t i = i0 + t;
+    const bool live = i < in.n;
+    const uint32_t key = live ? in.key(i) : 0, digit = digit_of(key);
+    const uint64_t peers = same_digit(digit, live, bits);
+    const uint32_t rank = (uint32_t)__popcll(peers & before);
+    if (live && rank == 0) waves[w][digit] = (uint32_t)__popcll(peers);
+    __syncthreads();
+    if (t < SORT_BINS) {
+#pragma unroll
+      for (int i = 0; i < SORT_WAVES; ++i) {
+        const uint32_t c = waves[i][t];
+        waves[i][t] = base;
+        base += c;
+      }
+    }
+    __syncthreads();
+    if (live) {
+      const uint32_t to = waves[w][digit] + rank;
+      keys[to] = key;
+      at[to] = in.position(i);
+    }
+    __syncthreads();
+  }
+}
+
+// ------------------------------------------------------------------ sums
+// Blocks of `block` sorted positions, TPR threads of 8 columns each; wider rows
+// are shared by workgroups along the grid's y.  A run of equal tokens inside one
+// block is a whole row of dW.  One that goes on into the next block leaves its
+// sum in part (blocks, 2, d): slot 0 where it came from the block before, slot 1
+// where it begins here.
+struct Sorted {
+  const uint32_t *keys, *at;
+  int64_t n, vocab;
+  // first position whose key is not below k
+  GMDN_DEV int64_t lower(uint32_t k) const {
+    int64_t lo = 0, hi = n;
+    while (lo < hi) {
+      const int64_t mid = (lo + hi) >> 1;
+      if (keys[mid] < k)
+        lo = mid + 1;
+      else
+        hi = mid;
+    }
+    return lo;
+  }
+};
+
+constexpr int SUM_AHEAD = 8;   // rows of dy in flight
+constexpr int ZERO_ROWS = 64;  // rows of dW that a zeroing workgroup looks after
+
+template <typename T, int TPR>
+__global__ void __launch_bounds__(EM_THREADS)
+em_sums(Sorted s, const T* __restrict__ dy, T* __restrict__ dw, float* __restrict__ part, int64_t block,
+        unsigned sum_groups, int d, int64_t ds, float scale) {
+  constexpr int GROUPS = EM_THREADS / TPR;
+  const int g = threadIdx.x / TPR, t = threadIdx.x % TPR;
+  if (blockIdx.x >= sum_groups) {
+    __shared__ int absent[ZERO_ROWS];
+    const int64_t v0 = (int64_t)(blockIdx.x - sum_groups) * ZERO_ROWS;
+    if (threadIdx.x < ZERO_ROWS) {
+      const int64_t v = v0 + threadIdx.x;
+      const int64_t p = v < s.vocab ? s.lower((uint32_t)v) : s.n;
+      absent[threadIdx.x] = v < s.vocab && (p == s.n || s.keys[p] != (uint32_t)v);
+    }
+    __syncthreads();
+    const float zero[8] = {};
+    const int c = 8 * (blockIdx.y * TPR + t);
+    if (c < d)
+      for (int r = g; r < ZERO_ROWS; r += GROUPS)
+        if (absent[r]) store8(dw + (v0 + r) * d + c, d - c, zero);
+    return;
+  }
+  const int64_t b = (int64_t)blockIdx.x * GROUPS + g;
+  const int64_t p0 = b * block, p1 = p0 + block < s.n ? p0 + block : s.n;
+  const int c = 8 * (blockIdx.y * TPR + t);
+  if (p0 >= s.n || c >= d) return;
+  uint32_t cur = s.keys[p0];
+  bool from_before = p0 > 0 && s.keys[p0 - 1] == cur;
+  float sum[8] = {};
+  auto flush = [&](bool goes_on) {
+    if (cur >= s.vocab) return;
+    if (from_before || goes_on) {
+      store8(part + (2 * b + (from_before ? 0 : 1)) * d + c, d - c, sum);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) sum[j] *= scale;
+      store8(dw + (int64_t)cur * d + c, d - c, sum);
+    }
+  };
+  for (int64_t p = p0; p < p1; p += SUM_AHEAD) {
+    uint32_t key[SUM_AHEAD];
+    Raw8<T> raw[SUM_AHEAD];
+#pragma unroll
+    for (int i = 0; i < SUM_AHEAD; ++i) {
+      const int64_t q = p + i < p1 ? p + i : p1 - 1;
+      key[i] = s.keys[q];
+      raw[i].load(dy + (int64_t)s.at[q] * ds + c, d - c);
+    }
+#pragma unroll
+    for (int i = 0; i < SUM_AHEAD; ++i) {
+      if (p + i >= p1) break;
+      if (key[i] != cur) {
+        flush(false);
+        cur = key[i];
+        from_before = false;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum[j] = 0.f;
+      }
+      float v[8];
+      raw[i].get(v);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) sum[j] += v[j];
+    }
+  }
+  flush(p1 < s.n && s.keys[p1] == cur);
+}
+
+// The runs that cross blocks: the block where one begins adds its parts.
+template <typename T, int TPR>
+__global__ void __launch_bounds__(EM_THREADS)
+em_join(Sorted s, const float* __restrict__ part, T* __restrict__ dw, int64_t block, int d, float scale) {
+  constexpr int GROUPS = EM_THREADS / TPR;
+  const int64_t b = (int64_t)blockIdx.x * GROUPS + threadIdx.x / TPR;
+  const int64_t p0 = b * block, p1 = p0 + block;
+  const int c = 8 * (blockIdx.y * TPR + threadIdx.x % TPR);
+  if (p1 >= s.n || c >= d) return;
+  const uint32_t k = s.keys[p1];
+  if (k >= s.vocab || s.keys[p1 - 1] != k || (p0 > 0 && s.keys[p0] == k && s.keys[p0 - 1] == k)) return;
+  const int64_t last = (s.lower(k + 1) - 1) / block;
+  float sum[8];
+  load8(part + (2 * b + 1) * d + c, d - c, sum);
+  for (int64_t i = b + 1; i <= last; i += SUM_AHEAD) {
+    Raw8<float> raw[SUM_AHEAD];
+#pragma unroll
+    for (int j = 0; j < SUM_AHEAD; ++j) raw[j].load(part + 2 * (i + j <= last ? i + j : last) * d + c, d - c);
+#pragma unroll
+    for (int j = 0; j < SUM_AHEAD; ++j) {
+      if (i + j > last) break;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum[e] += raw[j].v[e];
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) sum[j] *= scale;
+  store8(dw + (int64_t)k * d + c, d - c, sum);
+}
+
+template <int N>
+struct Threads {
+  static constexpr int TPR = N;
+};
+template <class F>
+void with_threads(int64_t d, F&& f) {
+  if (d <= 64) f(Threads<8>{});
+  else if (d <= 128) f(Threads<16>{});
+  else if (d <= 256) f(Threads<32>{});
+  else if (d <= 512) f(Threads<64>{});
+  else if (d <= 1024) f(Threads<128>{});
+  else f(Threads<256>{});
+}
+template <class F>
+void with_type(int32_t dtype, F&& f) {
+  if (dtype == GMDN_DTYPE_BF16) f(bf16{});
+  else f(float{});
+}
+
+// How a gradient's work is cut.  A block adds its positions one after another
+// and a token's run of them is joined one after another, so the block grows with the
+// square root of the positions.
+struct Plan {
+  int64_t tile, tiles, block, blocks;
+  int passes, bits;
+  bool self;
+  size_t keys, counts, part;  // bytes
+  size_t bytes() const { return 4 * keys + counts + part; }
+};
+size_t up(size_t n) { return (n + 255) / 256 * 256; }
+Plan plan_of(int64_t n, int64_t vocab, int64_t d) {
+  Plan p{};
+  const int64_t per = (n + SORT_TILES * (int64_t)SORT_THREADS - 1) / (SORT_TILES * (int64_t)SORT_THREADS);
+  p.tile = (per > 0 ? per : 1) * SORT_THREADS;
+  p.tiles = (n + p.tile - 1) / p.tile;
+  int width = 1;
+  while ((vocab >> width) != 0) ++width;
+  p.passes = (width + SORT_BITS - 1) / SORT_BITS;
+  p.bits = (width + p.passes - 1) / p.passes;
+  p.self = n <= SORT_SELF;
+  p.block = 32;
+  while (p.block * p.block * 8 < n) p.block *= 2;
+  p.blocks = (n + p.block - 1) / p.block;
+  p.keys = up((size_t)n * 4);
+  p.counts = p.self ? 0 : up((size_t)p.tiles * SORT_BINS * 4);
+  p.part = up((size_t)p.blocks * 2 * d * 4);
+  return p;
+}
+
+int check_sizes(int64_t rows, int64_t vocab, int64_t d) {
+  if (rows < 0 || vocab <= 0 || d <= 0 || rows > INT32_MAX) return GMDN_ERR_ARG;
+  return vocab > (1 << 27) || d > (1 << 20) ? GMDN_ERR_UNSUPPORTED : GMDN_OK;
+}
+
+}  // namespace
+}  // namespace gmdn
+
+using namespace gmdn;
+
+extern "C" {
+
+int gmdn_embed_fwd(const void* weight, const int64_t* tokens, void* y, int64_t rows, int64_t vocab, int64_t d,
+                   int64_t w_stride, float scale, int32_t dtype, void* stream) {
+  const int rc = check_sizes(rows, vocab, d);
+  if (rc != GMDN_OK) return rc;
+  if (!type_ok(dtype)) return GMDN_ERR_UNSUPPORTED;
+  if (w_stride < 0) return GMDN_ERR_ARG;
+  if (rows == 0) return GMDN_OK;
+  if (!weight || !tokens || !y) return GMDN_ERR_ARG;
+  const int64_t per_row = (d + 7) / 8, pieces = rows * per_row, groups = (pieces + EM_THREADS - 1) / EM_THREADS;
+  if (pieces >= (int64_t)1 << 32) return GMDN_ERR_UNSUPPORTED;
+  with_type(dtype, [&](auto t) {
+    using T = decltype(t);
+    hipLaunchKernelGGL((em_gather<T>), dim3((unsigned)groups), dim3(EM_THREADS), 0, (hipStream_t)stream,
+                       (const T*)weight, tokens, (T*)y, pieces, (int)per_row, (int)d, vocab, w_stride, scale);
+  });
+  return launched();
+}
+
+size_t gmdn_embed_bwd_workspace_bytes(int64_t rows, int64_t vocab, int64_t d) {
+  if (rows <= 0 || check_sizes(rows, vocab, d) != GMDN_OK) return 0;
+  return plan_of(rows, vocab, d).bytes();
+}
+
+int gmdn_embed_bwd(const void* dy, const int64_t* tokens, void* dweight, void* workspace, size_t workspace_bytes,
+                   int64_t rows, int64_t vocab, int64_t d, int64_t dy_stride, float scale, int64_t padding_idx,
+                   int32_t dtype, void* stream) {
+  const int rc = check_sizes(rows, vocab, d);
+  if (rc != GMDN_OK) return rc;
+  if (!type_ok(dtype)) return GMDN_ERR_UNSUPPORTED;
+  if (dy_stride < 0 || !dweight || (rows > 0 && (!dy || !tokens))) return GMDN_ERR_ARG;
+  const Plan p = plan_of(rows, vocab, d);
+  if (rows > 0 && (!workspace || workspace_bytes < p.bytes())) return GMDN_ERR_WORKSPACE;
+  const hipStream_t st = (hipStream_t)stream;
+  char* at = (char*)workspace;
+  uint32_t* buf[4];
+  for (auto& b : buf) {
+    b = (uint32_t*)at;
+    at += p.keys;
+  }
+  uint32_t* const counts = p.self ? nullptr : (uint32_t*)at;
+  float* const part = (float*)(at + p.counts);
+  SortInput in{tokens, nullptr, nullptr, rows, vocab, padding_idx};
+  int to = 0;
+  for (int pass = 0; pass < p.passes && rows > 0; ++pass, to ^= 1) {
+    const int shift = pass * p.bits;
+    if (counts)
+      hipLaunchKernelGGL(em_count, dim3((unsigned)p.tiles), dim3(SORT_THREADS), 0, st, in, counts, p.tile, shift, p.bits);
+    hipLaunchKernelGGL(em_scatter, dim3((unsigned)p.tiles), dim3(SORT_THREADS), 0, st, in, counts, buf[2 * to],
+                       buf[2 * to + 1], p.tile, shift, p.bits);
+    in.tokens = nullptr;
+    in.keys = buf[2 * to];
+    in.at = buf[2 * to + 1];
+  }
+  const Sorted sorted{in.keys, in.at, rows, vocab};
+  with_type(dtype, [&](auto t) {
+    using T = decltype(t);
+    with_threads(d, [&](auto n) {
+      constexpr int TPR = decltype(n)::TPR;
+      constexpr int GROUPS = EM_THREADS / TPR;
+      const unsigned slices = (unsigned)((d + 8 * TPR - 1) / (8 * TPR));
+      const unsigned sums = (unsigned)((p.blocks + GROUPS - 1) / GROUPS);
+      const unsigned zeros = (unsigned)((vocab + ZERO_ROWS - 1) / ZERO_ROWS);
+      hipLaunchKernelGGL((em_sums<T, TPR>), dim3(sums + zeros, slices), dim3(EM_THREADS), 0, st, sorted, (const T*)dy,
+                         (T*)dweight, part, p.block, sums, (int)d, dy_stride, scale);
+      if (p.blocks > 1)
+        hipLaunchKernelGGL((em_join<T, TPR>), dim3(sums, slices), dim3(EM_THREADS), 0, st, sorted, part, (T*)dweight,
+                           p.block, (int)d, scale);
+    });
+  });
+  return launched();
+}
+
+}  // extern "C"

@@ -1,0 +1,562 @@
+// Log probabilities of given tokens from hidden states and the head's weight,
+// without the logits, and the gradients of both (include/gmdn_lm.h).
+//
+// With logits l = x W^T of a row x, its token t and the cotangents gl, gh of the
+// two outputs:
+//   lp = l_t - M - log s,  H = log s - w / s      (M, s, w: logsums.h)
+//   d_v = gl ([v = t] - p_v) - gh p_v (log p_v + H),   p = softmax(l)
+//   dx = d W,    dW = d^T x     (over all rows)
+//
+// Matrix bound: 2 T V D operations a product.  The forward forms tiles of the logits
+// in registers and leaves of each row of a tile three sums; they are joined
+// by row afterwards.  The backward forms the logits again, a piece of the
+// vocabulary at a time, writes the piece's d in bfloat16 and takes both
+// products from it: four products in all, and of the logits never more than
+// PIECE_BYTES of memory.
+//
+// bfloat16 operands are multiplied as they are; d is rounded to bfloat16 as the
+// gradient of bfloat16 logits would be.  float32 operands, and d beside them, are
+// split into two bfloat16 pieces (x = hi + lo up to 2^-17 |x|) and multiplied as lo hi +
+// hi lo + hi hi, what this library's other float32 products do.
+#include "../../include/gmdn_lm.h"
+#include <type_traits>
+#include "bf16mm.h"
+#include "logsums.h"
+
+namespace gmdn {
+namespace {
+
+constexpr int64_t PIECE_BYTES = 512 << 20;
+constexpr int64_t PIECE_MOST = 1 << 20;   // columns: 256 rows of them within 32 bits of bytes
+constexpr int UNIT = 256;                 // a piece's columns: a multiple
+constexpr int KPAD = 64;                  // k in planes: a multiple, zeros behind the values
+constexpr float HALF_LOG2E = 0.5f * LOG2E;
+
+// ------------------------------------------------------------------ planes
+// (rows, d) as P planes (rows, kp) of bfloat16 pieces, zeros behind d.
+template <typename T, int P>
+__global__ void __launch_bounds__(256)
+ll_planes(const T* __restrict__ x, int64_t stride, bf16* __restrict__ out, int64_t rows, int d, int kp) {
+  const int per = kp / 8;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t r = i / per;
+  if (r >= rows) return;
+  const int c = 8 * (int)(i - r * per);
+  float v[8];
+  load8(x + r * stride + c, d - c, v);
+  bf16* o = out + r * kp + c;
+#pragma unroll
+  for (int p = 0; p < P; ++p, o += rows * kp) {
+    bf16x8 h;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      h[j] = (bf16)v[j];
+      v[j] -= (float)h[j];
+    }
+    *reinterpret_cast<bf16x8*>(o) = h;
+  }
+}
+
+// ------------------------------------------------------------------ forward
+// m: vocabulary, n: rows of x.  part (tiles of m, 3, rows): each tile's sums.
+struct SumsArgs {
+  const int64_t* tokens;
+  float *at_token, *part;
+  int64_t rows;
+  int V;
+};
+GMDN_DEV void join_sums(Sums& a, Sums b) {
+  const float m = fmaxf(a.m, b.m);
+  rescale(a, m);
+  rescale(b, m);
+  a.s += b.s;
+  a.w += b.w;
+}
+template <class S, bool PERM>
+struct SumsEpi {
+  SumsArgs e;
+  GMDN_DEV void operator()(f32x4 (&acc)[S::MT][S::NT], const MMTile& tile, int64_t m0, int64_t n0, int wm, int wn,
+                           char* smem) const {
+    const int l = lane_id(), G = l >> 4;
+    Sums* const waves = reinterpret_cast<Sums*>(smem);  // (WM, TN)
+    const int left = e.V - (int)m0;
+    if (left < S::TM)  // the vocabulary ends in this tile
+#pragma unroll
+      for (int i = 0; i < S::MT; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          if (m_of<PERM>(wm * S::MT + i, G) + q >= left)
+#pragma unroll
+            for (int j = 0; j < S::NT; ++j) acc[i][j][q] = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < S::NT; ++j) {
+      const int n = 16 * (wn * S::NT + j) + (l & 15);
+      const int64_t row = n0 + n, token = row < e.rows ? e.tokens[row] : -1;
+      if (token >= m0 && token < m0 + S::TM && token < e.V)
+#pragma unroll
+        for (int i = 0; i < S::MT; ++i)
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            if (m_of<PERM>(wm * S::MT + i, G) + q == (int)(token - m0)) e.at_token[row] = acc[i][j][q];
+      Sums a = no_sums();
+#pragma unroll
+      for (int i = 0; i < S::MT; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) a.m = fmaxf(a.m, acc[i][j][q]);
+#pragma unroll
+      for (int i = 0; i < S::MT; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const float u = acc[i][j][q] - a.m, x = exp_of(u);
+          a.s += x;
+          a.w += x * fmaxf(u, FAR);
+        }
+      // the four lane groups, then the waves along m through LDS
+#pragma unroll
+      for (int o = 16; o < 64; o <<= 1) join_sums(a, {__shfl_xor(a.m, o, 64), __shfl_xor(a.s, o, 64), __shfl_xor(a.w, o, 64)});
+      if (G == 0) waves[wm * S::TN + n] = a;
+    }
+    __syncthreads();
+    for (int n = threadIdx.x; n < S::TN; n += S::THREADS) {
+      Sums a = waves[n];
+      for (int i = 1; i < S::WM; ++i) join_sums(a, waves[i * S::TN + n]);
+      const int64_t row = n0 + n;
+      if (row >= e.rows) continue;
+      float* const p = e.part + (int64_t)tile.m * 3 * e.rows + row;
+      p[0] = a.m;
+      p[e.rows] = a.s;
+      p[2 * e.rows] = a.w;
+    }
+  }
+};
+
+// A row's sums from its tiles': R rows a workgroup, 256 / R threads each.
+template <int R>
+__global__ void __launch_bounds__(256)
+ll_join(const float* __restrict__ part, const float* __restrict__ at_token, const int64_t* __restrict__ tokens,
+        float* __restrict__ lp, float* __restrict__ entropy, float* __restrict__ stats, int tiles, int64_t rows,
+        int64_t V, int64_t ignore) {
+  constexpr int PER = 256 / R;
+  __shared__ Sums all[PER][R];
+  const int r = threadIdx.x % R, part_of = threadIdx.x / R;
+  const int64_t row = (int64_t)blockIdx.x * R + r;
+  Sums a = no_sums();
+  if (row < rows)
+    for (int i = part_of; i < tiles; i += PER) {
+      const float* const p = part + (int64_t)i * 3 * rows + row;
+      join_sums(a, {p[0], p[rows], p[2 * rows]});
+    }
+  all[part_of][r] = a;
+  for (int n = PER / 2; n > 0; n /= 2) {
+    __syncthreads();
+    if (part_of < n) {
+      join_sums(a, all[part_of + n][r]);
+      all[part_of][r] = a;
+    }
+  }
+  if (part_of != 0 || row >= rows) return;
+  const Row w = row_of(a);
+  const int64_t token = tokens[row];
+  lp[row] = token == ignore ? 0.f : token >= 0 && token < V ? w.logprob(at_token[row]) : NAN;
+  entropy[row] = w.entropy;
+  stats[2 * row] = w.m;
+  stats[2 * row + 1] = w.logs;
+}
+// One row a workgroup while those are few: the tiles of a large vocabulary are read one
+// after another by each thread.
+constexpr int64_t JOIN_FEW = 1024;
+
+// ------------------------------------------------------------------ backward
+// d of a piece of the vocabulary: P planes (padded rows, columns) of bfloat16, zeros
+// behind the vocabulary, to the end of its tile of it, and behind the rows.
+struct GradArgs {
+  const int64_t* tokens;
+  const float *stats, *entropy, *dlp, *dent;
+  bf16* d;
+  int64_t rows, padded, columns, left, first, V, ignore;  // left: the piece's columns inside the vocabulary
+};
+template <class S, bool PERM, int P>
+struct GradEpi {
+  GradArgs e;
+  GMDN_DEV void operator()(f32x4 (&acc)[S::MT][S::NT], const MMTile&, int64_t m0, int64_t n0, int wm, int wn,
+                           char*) const {
+    static_assert(PERM && S::MT % 2 == 0, "two tiles hold eight consecutive columns");
+    const int l = lane_id(), G = l >> 4;
+    const int left = (int)(e.left - m0);  // the tile's columns inside the vocabulary
+#pragma unroll
+    for (int j = 0; j < S::NT; ++j) {
+      const int64_t row = n0 + 16 * (wn * S::NT + j) + (l & 15);
+      if (row >= e.padded) continue;
+      float m = 0.f, logs = 0.f, h = 0.f, gl = 0.f, gh = 0.f;
+      int token = -1;  // from the tile's first column
+      if (row < e.rows) {
+        const int64_t t = e.tokens[row];
+        gl = e.dlp && t != e.ignore ? e.dlp[row] : 0.f;
+        gh = e.dent ? e.dent[row] : 0.f;
+        if (t != e.ignore && (t < 0 || t >= e.V)) gl = NAN;
+        m = e.stats[2 * row];
+        logs = e.stats[2 * row + 1];
+        h = e.entropy[row];
+        const int64_t from = t - e.first - m0;
+        token = from >= 0 && from < S::TM ? (int)from : -1;
+      }
+      const bool none = (gl == 0.f && gh == 0.f) || m == -INFINITY;
+      bf16* const to = e.d + row * e.columns + m0;
+#pragma unroll
+      for (int i = 0; i < S::MT; i += 2) {
+        const int c = m_of<PERM>(wm * S::MT + i, G);
+        float g[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          // p as the square of e^(log p / 2): the exponential flushes results below 2^-126
+          const float u = acc[i + q / 4][j][q % 4] - m - logs, x = __builtin_amdgcn_exp2f(u * HALF_LOG2E);
+          const float f = e.dent ? gl + gh * (fmaxf(u, FAR) + h) : gl;
+          g[q] = none ? 0.f : -x * (x * f);
+        }
+        if (token >= 0 && !none)
+#pragma unroll
+          for (int q = 0; q < 8; ++q)
+            if (c + q == token) g[q] += gl;
+        if (left < S::TM)  // the vocabulary ends in this tile
+#pragma unroll
+          for (int q = 0; q < 8; ++q)
+            if (c + q >= left) g[q] = 0.f;
+        bf16* o = to + c;
+#pragma unroll
+        for (int p = 0; p < P; ++p, o += e.padded * e.columns) {
+          const bf16x8 b = cat8(to_bf16x4(f32x4{g[0], g[1], g[2], g[3]}), to_bf16x4(f32x4{g[4], g[5], g[6], g[7]}));
+          *reinterpret_cast<bf16x8*>(o) = b;
+#pragma unroll
+          for (int q = 0; q < 8; ++q) g[q] -= (float)b[q];
+        }
+      }
+    }
+  }
+};
+
+// C (n, m): to `out` in its type, or to float32 planes (splits, n, m); `add`: on
+// what the plane holds.
+template <typename T>
+struct StoreArgs {
+  float* plane;
+  T* out;
+  int64_t M, N;
+  bool add;
+};
+template <class S, typename T>
+struct StoreEpi {
+  StoreArgs<T> e;
+  GMDN_DEV void operator()(f32x4 (&acc)[S::MT][S::NT], const MMTile&, int64_t m0, int64_t n0, int wm, int wn,
+                           char*) const {
+    const int l = lane_id(), G = l >> 4;
+    float* const plane = e.plane ? e.plane + (int64_t)blockIdx.y * e.M * e.N : nullptr;
+#pragma unroll
+    for (int j = 0; j < S::NT; ++j) {
+      const int64_t n = n0 + 16 * (wn * S::NT + j) + (l & 15);
+      if (n >= e.N) continue;
+#pragma unroll
+      for (int i = 0; i < S::MT; ++i) {
+        const int64_t m = m0 + m_of<false>(wm * S::MT + i, G);
+        if (m >= e.M) continue;
+        f32x4 v = acc[i][j];
+        const int64_t at = n * e.M + m;
+        const bool whole = m + 4 <= e.M;
+        if (e.add) {
+          if (whole) {
+            v += *reinterpret_cast<const f32x4_any*>(plane + at);
+          } else {
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              if (m + q < e.M) v[q] += plane[at + q];
+          }
+        }
+        if (e.out)
+          put(e.out + at, v, whole, e.M - m);
+        else
+          put(plane + at, v, whole, e.M - m);
+      }
+    }
+  }
+  static GMDN_DEV void put(float* o, const f32x4& v, bool whole, int64_t left) {
+    if (whole) {
+      *reinterpret_cast<f32x4_any*>(o) = v;
+    } else {
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        if (q < left) o[q] = v[q];
+    }
+  }
+  static GMDN_DEV void put(bf16* o, const f32x4& v, bool whole, int64_t left) {
+    typedef bf16 bf16x4_any __attribute__((ext_vector_type(4), aligned(2)));
+    const bf16x4 b = to_bf16x4(v);
+    if (whole) {
+      *reinterpret_cast<bf16x4_any*>(o) = b;
+    } else {
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        if (q < left) o[q] = b[q];
+    }
+  }
+};
+
+// out = the sum of the planes, in their order.
+template <typename T>
+__global__ void __launch_bounds__(256)
+ll_sum_planes(const float* __restrict__ planes, T* __restrict__ out, int64_t n, int count) {
+  const int64_t at = 8 * ((int64_t)blockIdx.x * 256 + threadIdx.x);
+  if (at >= n) return;
+  const int left = n - at < 8 ? (int)(n - at) : 8;
+  float s[8] = {};
+  for (int p = 0; p < count; ++p) {
+    float v[8];
+    load8(planes + p * n + at, left, v);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s[j] += v[j];
+  }
+  store8(out + at, left, s);
+}
+
+// ------------------------------------------------------------------ the calls
+using Big = MMShape<256, 256, 64, 2, 2, 4>;
+using Small = MMShape<64, 64, 64, 3, 2, 2>;
+
+int64_t div_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
+int64_t round_up(int64_t a, int64_t b) { return div_up(a, b) * b; }
+size_t up(size_t n) { return (n + 255) / 256 * 256; }
+
+// Whether the products read a matrix where it is: bfloat16 rows of whole stages at
+// 16-byte addresses, 256 of which stay within 32 bits.
+bool in_place(const void* p, int64_t stride, int64_t d, int32_t dtype) {
+  return dtype == GMDN_DTYPE_BF16 && d % KPAD == 0 && stride % 8 == 0 && stride <= (1 << 22) && (uintptr_t)p % 16 == 0;
+}
+
+struct Sizes {
+  int64_t rows, V, d, kp;
+  int P;
+  bool x_in, w_in, big;
+  size_t x, w;                     // bytes of the operands' planes
+  // forward
+  int64_t tiles;                   // of the vocabulary
+  size_t at_token, part;
+  // backward
+  int64_t piece, pieces, padded;   // columns, pieces, rows of d
+  int x_per, x_splits, w_per, w_splits;  // stages of a split, splits
+  size_t grad, x_acc, w_acc;
+  size_t forward() const { return x + w + at_token + part; }
+  size_t backward() const { return x + w + grad + x_acc + w_acc; }
+};
+
+// A product of few tiles is split along k until the chip is filled, while a part
+// keeps four stages or more.
+int splits_of(int64_t tiles, int64_t steps) {
+  int64_t s = 256 / tiles;
+  if (s > steps / 4) s = steps / 4;
+  return (int)(s < 1 ? 1 : s > 64 ? 64 : s);
+}
+
+Sizes sizes_of(const void* x, const void* w, int64_t rows, int64_t V, int64_t d, int64_t xs, int64_t ws, int32_t dtype) {
+  Sizes z{};
+  z.rows = rows;
+  z.V = V;
+  z.d = d;
+  z.kp = round_up(d, KPAD);
+  z.P = dtype == GMDN_DTYPE_F32 ? 2 : 1;
+  z.x_in = in_place(x, xs, d, dtype);
+  z.w_in = in_place(w, ws, d, dtype);
+  z.x = z.x_in ? 0 : up((size_t)(z.P * rows * z.kp * 2));
+  z.w = z.w_in ? 0 : up((size_t)(z.P * V * z.kp * 2));
+  z.big = div_up(V, 256) * div_up(rows, 256) >= 256;
+  const int64_t tile = z.big ? 256 : 64;
+  z.tiles = div_up(V, tile);
+  z.at_token = up((size_t)rows * 4);
+  z.part = up((size_t)(z.tiles * 3 * rows * 4));
+  z.padded = round_up(rows, 64);
+  int64_t most = PIECE_BYTES / (z.padded * 2 * z.P) / UNIT * UNIT;
+  most = most < UNIT ? UNIT : most > PIECE_MOST ? PIECE_MOST : most;
+  z.pieces = div_up(V, most);
+  z.piece = round_up(div_up(V, z.pieces), UNIT);
+  z.pieces = div_up(V, z.piece);
+  z.grad = up((size_t)(z.P * z.padded * z.piece * 2));
+  const int64_t most_v = z.piece < V ? z.piece : V, x_steps = div_up(most_v, 64), w_steps = z.padded / 64;
+  z.x_per = (int)div_up(x_steps, splits_of(div_up(d, tile) * div_up(rows, tile), x_steps));
+  z.w_per = (int)div_up(w_steps, splits_of(div_up(d, tile) * div_up(most_v, tile), w_steps));
+  z.x_splits = (int)div_up(x_steps, z.x_per);
+  z.w_splits = (int)div_up(w_steps, z.w_per);
+  z.x_acc = z.x_splits > 1 || z.pieces > 1 ? up((size_t)(z.x_splits * rows * d * 4)) : 0;
+  z.w_acc = z.w_splits > 1 ? up((size_t)(z.w_splits * most_v * d * 4)) : 0;
+  return z;
+}
+
+int check_ll(int64_t rows, int64_t V, int64_t d, int64_t xs, int64_t ws, int32_t dtype) {
+  if (rows < 0 || V <= 0 || d <= 0 || xs < 0 || ws < 0 || rows > ((int64_t)1 << 30)) return GMDN_ERR_ARG;
+  return !type_ok(dtype) || V > (1 << 27) || d > (1 << 17) ? GMDN_ERR_UNSUPPORTED : GMDN_OK;
+}
+
+// An operand's planes: where it lies, or made at `at`, which moves on.
+template <typename T>
+const bf16* planes_of(const T* x, int64_t stride, int64_t rows, const Sizes& z, bool in, size_t bytes, char*& at,
+                      hipStream_t st) {
+  if (in) return (const bf16*)x;
+  bf16* const out = (bf16*)at;
+  at += bytes;
+  hipLaunchKernelGGL((ll_planes<T, std::is_same_v<T, float> ? 2 : 1>), dim3((unsigned)div_up(rows * (z.kp / 8), 256)),
+                     dim3(256), 0, st, x, stride, out, rows, (int)z.d, (int)z.kp);
+  return out;
+}
+
+// The pairs of planes of a product, the small terms first: lo hi, hi lo, hi hi.
+void set_pairs(MMArgs& a, int P) {
+  a.pairs = P == 1 ? 1 : 3;
+  a.pair_a = P == 1 ? 0 : 0x001;
+  a.pair_b = P == 1 ? 0 : 0x010;
+}
+
+template <class S>
+MMArgs args_of(const MMOperand& a, const MMOperand& b, int64_t M, int64_t N, int64_t k, int P, int per) {
+  static_assert(S::BK == KPAD, "a stage is what the operands are padded to");
+  MMArgs r{};
+  r.a = a;
+  r.b = b;
+  r.steps = (int)div_up(k, S::BK);
+  r.per = per ? per : r.steps;
+  r.tiles_m = (int)div_up(M, S::TM);
+  r.tiles_n = (int)div_up(N, S::TN);
+  set_pairs(r, P);
+  return r;
+}
+
+struct Matrices {
+  const bf16 *x, *w;
+  int64_t xs, ws, xp, wp;  // row strides, plane strides
+};
+template <typename T>
+Matrices matrices_of(const void* x, const void* w, int64_t xs, int64_t ws, const Sizes& z, char*& at, hipStream_t st) {
+  Matrices m;
+  m.x = planes_of((const T*)x, xs, z.rows, z, z.x_in, z.x, at, st);
+  m.w = planes_of((const T*)w, ws, z.V, z, z.w_in, z.w, at, st);
+  m.xs = z.x_in ? xs : z.kp;
+  m.ws = z.w_in ? ws : z.kp;
+  m.xp = z.rows * z.kp;
+  m.wp = z.V * z.kp;
+  return m;
+}
+
+// Logits of `columns` of the vocabulary from v0 on.
+template <class S, class Epi>
+bool logits(const Matrices& m, const Sizes& z, int64_t v0, int64_t columns, const Epi& epi, hipStream_t st) {
+  const MMArgs a = args_of<S>({m.w + v0 * m.ws, m.ws, m.wp, columns - 1, 0}, {m.x, m.xs, m.xp, z.rows - 1, 0}, columns,
+                              z.rows, z.kp, z.P, 0);
+  return mm_launch<S, false, false, true>(a, epi, 1, st);
+}
+
+template <class S>
+bool forward(const Matrices& m, const Sizes& z, const SumsArgs& e, hipStream_t st) {
+  return logits<S>(m, z, 0, z.V, SumsEpi<S, true>{e}, st);
+}
+
+template <typename T>
+void sum_planes(const float* planes, T* out, int64_t n, int count, hipStream_t st) {
+  hipLaunchKernelGGL((ll_sum_planes<T>), dim3((unsigned)div_up(n, 8 * 256)), dim3(256), 0, st, planes, out, n, count);
+}
+
+template <class S, typename T>
+bool backward(const Matrices& m, const Sizes& z, GradArgs e, float* x_acc, float* w_acc, T* dx, T* dw, hipStream_t st) {
+  constexpr int P = std::is_same_v<T, float> ? 2 : 1;
+  const int64_t plane = z.padded * z.piece;
+  for (int64_t i = 0; i < z.pieces; ++i) {
+    const int64_t v0 = i * z.piece, left = z.V - v0 < z.piece ? z.V - v0 : z.piece;
+    e.first = v0;
+    e.left = left;
+    if (!logits<S>(m, z, v0, left, GradEpi<S, true, P>{e}, st)) return false;
+    if (dx) {
+      const bool last = i + 1 == z.pieces;
+      const MMArgs a = args_of<S>({m.w + v0 * m.ws, m.ws, m.wp, z.kp - 1, left - 1}, {e.d, z.piece, plane, z.rows - 1, 0},
+                                  z.d, z.rows, left, P, z.x_per);
+      const int splits = (int)div_up(a.steps, a.per);
+      const StoreArgs<T> s{x_acc, last && z.x_splits == 1 ? dx : nullptr, z.d, z.rows, i > 0};
+      if (!mm_launch<S, true, false, false>(a, StoreEpi<S, T>{s}, splits, st)) return false;
+      if (last && z.x_splits > 1) sum_planes(x_acc, dx, z.rows * z.d, z.x_splits, st);
+    }
+    if (dw) {
+      const MMArgs a = args_of<S>({m.x, m.xs, m.xp, z.kp - 1, z.rows - 1}, {e.d, z.piece, plane, z.piece - 1, z.padded - 1},
+                                  z.d, left, z.padded, P, z.w_per);
+      const StoreArgs<T> s{w_acc, z.w_splits == 1 ? dw + v0 * z.d : nullptr, z.d, left, false};
+      if (!mm_launch<S, true, true, false>(a, StoreEpi<S, T>{s}, z.w_splits, st)) return false;
+      if (z.w_splits > 1) sum_planes(w_acc, dw + v0 * z.d, left * z.d, z.w_splits, st);
+    }
+  }
+  return true;
+}
+
+}  // namespace
+}  // namespace gmdn
+
+using namespace gmdn;
+
+extern "C" {
+
+size_t gmdn_linear_logprobs_fwd_workspace_bytes(const void* x, const void* weight, int64_t rows, int64_t vocab,
+                                                int64_t d, int64_t x_stride, int64_t w_stride, int32_t dtype) {
+  if (rows == 0 || check_ll(rows, vocab, d, x_stride, w_stride, dtype) != GMDN_OK) return 0;
+  return sizes_of(x, weight, rows, vocab, d, x_stride, w_stride, dtype).forward();
+}
+
+int gmdn_linear_logprobs_fwd(const void* x, const void* weight, const int64_t* tokens, float* logprob, float* entropy,
+                             float* stats, void* workspace, size_t workspace_bytes, int64_t rows, int64_t vocab,
+                             int64_t d, int64_t x_stride, int64_t w_stride, int64_t ignore_index, int32_t dtype,
+                             void* stream) {
+  const int rc = check_ll(rows, vocab, d, x_stride, w_stride, dtype);
+  if (rc != GMDN_OK || rows == 0) return rc;
+  if (!x || !weight || !tokens || !logprob || !entropy || !stats) return GMDN_ERR_ARG;
+  const Sizes z = sizes_of(x, weight, rows, vocab, d, x_stride, w_stride, dtype);
+  if (!workspace || workspace_bytes < z.forward()) return GMDN_ERR_WORKSPACE;
+  const hipStream_t st = (hipStream_t)stream;
+  char* at = (char*)workspace;
+  const Matrices m = dtype == GMDN_DTYPE_F32 ? matrices_of<float>(x, weight, x_stride, w_stride, z, at, st)
+                                             : matrices_of<bf16>(x, weight, x_stride, w_stride, z, at, st);
+  const SumsArgs e{tokens, (float*)at, (float*)(at + z.at_token), rows, (int)vocab};
+  if (!(z.big ? forward<Big>(m, z, e, st) : forward<Small>(m, z, e, st))) return GMDN_ERR_LAUNCH;
+  if (rows <= JOIN_FEW)
+    hipLaunchKernelGGL((ll_join<1>), dim3((unsigned)rows), dim3(256), 0, st, e.part, e.at_token, tokens, logprob, entropy,
+                       stats, (int)z.tiles, rows, vocab, ignore_index);
+  else
+    hipLaunchKernelGGL((ll_join<16>), dim3((unsigned)div_up(rows, 16)), dim3(256), 0, st, e.part, e.at_token, tokens,
+                       logprob, entropy, stats, (int)z.tiles, rows, vocab, ignore_index);
+  return launched();
+}
+
+size_t gmdn_linear_logprobs_bwd_workspace_bytes(const void* x, const void* weight, int64_t rows, int64_t vocab,
+                                                int64_t d, int64_t x_stride, int64_t w_stride, int32_t dtype) {
+  if (rows == 0 || check_ll(rows, vocab, d, x_stride, w_stride, dtype) != GMDN_OK) return 0;
+  return sizes_of(x, weight, rows, vocab, d, x_stride, w_stride, dtype).backward();
+}
+
+int gmdn_linear_logprobs_bwd(const void* x, const void* weight, const int64_t* tokens, const float* stats,
+                             const float* entropy, const float* dlogprob, const float* dentropy, void* dx,
+                             void* dweight, void* workspace, size_t workspace_bytes, int64_t rows, int64_t vocab,
+                             int64_t d, int64_t x_stride, int64_t w_stride, int64_t ignore_index, int32_t dtype,
+                             void* stream) {
+  const int rc = check_ll(rows, vocab, d, x_stride, w_stride, dtype);
+  if (rc != GMDN_OK || rows == 0) return rc;
+  if (!x || !weight || !tokens || !stats || !entropy || (!dx && !dweight)) return GMDN_ERR_ARG;
+  const Sizes z = sizes_of(x, weight, rows, vocab, d, x_stride, w_stride, dtype);
+  if (!workspace || workspace_bytes < z.backward()) return GMDN_ERR_WORKSPACE;
+  const hipStream_t st = (hipStream_t)stream;
+  char* at = (char*)workspace;
+  const Matrices m = dtype == GMDN_DTYPE_F32 ? matrices_of<float>(x, weight, x_stride, w_stride, z, at, st)
+                                             : matrices_of<bf16>(x, weight, x_stride, w_stride, z, at, st);
+  const GradArgs e{tokens, stats, entropy, dlogprob, dentropy, (bf16*)at, rows, z.padded, z.piece, 0, 0, vocab,
+                  ignore_index};
+  float* const xa = (float*)(at + z.grad);
+  float* const wa = (float*)(at + z.grad + z.x_acc);
+  auto run = [&](auto s, auto t) {
+    using S = decltype(s);
+    using T = decltype(t);
+    return backward<S, T>(m, z, e, xa, wa, (T*)dx, (T*)dweight, st);
+  };
+  const bool ok = dtype == GMDN_DTYPE_F32 ? (z.big ? run(Big{}, float{}) : run(Small{}, float{}))
+                                          : (z.big ? run(Big{}, bf16{}) : run(Small{}, bf16{}));
+  return ok ? launched() : GMDN_ERR_LAUNCH;
+}
+
+}  // extern "C"

@@ -90,6 +90,16 @@ SIGNATURES = {
     "gmdn_logprobs_fwd_workspace_bytes": (c_size, [c_i64, c_i64, c_i32]),
     "gmdn_logprobs_fwd": (c_i32, [c_vp] * 8 + [c_size] + [c_i64] * 3 + [c_i32, c_i64, c_i32, c_vp]),
     "gmdn_logprobs_bwd": (c_i32, [c_vp] * 9 + [c_i64] * 3 + [c_i32, c_i64, c_i32, c_vp]),
+    "gmdn_embed_fwd": (c_i32, [c_vp] * 3 + [c_i64] * 4 + [ctypes.c_float, c_i32, c_vp]),
+    "gmdn_embed_bwd_workspace_bytes": (c_size, [c_i64] * 3),
+    "gmdn_embed_bwd": (c_i32, [c_vp] * 4 + [c_size] + [c_i64] * 4 + [ctypes.c_float, c_i64, c_i32, c_vp]),
+    "gmdn_residual_norm_fwd": (c_i32, [c_vp] * 10 + [c_i64] * 5 + [ctypes.c_float] + [c_i32] * 3 + [c_vp]),
+    "gmdn_residual_norm_bwd_workspace_floats": (c_size, [c_i64] * 2),
+    "gmdn_residual_norm_bwd": (c_i32, [c_vp] * 17 + [c_size] + [c_i64] * 7 + [c_i32] * 3 + [c_vp]),
+    "gmdn_linear_logprobs_fwd_workspace_bytes": (c_size, [c_vp] * 2 + [c_i64] * 5 + [c_i32]),
+    "gmdn_linear_logprobs_fwd": (c_i32, [c_vp] * 7 + [c_size] + [c_i64] * 6 + [c_i32, c_vp]),
+    "gmdn_linear_logprobs_bwd_workspace_bytes": (c_size, [c_vp] * 2 + [c_i64] * 5 + [c_i32]),
+    "gmdn_linear_logprobs_bwd": (c_i32, [c_vp] * 10 + [c_size] + [c_i64] * 6 + [c_i32, c_vp]),
 }
 
 

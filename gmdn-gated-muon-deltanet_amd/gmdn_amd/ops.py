@@ -41,6 +41,20 @@ its model, train_ablation.py:420-422):
   top_logprobs, top_tokens, stats)`` and ``gmdn::logprobs_bwd(logits, tokens,
   stats, entropy, top_tokens, dlogprob, dentropy, dtop, ignore_index) ->
   dlogits`` -- log probabilities of given tokens (gmdn_amd.logprobs).
+* ``gmdn::embed_fwd(weight, tokens, scale, padding_idx) -> y`` and
+  ``gmdn::embed_bwd(dy, tokens, vocab, scale, padding_idx) -> dweight`` -- token
+  embedding (gmdn_amd.embedding).
+* ``gmdn::residual_norm_fwd(x, y, weight, post_weight, gate, scale, eps) -> (r,
+  z, rstd, post_rstd)`` and ``gmdn::residual_norm_bwd(dr, dz, r, y, weight,
+  post_weight, gate, scale, rstd, post_rstd) -> (dx, dy, dweight, dpost_weight,
+  dgate, dscale)`` -- a branch's way back into the residual stream and the norm
+  that follows; gradients of what is absent are empty, and ``dy`` where it is
+  ``dx`` (gmdn_amd.residual).
+* ``gmdn::linear_logprobs_fwd(x, weight, tokens, ignore_index) -> (logprob,
+  entropy, stats)`` and ``gmdn::linear_logprobs_bwd(x, weight, tokens, stats,
+  entropy, dlogprob, dentropy, ignore_index, need_x, need_weight) -> (dx,
+  dweight)`` -- log probabilities from hidden states and the head's weight,
+  without the logits (gmdn_amd.logprobs).
 * ``gmdn::msign(M, steps, eps) -> X`` -- the outer Muon optimizer's msign of
   a batch of matrices (train_ablation.py:60-73); no autograd (the optimizer
   runs it under ``no_grad``).
@@ -242,6 +256,36 @@ def _logprobs_bwd_fake(logits, tokens, stats, entropy, top_tokens, dlogprob, den
     return logits.new_empty(logits.shape)
 
 
+def _embed_fwd_fake(weight, tokens, scale=1.0, padding_idx=-1):
+    return weight.new_empty((*tokens.shape, weight.shape[1]))
+
+
+def _embed_bwd_fake(dy, tokens, vocab, scale, padding_idx):
+    return dy.new_empty((vocab, dy.shape[-1]))
+
+
+def _residual_norm_fwd_fake(x, y, weight, post_weight, gate, scale, eps):
+    lead = x.shape[:-1]
+    return (x.new_empty(x.shape), y.new_empty(x.shape), x.new_empty(lead, dtype=torch.float32),
+            x.new_empty(lead if post_weight is not None else (0,), dtype=torch.float32))
+
+
+def _residual_norm_bwd_fake(dr, dz, r, y, weight, post_weight, gate, scale, rstd, post_rstd):
+    same = post_weight is None and gate is None and scale is None and r.dtype == y.dtype
+    dw, dp, ds = (v.new_empty(v.shape) if v is not None else _empty(r) for v in (weight, post_weight, scale))
+    return (r.new_empty(r.shape), y.new_empty((0,) if same else r.shape), dw, dp,
+            y.new_empty(r.shape if gate is not None else (0,)), ds)
+
+
+def _linear_logprobs_fwd_fake(x, weight, tokens, ignore_index):
+    lead = x.shape[:-1]
+    return (*(x.new_empty(lead, dtype=torch.float32) for _ in range(2)), x.new_empty((*lead, 2), dtype=torch.float32))
+
+
+def _linear_logprobs_bwd_fake(x, weight, tokens, stats, entropy, dlogprob, dentropy, ignore_index, need_x, need_weight):
+    return x.new_empty(x.shape if need_x else (0,)), weight.new_empty(weight.shape if need_weight else (0,))
+
+
 _FAKES = {
     "state_scan": _state_scan_fake,
     "state_scan_bwd": _state_scan_bwd_fake,
@@ -266,6 +310,12 @@ _FAKES = {
     "gelu8_bwd": _gelu8_bwd_fake,
     "logprobs_fwd": _logprobs_fwd_fake,
     "logprobs_bwd": _logprobs_bwd_fake,
+    "embed_fwd": _embed_fwd_fake,
+    "embed_bwd": _embed_bwd_fake,
+    "residual_norm_fwd": _residual_norm_fwd_fake,
+    "residual_norm_bwd": _residual_norm_bwd_fake,
+    "linear_logprobs_fwd": _linear_logprobs_fwd_fake,
+    "linear_logprobs_bwd": _linear_logprobs_bwd_fake,
 }
 # Set by _register_fakes.  Without the native libraries the operators do not
 # exist: every entry point calls ensure(), which raises what _native.load raises.
@@ -293,6 +343,15 @@ def ensure() -> None:
 def wants_grad(*tensors: Tensor | None) -> bool:
     """Whether a call on these tensors is recorded for a backward."""
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def autocast_dtype(t: Tensor) -> torch.dtype | None:
+    """The type that autocast has products on ``t``'s device run in; None
+    without it (and on devices that have none, as meta)."""
+    dev = t.device.type
+    if dev not in ("cuda", "cpu") or not torch.is_autocast_enabled(dev):
+        return None
+    return torch.get_autocast_dtype(dev)
 
 
 def __getattr__(name: str):

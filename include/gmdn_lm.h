@@ -1,6 +1,7 @@
 /* C-ABI of the operators of an LM's training and scoring step around the
- * mixer in libgmdn_scan.so (MI355X, gfx950): layer norm, 8-bit activation
- * checkpoints, and log probabilities of given tokens.
+ * mixer in libgmdn_scan.so (MI355X, gfx950): token embedding, layer norm, a
+ * branch's residual with its norms, 8-bit activation checkpoints, and log
+ * probabilities of given tokens.
  *
  * Matrices are (rows, d) with unit-stride rows; inputs take a row stride in
  * elements (any value >= 0: a slice of a wider tensor, a broadcast row),
@@ -55,6 +56,50 @@ int gmdn_layer_norm8_rebuild(const int8_t* q, const float* scale, const void* we
                              const float* mean, const float* rstd, void* y, int64_t rows, int64_t d, int32_t y_type,
                              int32_t w_type, void* stream);
 
+/* ------------------------------------------------------------ token embedding
+ * y (rows, d) = scale * weight[token]; a token outside [0, vocab) gives a row of
+ * NaN.  weight is (vocab, d) with a row stride; vocab <= 2^27, d <= 2^20, and
+ * y at most 2^32 pieces of eight values. */
+int gmdn_embed_fwd(const void* weight, const int64_t* tokens, void* y, int64_t rows, int64_t vocab, int64_t d,
+                   int64_t w_stride, float scale, int32_t dtype, void* stream);
+
+/* Bytes of the backward's workspace (256-byte aligned). */
+size_t gmdn_embed_bwd_workspace_bytes(int64_t rows, int64_t vocab, int64_t d);
+
+/* dweight (vocab, d), every row of it: scale times the sum of the rows of dy whose
+ * token it is, zeros where there are none.  The rows of tokens outside the vocabulary and of
+ * padding_idx (any value outside it: none) are left out. */
+int gmdn_embed_bwd(const void* dy, const int64_t* tokens, void* dweight, void* workspace, size_t workspace_bytes,
+                   int64_t rows, int64_t vocab, int64_t d, int64_t dy_stride, float scale, int64_t padding_idx,
+                   int32_t dtype, void* stream);
+
+/* ------------------------------------------------------ residual with its norms
+ * r = x + scale sigmoid(gate) n and z = r rstd weight over rows of d <= 8192
+ * values, with n = y post_rstd post_weight (n = y where post_weight is NULL),
+ * rstd = 1 / sqrt(mean(r^2) + eps) and post_rstd the same of y.  x is the stream,
+ * y a branch's output; gate (rows, d) holds logits; weight, post_weight and
+ * scale are (d), of one type.  Each of the last four may be NULL: 1.
+ * (x_type, y_type) is (bf16, bf16), (f32, f32) or (f32, bf16); r has x's type,
+ * gate and z have y's.  z is computed from r before r is rounded.  rstd and
+ * post_rstd (rows) are kept for the backward. */
+int gmdn_residual_norm_fwd(const void* x, const void* y, const void* weight, const void* post_weight, const void* gate,
+                           const void* scale, void* r, void* z, float* rstd, float* post_rstd, int64_t rows, int64_t d,
+                           int64_t x_stride, int64_t y_stride, int64_t gate_stride, float eps, int32_t x_type,
+                           int32_t y_type, int32_t w_type, void* stream);
+
+/* Floats of the backward's workspace (sums of the vectors' gradients). */
+size_t gmdn_residual_norm_bwd_workspace_floats(int64_t rows, int64_t d);
+
+/* The gradients from dr and dz (either may be NULL: zeros) and what the forward
+ * kept.  dy may be NULL where it would be dx: no post norm, gate or scale, and
+ * one type.  dweight, dpost_weight and dscale may be NULL each. */
+int gmdn_residual_norm_bwd(const void* dr, const void* dz, const void* r, const void* y, const void* weight,
+                           const void* post_weight, const void* gate, const void* scale, const float* rstd,
+                           const float* post_rstd, void* dx, void* dy, void* dgate, void* dweight, void* dpost_weight,
+                           void* dscale, float* workspace, size_t workspace_floats, int64_t rows, int64_t d,
+                           int64_t dr_stride, int64_t dz_stride, int64_t r_stride, int64_t y_stride,
+                           int64_t gate_stride, int32_t x_type, int32_t y_type, int32_t w_type, void* stream);
+
 /* ------------------------------------------------------- 8-bit checkpoints */
 /* Groups of a row: ceil(d / 128). */
 int64_t gmdn_act8_groups(int64_t d);
@@ -98,6 +143,32 @@ int gmdn_logprobs_bwd(const void* logits, const int64_t* tokens, const float* st
                       const int64_t* top_tokens, const float* dlogprob, const float* dentropy, const float* dtop,
                       void* dlogits, int64_t rows, int64_t vocab, int64_t stride, int32_t top, int64_t ignore_index,
                       int32_t dtype, void* stream);
+
+/* -------------------------------- log probabilities from hidden states and a head
+ * The same of the logits x weight^T, without them in memory: x (rows, d) and weight
+ * (vocab, d) of one type, each with a row stride; vocab <= 2^27, d <= 2^17.
+ * logprob, entropy and stats are as above.  bfloat16 operands are multiplied as they
+ * are (rows of a multiple of 64 values at 16-byte addresses from where they lie, others
+ * from copies in the workspace), float32 ones as three products of bfloat16 pieces,
+ * about 2^-16 relative error a product. */
+size_t gmdn_linear_logprobs_fwd_workspace_bytes(const void* x, const void* weight, int64_t rows, int64_t vocab,
+                                                int64_t d, int64_t x_stride, int64_t w_stride, int32_t dtype);
+int gmdn_linear_logprobs_fwd(const void* x, const void* weight, const int64_t* tokens, float* logprob, float* entropy,
+                             float* stats, void* workspace, size_t workspace_bytes, int64_t rows, int64_t vocab,
+                             int64_t d, int64_t x_stride, int64_t w_stride, int64_t ignore_index, int32_t dtype,
+                             void* stream);
+
+/* dx (rows, d) and dweight (vocab, d), of the operands' type; either may be NULL.
+ * dlogprob and dentropy may each be NULL: zeros.  The logits' gradient, of which the
+ * workspace holds a piece of the vocabulary at a time, is rounded as the operands
+ * are. */
+size_t gmdn_linear_logprobs_bwd_workspace_bytes(const void* x, const void* weight, int64_t rows, int64_t vocab,
+                                                int64_t d, int64_t x_stride, int64_t w_stride, int32_t dtype);
+int gmdn_linear_logprobs_bwd(const void* x, const void* weight, const int64_t* tokens, const float* stats,
+                             const float* entropy, const float* dlogprob, const float* dentropy, void* dx,
+                             void* dweight, void* workspace, size_t workspace_bytes, int64_t rows, int64_t vocab,
+                             int64_t d, int64_t x_stride, int64_t w_stride, int64_t ignore_index, int32_t dtype,
+                             void* stream);
 
 #ifdef __cplusplus
 }
