@@ -30,7 +30,9 @@ import torch.nn.functional as F
 from . import act8, logprobs
 from . import ops  # registers torch.ops.gmdn.*
 from .chunk import chunk_scan
+from .embedding import Embedding
 from .layer_norm import LayerNorm, checked_checkpoint
+from .residual import residual_norm
 
 
 class FastWeightMixer(nn.Module):
@@ -122,6 +124,58 @@ def _plain(module: nn.Module, kind: type) -> bool:
         module._forward_hooks or module._forward_pre_hooks or module._backward_hooks or module._backward_pre_hooks)
 
 
+def _norm_eps(norm: nn.RMSNorm) -> float:
+    """What the norm adds to the mean square: by default the epsilon of float32,
+    which it computes in whatever its input's type."""
+    return norm.eps if norm.eps is not None else torch.finfo(torch.float32).eps
+
+
+def _one_type(*vectors: torch.Tensor | None):
+    """The vectors in one type: their own where they share it, else float32."""
+    if len({v.dtype for v in vectors if v is not None}) <= 1:
+        return vectors
+    return tuple(v if v is None else v.float() for v in vectors)
+
+
+class Branch(nn.Module):
+    """What a block with ``residual="fused"`` does with a branch's output on its
+    way back into the stream, beside adding it: a norm, a sigmoid gate of the branch's
+    input, a learned scale of each channel."""
+
+    def __init__(self, d_model: int, post_norm: bool, gated: bool, layer_scale: float | None):
+        super().__init__()
+        self.post = nn.RMSNorm(d_model) if post_norm else None
+        self.gate = nn.Linear(d_model, d_model) if gated else None
+        self.scale = None if layer_scale is None else nn.Parameter(torch.full((d_model,), float(layer_scale)))
+
+    def forward(self, x, y, z, norm):
+        """(r, norm(r)) of the stream ``x``, the branch's output ``y`` and its
+        input ``z``; (r, None) without a norm."""
+        if x.dtype != torch.float32 and y.dtype == torch.float32:
+            x = x.float()  # as their sum would be
+        gate = None if self.gate is None else self.gate(z).to(y.dtype)
+        fused = norm is not None and _plain(norm, nn.RMSNorm)
+        eps = _norm_eps(norm) if fused else None
+        post, inside = self.post, False
+        if post is not None:
+            # inside the operator where it is the plain module, and its epsilon the norm's
+            inside = _plain(post, nn.RMSNorm) and post.weight is not None
+            inside = inside and (not fused or _norm_eps(post) == eps)
+            if inside:
+                eps = _norm_eps(post)
+            else:
+                y = post(y).to(y.dtype)
+        if norm is None and not inside and gate is None and self.scale is None:
+            return x + y, None
+        weight, post_weight, scale = _one_type(norm.weight if fused else None, post.weight if inside else None,
+                                               self.scale)
+        r, z = residual_norm(x, y, weight, post_weight=post_weight, gate=gate, scale=scale,
+                             eps=1e-6 if eps is None else eps)
+        if fused or norm is None:
+            return r, z if fused else None
+        return r, norm(r)
+
+
 class Block(nn.Module):
     """Pre-norm residual block: mixer, then a 4x GELU MLP (train_ablation.py:197-210).
 
@@ -131,16 +185,33 @@ class Block(nn.Module):
     That is one operator in place of the MLP's modules, and of the norm before
     it: where one of them is replaced, has a hook or a bias, they are called
     as they are, and keep what they keep.
+
+    ``residual="fused"`` (RMSNorm) adds a branch's output to the stream and norms
+    the sum for the next branch in one pass (gmdn_amd.residual); with it ``post_norm``
+    norms a branch's output before it is added, ``gated`` multiplies it by a sigmoid
+    of a linear layer of the branch's input, and ``layer_scale`` by a learned scale of each
+    channel that begins at this value.  A norm that is replaced or has a hook is
+    called as it is.
     """
 
-    def __init__(self, d_model, n_heads, inner, chunk, ns_steps=3, norm="rms", checkpoint=None):
+    def __init__(self, d_model, n_heads, inner, chunk, ns_steps=3, norm="rms", checkpoint=None, residual="torch",
+                 post_norm=False, gated=False, layer_scale=None):
         super().__init__()
+        if residual not in ("torch", "fused"):
+            raise ValueError(f"residual is 'torch' or 'fused', got {residual!r}")
+        if residual == "fused" and norm != "rms":
+            raise ValueError(f"residual='fused' goes with norm='rms', got {norm!r}")
+        if residual != "fused" and (post_norm or gated or layer_scale is not None):
+            raise ValueError("post_norm, gated and layer_scale go with residual='fused'")
         self.keep8 = checked_checkpoint(checkpoint)
         self.n1 = _norm(norm, d_model, checkpoint)
         self.mixer = FastWeightMixer(d_model, n_heads, inner, chunk, ns_steps)
         self.n2 = _norm(norm, d_model, checkpoint)
         self.mlp = nn.Sequential(nn.Linear(d_model, 4 * d_model, bias=False), nn.GELU(),
                                  nn.Linear(4 * d_model, d_model, bias=False))
+        self.fused = residual == "fused"
+        if self.fused:
+            self.join1, self.join2 = (Branch(d_model, post_norm, gated, layer_scale) for _ in range(2))
 
     def _mlp_is_plain(self):
         m = self.mlp
@@ -156,7 +227,22 @@ class Block(nn.Module):
             return act8.norm_mlp(x, self.n2.weight, self.n2.bias, w1, w2, self.n2.eps)
         return act8.mlp(self.n2(x), w1, w2)
 
+    def _mlp_of(self, z):
+        """The MLP of what ``n2`` gave."""
+        if self.keep8 and self._mlp_is_plain():
+            return act8.mlp(z, self.mlp[0].weight, self.mlp[2].weight)
+        return self.mlp(z)
+
+    def step(self, x, z, norm):
+        """A block of ``residual="fused"`` from the stream ``x`` and its norm ``z``:
+        the stream after it and that one's norm by ``norm``, the module of the next
+        branch (None without one)."""
+        x, z = self.join1(x, self.mixer(z), z, self.n2)
+        return self.join2(x, self._mlp_of(z), z, norm)
+
     def forward(self, x):
+        if self.fused:
+            return self.step(x, self.n1(x), None)[0]
         x = x + self.mixer(self.n1(x))
         return x + self._mlp(x)
 
@@ -165,20 +251,30 @@ class LM(nn.Module):
     """Embedding, blocks, final RMSNorm and a tied head; next-token cross
     entropy in float32 (train_ablation.py:213-243).
 
-    ``norm`` and ``checkpoint`` are the blocks'.  ``loss="logprobs"`` takes the
-    same loss from the logits where they are, without their float32 copy
-    (gmdn_amd.logprobs).
+    ``norm``, ``checkpoint``, ``residual``, ``post_norm``, ``gated`` and
+    ``layer_scale`` are the blocks'; with ``residual="fused"`` the norm before each
+    branch, and the final one, comes from the pass that adds the branch before it.
+    ``loss="logprobs"`` takes the same loss from the logits where they are, without
+    their float32 copy; ``loss="linear"`` takes it from the hidden states and the
+    head's weight without the logits, which a call with targets then gives as None,
+    and scores the same way (gmdn_amd.logprobs).  ``embedding="sorted"`` looks
+    tokens up by gmdn_amd.embedding, times ``emb_scale``.
     """
 
     def __init__(self, vocab, d_model, n_layers, n_heads, inner, chunk=64, ns_steps=3, norm="rms", checkpoint=None,
-                 loss="torch"):
+                 loss="torch", residual="torch", post_norm=False, gated=False, layer_scale=None, embedding="torch",
+                 emb_scale=1.0):
         super().__init__()
-        if loss not in ("torch", "logprobs"):
-            raise ValueError(f"loss is 'torch' or 'logprobs', got {loss!r}")
+        if loss not in ("torch", "logprobs", "linear"):
+            raise ValueError(f"loss is 'torch', 'logprobs' or 'linear', got {loss!r}")
+        if embedding not in ("torch", "sorted"):
+            raise ValueError(f"embedding is 'torch' or 'sorted', got {embedding!r}")
+        if embedding == "torch" and emb_scale != 1.0:
+            raise ValueError("emb_scale goes with embedding='sorted'")
         self.loss = loss
-        self.emb = nn.Embedding(vocab, d_model)
-        self.blocks = nn.ModuleList(Block(d_model, n_heads, inner, chunk, ns_steps, norm, checkpoint)
-                                    for _ in range(n_layers))
+        self.emb = Embedding(vocab, d_model, scale=emb_scale) if embedding == "sorted" else nn.Embedding(vocab, d_model)
+        self.blocks = nn.ModuleList(Block(d_model, n_heads, inner, chunk, ns_steps, norm, checkpoint, residual, post_norm,
+                                          gated, layer_scale) for _ in range(n_layers))
         self.norm_f = _norm(norm, d_model, checkpoint)
         self.lm_head = nn.Linear(d_model, vocab, bias=False)
         self.lm_head.weight = self.emb.weight  # tied
@@ -197,11 +293,29 @@ class LM(nn.Module):
         elif isinstance(m, nn.Embedding):
             nn.init.normal_(m.weight, std=0.02)
 
-    def forward(self, idx, targets=None):
+    def _hidden(self, idx):
+        """What the head reads."""
         x = self.emb(idx)
+        if self.blocks and all(blk.fused and _plain(blk, Block) for blk in self.blocks):
+            norms = [*(blk.n1 for blk in self.blocks[1:]), self.norm_f]
+            z = self.blocks[0].n1(x)
+            for blk, norm in zip(self.blocks, norms):
+                x, z = blk.step(x, z, norm)
+            return z
         for blk in self.blocks:
             x = blk(x)
-        logits = self.lm_head(self.norm_f(x))
+        return self.norm_f(x)
+
+    def _head_is_plain(self):
+        return _plain(self.lm_head, nn.Linear) and self.lm_head.bias is None
+
+    def forward(self, idx, targets=None):
+        x = self._hidden(idx)
+        if targets is not None and self.loss == "linear":
+            if self._head_is_plain():
+                return None, logprobs.linear_cross_entropy(x, self.lm_head.weight, targets)
+            return None, logprobs.cross_entropy(self.lm_head(x), targets)
+        logits = self.lm_head(x)
         if targets is None:
             return logits, None
         if self.loss == "logprobs":
@@ -216,4 +330,8 @@ class LM(nn.Module):
         with entropies and ``top`` alternatives (``TokenLogprobs``)."""
         if tokens is None:
             tokens = F.pad(idx[:, 1:], (0, 1), value=logprobs.IGNORE)
+        if self.loss == "linear" and top == 0 and self._head_is_plain():
+            lp, entropy = logprobs.linear_logprobs(self._hidden(idx), self.lm_head.weight, tokens)
+            none = lp.new_empty((*lp.shape, 0))
+            return logprobs.TokenLogprobs(lp, entropy, none, none.long())
         return logprobs.token_logprobs(self(idx)[0], tokens, top)
