@@ -48,6 +48,7 @@ constexpr int SORT_THREADS = 1024;
 constexpr int SORT_WAVES = SORT_THREADS / 64;
 constexpr int SORT_BITS = 9;
 constexpr int SORT_BINS = 1 << SORT_BITS;
+constexpr int SORT_AHEAD = 8;            // keys of a thread in flight while it counts
 constexpr int SORT_TILES = 256;          // at most; a tile is a multiple of SORT_THREADS
 constexpr int64_t SORT_SELF = 32768;     // up to here each workgroup counts all digits itself
 
@@ -117,14 +118,25 @@ em_scatter(SortInput in, const uint32_t* __restrict__ counts, uint32_t* __restri
       below[t] = less;
     }
   } else {
-    for (int64_t i0 = 0; i0 < in.n; i0 += SORT_THREADS) {
-      const int64_t i = i0 + t;
-      const bool live = i < in.n;
-      const uint32_t digit = live ? digit_of(in.key(i)) : 0;
-      const uint64_t peers = same_digit(digit, live, bits);
-      if (live && (peers & before) == 0) {
-        atomicAdd(&total[digit], (uint32_t)__popcll(peers));
-        if (i0 < first) atomicAdd(&below[digit], (uint32_t)__popcll(peers));
+    // eight keys of a thread in flight: one after another they would wait for memory
+    // sixteen times for 16384 tokens
+    for (int64_t i0 = 0; i0 < in.n; i0 += SORT_AHEAD * SORT_THREADS) {
+      uint32_t key[SORT_AHEAD];
+#pragma unroll
+      for (int j = 0; j < SORT_AHEAD; ++j) {
+        const int64_t i = i0 + j * SORT_THREADS + t;
+        key[j] = in.key(i < in.n ? i : in.n - 1);
+      }
+#pragma unroll
+      for (int j = 0; j < SORT_AHEAD; ++j) {
+        const int64_t at = i0 + j * SORT_THREADS;
+        const bool live = at + t < in.n;
+        const uint32_t digit = digit_of(key[j]);
+        const uint64_t peers = same_digit(digit, live, bits);
+        if (live && (peers & before) == 0) {
+          atomicAdd(&total[digit], (uint32_t)__popcll(peers));
+          if (at < first) atomicAdd(&below[digit], (uint32_t)__popcll(peers));
+        }
       }
     }
   }

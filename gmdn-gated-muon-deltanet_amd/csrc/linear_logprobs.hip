@@ -317,8 +317,10 @@ ll_sum_planes(const float* __restrict__ planes, T* __restrict__ out, int64_t n, 
 }
 
 // ------------------------------------------------------------------ the calls
-using Big = MMShape<256, 256, 64, 2, 2, 4>;
-using Small = MMShape<64, 64, 64, 3, 2, 2>;
+// Tiles of 256, 128 and 64: 8 waves of 128 x 64, 4 of 64 x 64 and of 32 x 32.
+using Tile256 = MMShape<256, 256, 64, 2, 2, 4>;
+using Tile128 = MMShape<128, 128, 64, 2, 2, 2>;
+using Tile64 = MMShape<64, 64, 64, 3, 2, 2>;
 
 int64_t div_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 int64_t round_up(int64_t a, int64_t b) { return div_up(a, b) * b; }
@@ -330,29 +332,59 @@ bool in_place(const void* p, int64_t stride, int64_t d, int32_t dtype) {
   return dtype == GMDN_DTYPE_BF16 && d % KPAD == 0 && stride % 8 == 0 && stride <= (1 << 22) && (uintptr_t)p % 16 == 0;
 }
 
-struct Sizes {
-  int64_t rows, V, d, kp;
-  int P;
-  bool x_in, w_in, big;
-  size_t x, w;                     // bytes of the operands' planes
-  // forward
-  int64_t tiles;                   // of the vocabulary
-  size_t at_token, part;
-  // backward
-  int64_t piece, pieces, padded;   // columns, pieces, rows of d
-  int x_per, x_splits, w_per, w_splits;  // stages of a split, splits
-  size_t grad, x_acc, w_acc;
-  size_t forward() const { return x + w + at_token + part; }
-  size_t backward() const { return x + w + grad + x_acc + w_acc; }
+// How a product of tiles_m x tiles_n tiles over `steps` stages of k runs: which
+// tile, and the stages of a split along k.
+struct Product {
+  int edge, per, splits;
 };
-
-// A product of few tiles is split along k until the chip is filled, while a part
-// keeps four stages or more.
+// A product of few tiles is split until the chip is filled, while a part keeps four
+// stages or more.
 int splits_of(int64_t tiles, int64_t steps) {
   int64_t s = 256 / tiles;
   if (s > steps / 4) s = steps / 4;
   return (int)(s < 1 ? 1 : s > 64 ? 64 : s);
 }
+// The tile of the least cost: rounds over the 256 CUs, times a tile's work at the rate that its
+// reads from LDS leave it, of two stages more than it has (its ramp and epilogue).  For a stage
+// of 32 k the matrix units take 1024, 256 and 64 clocks, LDS at 128 bytes a clock 1024,
+// 384 and 192: rates as 6 to 4 to 2.
+Product product_of(int64_t M, int64_t N, int64_t steps, int pairs, bool split) {
+  Product best{};
+  double least = 0;
+  const int edges[3] = {64, 128, 256}, clocks[3] = {6, 3, 2};
+  for (int i = 0; i < 3; ++i) {
+    const int64_t e = edges[i], tiles = div_up(M, e) * div_up(N, e);
+    Product p{edges[i], (int)div_up(steps, split ? splits_of(tiles, steps) : 1), 1};
+    p.splits = (int)div_up(steps, p.per);
+    const double cost = (double)div_up(tiles * p.splits, 256) * (double)(e * e) * (p.per * pairs + 2) * clocks[i];
+    if (i == 0 || cost < least) {
+      best = p;
+      least = cost;
+    }
+  }
+  return best;
+}
+// f(tile's shape)
+template <class F>
+bool with_tile(const Product& p, F&& f) {
+  return p.edge == 64 ? f(Tile64{}) : p.edge == 128 ? f(Tile128{}) : f(Tile256{});
+}
+
+struct Sizes {
+  int64_t rows, V, d, kp;
+  int P, pairs;
+  bool x_in, w_in;
+  size_t x, w;                     // bytes of the operands' planes
+  // forward
+  Product logits;
+  size_t at_token, part;
+  // backward
+  int64_t piece, pieces, padded;   // columns, pieces, rows of d
+  Product again, for_x, for_w;     // a piece's logits, and the products for dx and dW
+  size_t grad, x_acc, w_acc;
+  size_t forward() const { return x + w + at_token + part; }
+  size_t backward() const { return x + w + grad + x_acc + w_acc; }
+};
 
 Sizes sizes_of(const void* x, const void* w, int64_t rows, int64_t V, int64_t d, int64_t xs, int64_t ws, int32_t dtype) {
   Sizes z{};
@@ -361,35 +393,40 @@ Sizes sizes_of(const void* x, const void* w, int64_t rows, int64_t V, int64_t d,
   z.d = d;
   z.kp = round_up(d, KPAD);
   z.P = dtype == GMDN_DTYPE_F32 ? 2 : 1;
+  z.pairs = z.P == 1 ? 1 : 3;
   z.x_in = in_place(x, xs, d, dtype);
   z.w_in = in_place(w, ws, d, dtype);
   z.x = z.x_in ? 0 : up((size_t)(z.P * rows * z.kp * 2));
   z.w = z.w_in ? 0 : up((size_t)(z.P * V * z.kp * 2));
-  z.big = div_up(V, 256) * div_up(rows, 256) >= 256;
-  const int64_t tile = z.big ? 256 : 64;
-  z.tiles = div_up(V, tile);
+  z.logits = product_of(V, rows, z.kp / KPAD, z.pairs, false);
   z.at_token = up((size_t)rows * 4);
-  z.part = up((size_t)(z.tiles * 3 * rows * 4));
-  z.padded = round_up(rows, 64);
+  z.part = up((size_t)(div_up(V, z.logits.edge) * 3 * rows * 4));
+  z.padded = round_up(rows, KPAD);
   int64_t most = PIECE_BYTES / (z.padded * 2 * z.P) / UNIT * UNIT;
   most = most < UNIT ? UNIT : most > PIECE_MOST ? PIECE_MOST : most;
   z.pieces = div_up(V, most);
   z.piece = round_up(div_up(V, z.pieces), UNIT);
   z.pieces = div_up(V, z.piece);
   z.grad = up((size_t)(z.P * z.padded * z.piece * 2));
-  const int64_t most_v = z.piece < V ? z.piece : V, x_steps = div_up(most_v, 64), w_steps = z.padded / 64;
-  z.x_per = (int)div_up(x_steps, splits_of(div_up(d, tile) * div_up(rows, tile), x_steps));
-  z.w_per = (int)div_up(w_steps, splits_of(div_up(d, tile) * div_up(most_v, tile), w_steps));
-  z.x_splits = (int)div_up(x_steps, z.x_per);
-  z.w_splits = (int)div_up(w_steps, z.w_per);
-  z.x_acc = z.x_splits > 1 || z.pieces > 1 ? up((size_t)(z.x_splits * rows * d * 4)) : 0;
-  z.w_acc = z.w_splits > 1 ? up((size_t)(z.w_splits * most_v * d * 4)) : 0;
+  // every piece as the first: the last may be shorter
+  const int64_t columns = z.piece < V ? z.piece : V;
+  z.again = product_of(columns, rows, z.kp / KPAD, z.pairs, false);
+  z.for_x = product_of(d, rows, div_up(columns, KPAD), z.pairs, true);
+  z.for_w = product_of(d, columns, z.padded / KPAD, z.pairs, true);
+  z.x_acc = z.for_x.splits > 1 || z.pieces > 1 ? up((size_t)(z.for_x.splits * rows * d * 4)) : 0;
+  z.w_acc = z.for_w.splits > 1 ? up((size_t)(z.for_w.splits * columns * d * 4)) : 0;
   return z;
 }
 
 int check_ll(int64_t rows, int64_t V, int64_t d, int64_t xs, int64_t ws, int32_t dtype) {
   if (rows < 0 || V <= 0 || d <= 0 || xs < 0 || ws < 0 || rows > ((int64_t)1 << 30)) return GMDN_ERR_ARG;
-  return !type_ok(dtype) || V > (1 << 27) || d > (1 << 17) ? GMDN_ERR_UNSUPPORTED : GMDN_OK;
+  if (!type_ok(dtype) || V > (1 << 27) || d > (1 << 17)) return GMDN_ERR_UNSUPPORTED;
+  // what a launch's grid holds: 2^32 threads (tiles below 256 are taken where one side has
+  // few of them)
+  const int64_t longer = rows > V ? rows : V, most = 1 << 22;
+  const bool fits = div_up(V, 256) * div_up(rows, 256) <= most && div_up(d, 256) * div_up(longer, 256) <= most &&
+                    longer * (round_up(d, KPAD) / 8) < (int64_t)1 << 32;
+  return fits ? GMDN_OK : GMDN_ERR_UNSUPPORTED;
 }
 
 // An operand's planes: where it lies, or made at `at`, which moves on.
@@ -404,24 +441,20 @@ const bf16* planes_of(const T* x, int64_t stride, int64_t rows, const Sizes& z, 
   return out;
 }
 
-// The pairs of planes of a product, the small terms first: lo hi, hi lo, hi hi.
-void set_pairs(MMArgs& a, int P) {
-  a.pairs = P == 1 ? 1 : 3;
-  a.pair_a = P == 1 ? 0 : 0x001;
-  a.pair_b = P == 1 ? 0 : 0x010;
-}
-
+// A product's arguments; the pairs of planes with the small terms first: lo hi, hi lo, hi hi.
 template <class S>
-MMArgs args_of(const MMOperand& a, const MMOperand& b, int64_t M, int64_t N, int64_t k, int P, int per) {
+MMArgs args_of(const MMOperand& a, const MMOperand& b, int64_t M, int64_t N, int64_t k, int pairs, int per) {
   static_assert(S::BK == KPAD, "a stage is what the operands are padded to");
   MMArgs r{};
   r.a = a;
   r.b = b;
   r.steps = (int)div_up(k, S::BK);
-  r.per = per ? per : r.steps;
+  r.per = per;
   r.tiles_m = (int)div_up(M, S::TM);
   r.tiles_n = (int)div_up(N, S::TN);
-  set_pairs(r, P);
+  r.pairs = pairs;
+  r.pair_a = pairs == 1 ? 0 : 0x001;
+  r.pair_b = pairs == 1 ? 0 : 0x010;
   return r;
 }
 
@@ -445,13 +478,8 @@ Matrices matrices_of(const void* x, const void* w, int64_t xs, int64_t ws, const
 template <class S, class Epi>
 bool logits(const Matrices& m, const Sizes& z, int64_t v0, int64_t columns, const Epi& epi, hipStream_t st) {
   const MMArgs a = args_of<S>({m.w + v0 * m.ws, m.ws, m.wp, columns - 1, 0}, {m.x, m.xs, m.xp, z.rows - 1, 0}, columns,
-                              z.rows, z.kp, z.P, 0);
+                              z.rows, z.kp, z.pairs, (int)(z.kp / KPAD));
   return mm_launch<S, false, false, true>(a, epi, 1, st);
-}
-
-template <class S>
-bool forward(const Matrices& m, const Sizes& z, const SumsArgs& e, hipStream_t st) {
-  return logits<S>(m, z, 0, z.V, SumsEpi<S, true>{e}, st);
 }
 
 template <typename T>
@@ -459,31 +487,43 @@ void sum_planes(const float* planes, T* out, int64_t n, int count, hipStream_t s
   hipLaunchKernelGGL((ll_sum_planes<T>), dim3((unsigned)div_up(n, 8 * 256)), dim3(256), 0, st, planes, out, n, count);
 }
 
-template <class S, typename T>
+template <typename T>
 bool backward(const Matrices& m, const Sizes& z, GradArgs e, float* x_acc, float* w_acc, T* dx, T* dw, hipStream_t st) {
   constexpr int P = std::is_same_v<T, float> ? 2 : 1;
   const int64_t plane = z.padded * z.piece;
   for (int64_t i = 0; i < z.pieces; ++i) {
     const int64_t v0 = i * z.piece, left = z.V - v0 < z.piece ? z.V - v0 : z.piece;
+    const bool last = i + 1 == z.pieces;
     e.first = v0;
     e.left = left;
-    if (!logits<S>(m, z, v0, left, GradEpi<S, true, P>{e}, st)) return false;
-    if (dx) {
-      const bool last = i + 1 == z.pieces;
-      const MMArgs a = args_of<S>({m.w + v0 * m.ws, m.ws, m.wp, z.kp - 1, left - 1}, {e.d, z.piece, plane, z.rows - 1, 0},
-                                  z.d, z.rows, left, P, z.x_per);
-      const int splits = (int)div_up(a.steps, a.per);
-      const StoreArgs<T> s{x_acc, last && z.x_splits == 1 ? dx : nullptr, z.d, z.rows, i > 0};
-      if (!mm_launch<S, true, false, false>(a, StoreEpi<S, T>{s}, splits, st)) return false;
-      if (last && z.x_splits > 1) sum_planes(x_acc, dx, z.rows * z.d, z.x_splits, st);
+    bool ok = with_tile(z.again, [&](auto s) {
+      using S = decltype(s);
+      return logits<S>(m, z, v0, left, GradEpi<S, true, P>{e}, st);
+    });
+    if (dx && ok) {
+      const int count = z.for_x.splits;
+      const StoreArgs<T> to{x_acc, last && count == 1 ? dx : nullptr, z.d, z.rows, i > 0};
+      ok = with_tile(z.for_x, [&](auto s) {
+        using S = decltype(s);
+        const MMArgs a = args_of<S>({m.w + v0 * m.ws, m.ws, m.wp, z.kp - 1, left - 1},
+                                    {e.d, z.piece, plane, z.rows - 1, 0}, z.d, z.rows, left, z.pairs, z.for_x.per);
+        return mm_launch<S, true, false, false>(a, StoreEpi<S, T>{to}, (int)div_up(a.steps, a.per), st);
+      });
+      if (ok && last && count > 1) sum_planes(x_acc, dx, z.rows * z.d, count, st);
     }
-    if (dw) {
-      const MMArgs a = args_of<S>({m.x, m.xs, m.xp, z.kp - 1, z.rows - 1}, {e.d, z.piece, plane, z.piece - 1, z.padded - 1},
-                                  z.d, left, z.padded, P, z.w_per);
-      const StoreArgs<T> s{w_acc, z.w_splits == 1 ? dw + v0 * z.d : nullptr, z.d, left, false};
-      if (!mm_launch<S, true, true, false>(a, StoreEpi<S, T>{s}, z.w_splits, st)) return false;
-      if (z.w_splits > 1) sum_planes(w_acc, dw + v0 * z.d, left * z.d, z.w_splits, st);
+    if (dw && ok) {
+      const int count = z.for_w.splits;
+      const StoreArgs<T> to{w_acc, count == 1 ? dw + v0 * z.d : nullptr, z.d, left, false};
+      ok = with_tile(z.for_w, [&](auto s) {
+        using S = decltype(s);
+        const MMArgs a = args_of<S>({m.x, m.xs, m.xp, z.kp - 1, z.rows - 1},
+                                    {e.d, z.piece, plane, z.piece - 1, z.padded - 1}, z.d, left, z.padded, z.pairs,
+                                    z.for_w.per);
+        return mm_launch<S, true, true, false>(a, StoreEpi<S, T>{to}, count, st);
+      });
+      if (ok && count > 1) sum_planes(w_acc, dw + v0 * z.d, left * z.d, count, st);
     }
+    if (!ok) return false;
   }
   return true;
 }
@@ -515,13 +555,18 @@ int gmdn_linear_logprobs_fwd(const void* x, const void* weight, const int64_t* t
   const Matrices m = dtype == GMDN_DTYPE_F32 ? matrices_of<float>(x, weight, x_stride, w_stride, z, at, st)
                                              : matrices_of<bf16>(x, weight, x_stride, w_stride, z, at, st);
   const SumsArgs e{tokens, (float*)at, (float*)(at + z.at_token), rows, (int)vocab};
-  if (!(z.big ? forward<Big>(m, z, e, st) : forward<Small>(m, z, e, st))) return GMDN_ERR_LAUNCH;
+  const int tiles = (int)div_up(vocab, z.logits.edge);
+  const bool ok = with_tile(z.logits, [&](auto s) {
+    using S = decltype(s);
+    return logits<S>(m, z, 0, vocab, SumsEpi<S, true>{e}, st);
+  });
+  if (!ok) return GMDN_ERR_LAUNCH;
   if (rows <= JOIN_FEW)
     hipLaunchKernelGGL((ll_join<1>), dim3((unsigned)rows), dim3(256), 0, st, e.part, e.at_token, tokens, logprob, entropy,
-                       stats, (int)z.tiles, rows, vocab, ignore_index);
+                       stats, tiles, rows, vocab, ignore_index);
   else
     hipLaunchKernelGGL((ll_join<16>), dim3((unsigned)div_up(rows, 16)), dim3(256), 0, st, e.part, e.at_token, tokens,
-                       logprob, entropy, stats, (int)z.tiles, rows, vocab, ignore_index);
+                       logprob, entropy, stats, tiles, rows, vocab, ignore_index);
   return launched();
 }
 
@@ -549,13 +594,8 @@ int gmdn_linear_logprobs_bwd(const void* x, const void* weight, const int64_t* t
                   ignore_index};
   float* const xa = (float*)(at + z.grad);
   float* const wa = (float*)(at + z.grad + z.x_acc);
-  auto run = [&](auto s, auto t) {
-    using S = decltype(s);
-    using T = decltype(t);
-    return backward<S, T>(m, z, e, xa, wa, (T*)dx, (T*)dweight, st);
-  };
-  const bool ok = dtype == GMDN_DTYPE_F32 ? (z.big ? run(Big{}, float{}) : run(Small{}, float{}))
-                                          : (z.big ? run(Big{}, bf16{}) : run(Small{}, bf16{}));
+  const bool ok = dtype == GMDN_DTYPE_F32 ? backward<float>(m, z, e, xa, wa, (float*)dx, (float*)dweight, st)
+                                          : backward<bf16>(m, z, e, xa, wa, (bf16*)dx, (bf16*)dweight, st);
   return ok ? launched() : GMDN_ERR_LAUNCH;
 }
 

@@ -103,9 +103,11 @@ def test_forward_backward(rows, V, D, dtype):
 
 
 @pytest.mark.parametrize("dtype", [B, F])
-@pytest.mark.parametrize("rows,V,D", [(4001, 4200, 72), (1000, 16500, 64), (4096, 4096, 65), (300, 33000, 128)])
-def test_large_tiles(rows, V, D, dtype):
-    """Products of 256 tiles of 256 x 256 or more."""
+@pytest.mark.parametrize("rows,V,D", [(4001, 4200, 72), (1000, 16500, 64), (4096, 4096, 65), (300, 33000, 128),
+                                      (1500, 3001, 200), (257, 2000, 1000)])
+def test_large_products(rows, V, D, dtype):
+    """Sizes at which the products are cut into larger tiles, whole and ragged, and
+    split along k."""
     _run(rows, V, D, dtype, rows + V + D)
 
 
