@@ -58,9 +58,9 @@ struct MMPlan {
   static constexpr int GPR = COLS / 8, NOPS = T * BK / 8 / THREADS;
   static constexpr int BYTES = PAIRS ? BK / 2 * PAIR : T * BK * 2;
   static_assert(T * BK / 8 % THREADS == 0, "a tile splits evenly over the workgroup");
-  // PERM: within 64 rows, row 16 mt + 4 G + j of the tile is the operand's 16 G + 4 mt
-  // + j, so that a lane's four tiles hold sixteen consecutive m.
-  static GMDN_DEV int row_of(int r) { return PERM ? (r & ~63) | ((r & 12) << 2) | ((r & 48) >> 2) | (r & 3) : r; }
+  // PERM: within 32 rows, row 16 u + 4 G + j of the tile is the operand's 8 G + 4 u + j, so
+  // that two tiles hold eight consecutive m of a lane and 32 of its four groups.
+  static GMDN_DEV int row_of(int r) { return PERM ? (r & ~31) | ((r & 12) << 1) | ((r & 16) >> 2) | (r & 3) : r; }
   uint32_t off[NOPS];
   GMDN_DEV void init(const MMOperand& o, int64_t first, int64_t k0) {
     const int l = lane_id(), w = wave_id();
@@ -249,7 +249,7 @@ mm_kernel(MMArgs a, Epi epi) {
 // lane group G, from the workgroup's first.
 template <bool PERM>
 GMDN_DEV int m_of(int i, int G) {
-  return PERM ? (i & ~3) * 16 + 16 * G + 4 * (i & 3) : 16 * i + 4 * G;
+  return PERM ? (i & ~1) * 16 + 8 * G + 4 * (i & 1) : 16 * i + 4 * G;
 }
 
 template <class S, bool ACOL, bool BCOL, bool PERM, class Epi>

@@ -550,6 +550,7 @@ int gmdn_linear_logprobs_fwd(const void* x, const void* weight, const int64_t* t
   if (!x || !weight || !tokens || !logprob || !entropy || !stats) return GMDN_ERR_ARG;
   const Sizes z = sizes_of(x, weight, rows, vocab, d, x_stride, w_stride, dtype);
   if (!workspace || workspace_bytes < z.forward()) return GMDN_ERR_WORKSPACE;
+  if ((uintptr_t)workspace % 16) return GMDN_ERR_ARG;
   const hipStream_t st = (hipStream_t)stream;
   char* at = (char*)workspace;
   const Matrices m = dtype == GMDN_DTYPE_F32 ? matrices_of<float>(x, weight, x_stride, w_stride, z, at, st)
@@ -586,6 +587,7 @@ int gmdn_linear_logprobs_bwd(const void* x, const void* weight, const int64_t* t
   if (!x || !weight || !tokens || !stats || !entropy || (!dx && !dweight)) return GMDN_ERR_ARG;
   const Sizes z = sizes_of(x, weight, rows, vocab, d, x_stride, w_stride, dtype);
   if (!workspace || workspace_bytes < z.backward()) return GMDN_ERR_WORKSPACE;
+  if ((uintptr_t)workspace % 16) return GMDN_ERR_ARG;
   const hipStream_t st = (hipStream_t)stream;
   char* at = (char*)workspace;
   const Matrices m = dtype == GMDN_DTYPE_F32 ? matrices_of<float>(x, weight, x_stride, w_stride, z, at, st)

@@ -194,6 +194,8 @@ class Block(nn.Module):
     called as it is.
     """
 
+    fused = False  # also of a block that was saved whole before there was a choice
+
     def __init__(self, d_model, n_heads, inner, chunk, ns_steps=3, norm="rms", checkpoint=None, residual="torch",
                  post_norm=False, gated=False, layer_scale=None):
         super().__init__()

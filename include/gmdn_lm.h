@@ -63,7 +63,7 @@ int gmdn_layer_norm8_rebuild(const int8_t* q, const float* scale, const void* we
 int gmdn_embed_fwd(const void* weight, const int64_t* tokens, void* y, int64_t rows, int64_t vocab, int64_t d,
                    int64_t w_stride, float scale, int32_t dtype, void* stream);
 
-/* Bytes of the backward's workspace (256-byte aligned). */
+/* Bytes of the backward's workspace (4-byte aligned). */
 size_t gmdn_embed_bwd_workspace_bytes(int64_t rows, int64_t vocab, int64_t d);
 
 /* dweight (vocab, d), every row of it: scale times the sum of the rows of dy whose
@@ -151,7 +151,8 @@ int gmdn_logprobs_bwd(const void* logits, const int64_t* tokens, const float* st
  * logprob, entropy and stats are as above.  bfloat16 operands are multiplied as they
  * are (rows of a multiple of 64 values at 16-byte addresses from where they lie, others
  * from copies in the workspace), float32 ones as three products of bfloat16 pieces,
- * about 2^-16 relative error a product. */
+ * about 2^-16 relative error a product.  The workspace is 16-byte aligned; its size
+ * goes by where x and weight lie, too. */
 size_t gmdn_linear_logprobs_fwd_workspace_bytes(const void* x, const void* weight, int64_t rows, int64_t vocab,
                                                 int64_t d, int64_t x_stride, int64_t w_stride, int32_t dtype);
 int gmdn_linear_logprobs_fwd(const void* x, const void* weight, const int64_t* tokens, float* logprob, float* entropy,

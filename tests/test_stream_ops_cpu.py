@@ -90,7 +90,7 @@ def test_linear_logprobs_argument_checks():
     def fwd_(x=P, w=P, t=P, lp=P, h=P, s=P, ws=P, n=need("fwd"), dims=sizes, dtype=BF16):
         return lib.gmdn_linear_logprobs_fwd(x, w, t, lp, h, s, ws, n, *dims, -100, dtype, None)
 
-    assert fwd_(n=need("fwd") - 1) == 3 and fwd_(ws=None) == 3
+    assert fwd_(n=need("fwd") - 1) == 3 and fwd_(ws=None) == 3 and fwd_(ws=P + 8) == 1
     for name in ("x", "w", "t", "lp", "h", "s"):
         assert fwd_(**{name: None}) == 1, name
     assert fwd_(dims=(-1, 300, 64, 64, 64)) == 1 and fwd_(dims=(100, 0, 64, 64, 64)) == 1
@@ -103,7 +103,7 @@ def test_linear_logprobs_argument_checks():
     def bwd(x=P, w=P, t=P, s=P, h=P, dx=P, dw=P, ws=P, n=need("bwd")):
         return lib.gmdn_linear_logprobs_bwd(x, w, t, s, h, None, None, dx, dw, ws, n, *sizes, -100, BF16, None)
 
-    assert bwd(n=need("bwd") - 1) == 3 and bwd(ws=None) == 3 and bwd(dx=None, dw=None) == 1
+    assert bwd(n=need("bwd") - 1) == 3 and bwd(ws=None) == 3 and bwd(ws=P + 8) == 1 and bwd(dx=None, dw=None) == 1
     for name in ("x", "w", "t", "s", "h"):
         assert bwd(**{name: None}) == 1, name
 
@@ -268,6 +268,7 @@ def test_replaced_and_hooked_norms_are_called():
         assert _ops_of(lambda: block(x)) == ["residual_norm_fwd"] and called == ["n2"]
         block.n2 = nn.LayerNorm(64)
         assert _ops_of(lambda: block(x)) == ["residual_norm_fwd"]
+        assert _ops_of(lambda: _fake_block(checkpoint="int8")(x)) == ["residual_norm_fwd", "gelu8_fwd", "act8_pack"]
         block = _fake_block(post_norm=True)
         assert _ops_of(lambda: block(x)) == ["residual_norm_fwd"] * 2
         block.join1.post.register_forward_hook(lambda *a: called.append("post"))
