@@ -195,9 +195,8 @@ em_scatter(SortInput in, const uint32_t* __restrict__ counts, uint32_t* __restri
 struct Sorted {
   const uint32_t *keys, *at;
   int64_t n, vocab;
-  // first position whose key is not below k
-  GMDN_DEV int64_t lower(uint32_t k) const {
-    int64_t lo = 0, hi = n;
+  // first position in [lo, hi) whose key is not below k (hi without one)
+  GMDN_DEV int64_t lower(uint32_t k, int64_t lo, int64_t hi) const {
     while (lo < hi) {
       const int64_t mid = (lo + hi) >> 1;
       if (keys[mid] < k)
@@ -207,10 +206,27 @@ struct Sorted {
     }
     return lo;
   }
+  // The same over all positions by the two halves of a wave, each for its own k: 32
+  // probes a step, four steps for 16384 positions where a bisection waits for memory
+  // fourteen times.
+  GMDN_DEV int64_t lower_half_wave(uint32_t k) const {
+    const int i = lane_id() & 31, shift = lane_id() & 32;
+    int64_t lo = 0, hi = n;
+    while (__ballot(lo < hi) != 0) {
+      const int64_t step = (hi - lo + 31) / 32, p = lo + i * step;
+      const uint32_t below = (uint32_t)(__ballot(p < hi && keys[p] < k) >> shift);
+      const int c = __popcll(below);  // probes below k: the first c
+      const int64_t next = lo + c * step;
+      lo = c ? next - step + 1 : lo;
+      hi = next < hi ? next : hi;
+    }
+    return lo;
+  }
 };
 
 constexpr int SUM_AHEAD = 8;   // rows of dy in flight
-constexpr int ZERO_ROWS = 64;  // rows of dW that a zeroing workgroup looks after
+constexpr int ZERO_ROWS = 64;  // rows of dW that a zeroing workgroup looks after: a wave's lanes
+constexpr int ZERO_SCAN = 16 * EM_THREADS;  // keys of theirs that it looks at one by one, at most
 
 template <typename T, int TPR>
 __global__ void __launch_bounds__(EM_THREADS)
@@ -220,11 +236,22 @@ em_sums(Sorted s, const T* __restrict__ dy, T* __restrict__ dw, float* __restric
   const int g = threadIdx.x / TPR, t = threadIdx.x % TPR;
   if (blockIdx.x >= sum_groups) {
     __shared__ int absent[ZERO_ROWS];
+    __shared__ int64_t ends[2];
     const int64_t v0 = (int64_t)(blockIdx.x - sum_groups) * ZERO_ROWS;
-    if (threadIdx.x < ZERO_ROWS) {
-      const int64_t v = v0 + threadIdx.x;
-      const int64_t p = v < s.vocab ? s.lower((uint32_t)v) : s.n;
-      absent[threadIdx.x] = v < s.vocab && (p == s.n || s.keys[p] != (uint32_t)v);
+    const int64_t v1 = v0 + ZERO_ROWS < s.vocab ? v0 + ZERO_ROWS : s.vocab;
+    if (threadIdx.x < 64) {  // where the keys of these rows begin and end
+      absent[threadIdx.x] = v0 + threadIdx.x < v1;
+      const int64_t p = s.lower_half_wave((uint32_t)(threadIdx.x < 32 ? v0 : v1));
+      if (threadIdx.x % 32 == 0) ends[threadIdx.x / 32] = p;
+    }
+    __syncthreads();
+    const int64_t lo = ends[0], hi = ends[1];
+    if (hi - lo <= ZERO_SCAN) {
+      for (int64_t p = lo + threadIdx.x; p < hi; p += EM_THREADS) absent[s.keys[p] - v0] = 0;
+    } else if (threadIdx.x < v1 - v0) {
+      const uint32_t v = (uint32_t)(v0 + threadIdx.x);
+      const int64_t p = s.lower(v, lo, hi);
+      if (p < hi && s.keys[p] == v) absent[threadIdx.x] = 0;
     }
     __syncthreads();
     const float zero[8] = {};
@@ -251,15 +278,25 @@ em_sums(Sorted s, const T* __restrict__ dy, T* __restrict__ dw, float* __restric
       store8(dw + (int64_t)cur * d + c, d - c, sum);
     }
   };
-  for (int64_t p = p0; p < p1; p += SUM_AHEAD) {
-    uint32_t key[SUM_AHEAD];
-    Raw8<T> raw[SUM_AHEAD];
+  // the next rows' places are loaded beside these rows
+  uint32_t key[SUM_AHEAD], next_key[SUM_AHEAD], next_at[SUM_AHEAD];
+  auto places = [&](int64_t p) {
 #pragma unroll
     for (int i = 0; i < SUM_AHEAD; ++i) {
       const int64_t q = p + i < p1 ? p + i : p1 - 1;
-      key[i] = s.keys[q];
-      raw[i].load(dy + (int64_t)s.at[q] * ds + c, d - c);
+      next_key[i] = s.keys[q];
+      next_at[i] = s.at[q];
     }
+  };
+  places(p0);
+  for (int64_t p = p0; p < p1; p += SUM_AHEAD) {
+    Raw8<T> raw[SUM_AHEAD];
+#pragma unroll
+    for (int i = 0; i < SUM_AHEAD; ++i) {
+      raw[i].load(dy + (int64_t)next_at[i] * ds + c, d - c);
+      key[i] = next_key[i];
+    }
+    places(p + SUM_AHEAD);
 #pragma unroll
     for (int i = 0; i < SUM_AHEAD; ++i) {
       if (p + i >= p1) break;
@@ -287,10 +324,23 @@ em_join(Sorted s, const float* __restrict__ part, T* __restrict__ dw, int64_t bl
   const int64_t b = (int64_t)blockIdx.x * GROUPS + threadIdx.x / TPR;
   const int64_t p0 = b * block, p1 = p0 + block;
   const int c = 8 * (blockIdx.y * TPR + threadIdx.x % TPR);
-  if (p1 >= s.n || c >= d) return;
+  if (p1 >= s.n) return;
   const uint32_t k = s.keys[p1];
   if (k >= s.vocab || s.keys[p1 - 1] != k || (p0 > 0 && s.keys[p0] == k && s.keys[p0 - 1] == k)) return;
-  const int64_t last = (s.lower(k + 1) - 1) / block;
+  // The block where the run ends: the first whose successor begins with another
+  // token.  Each lane of the group looks at one (a group's lanes are here together).
+  constexpr int LANES = TPR < 64 ? TPR : 64;
+  const int i = lane_id() % LANES, shift = lane_id() - i;
+  int64_t last = b + 1;
+  for (;; last += LANES) {
+    const int64_t q = (last + i + 1) * block;
+    const uint64_t ends = __ballot(q >= s.n || s.keys[q] != k) >> shift & (~0ull >> (64 - LANES));
+    if (ends) {
+      last += __builtin_ctzll(ends);
+      break;
+    }
+  }
+  if (c >= d) return;
   float sum[8];
   load8(part + (2 * b + 1) * d + c, d - c, sum);
   for (int64_t i = b + 1; i <= last; i += SUM_AHEAD) {
