@@ -200,36 +200,44 @@ struct GradEpi {
         const int64_t from = t - e.first - m0;
         token = from >= 0 && from < S::TM ? (int)from : -1;
       }
+      // a row without a gradient has zeros, whatever its logits are
       const bool none = (gl == 0.f && gh == 0.f) || m == -INFINITY;
+      const uint32_t keep = none ? 0u : ~0u;
       bf16* const to = e.d + row * e.columns + m0;
+      // p as the square of x = e^(log p / 2): the exponential flushes results below 2^-126
+      auto columns = [&](auto&& term) {
 #pragma unroll
-      for (int i = 0; i < S::MT; i += 2) {
-        const int c = m_of<PERM>(wm * S::MT + i, G);
-        float g[8];
+        for (int i = 0; i < S::MT; i += 2) {
+          const int c = m_of<PERM>(wm * S::MT + i, G);
+          float g[8];
 #pragma unroll
-        for (int q = 0; q < 8; ++q) {
-          // p as the square of e^(log p / 2): the exponential flushes results below 2^-126
-          const float u = acc[i + q / 4][j][q % 4] - m - logs, x = __builtin_amdgcn_exp2f(u * HALF_LOG2E);
-          const float f = e.dent ? gl + gh * (fmaxf(u, FAR) + h) : gl;
-          g[q] = none ? 0.f : -x * (x * f);
+          for (int q = 0; q < 8; ++q) {
+            const float u = acc[i + q / 4][j][q % 4] - m - logs;
+            g[q] = term(u, __builtin_amdgcn_exp2f(u * HALF_LOG2E));
+          }
+          if (token >= 0)
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+              if (c + q == token) g[q] += gl;
+          if (left < S::TM)  // the vocabulary ends in this tile
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+              if (c + q >= left) g[q] = 0.f;
+          bf16* o = to + c;
+#pragma unroll
+          for (int p = 0; p < P; ++p, o += e.padded * e.columns) {
+            const bf16x8 b = cat8(to_bf16x4(f32x4{g[0], g[1], g[2], g[3]}), to_bf16x4(f32x4{g[4], g[5], g[6], g[7]}));
+            *reinterpret_cast<u32x4*>(o) = __builtin_bit_cast(u32x4, b) & keep;
+            if (p + 1 < P)
+#pragma unroll
+              for (int q = 0; q < 8; ++q) g[q] -= (float)b[q];
+          }
         }
-        if (token >= 0 && !none)
-#pragma unroll
-          for (int q = 0; q < 8; ++q)
-            if (c + q == token) g[q] += gl;
-        if (left < S::TM)  // the vocabulary ends in this tile
-#pragma unroll
-          for (int q = 0; q < 8; ++q)
-            if (c + q >= left) g[q] = 0.f;
-        bf16* o = to + c;
-#pragma unroll
-        for (int p = 0; p < P; ++p, o += e.padded * e.columns) {
-          const bf16x8 b = cat8(to_bf16x4(f32x4{g[0], g[1], g[2], g[3]}), to_bf16x4(f32x4{g[4], g[5], g[6], g[7]}));
-          *reinterpret_cast<bf16x8*>(o) = b;
-#pragma unroll
-          for (int q = 0; q < 8; ++q) g[q] -= (float)b[q];
-        }
-      }
+      };
+      if (e.dent)
+        columns([&](float u, float x) { return -x * (x * (gl + gh * (fmaxf(u, FAR) + h))); });
+      else
+        columns([&](float, float x) { return -x * (x * gl); });
     }
   }
 };

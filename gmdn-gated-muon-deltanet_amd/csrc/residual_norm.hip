@@ -12,6 +12,9 @@
 //   dg = dx s n u (1 - u)
 //   dw = sum dz rh,  dp = sum dn yh,  ds = sum dx u n     over the rows
 //
+// The backward forms r again from x and y, unrounded; with a float32 stream and nothing
+// but the sum it reads the kept r instead.
+//
 // Memory bound: about 60 operations a value against 16 to 26 bytes.  As in the
 // layer norm a row stays in its threads' registers between the sums and the
 // outputs, so each matrix is read and written once, and the weights' sums stay
@@ -165,12 +168,20 @@ rn_fwd(const TX* __restrict__ x, int64_t xs, Branch<TY> in, Vectors vec, TX* __r
   }
 }
 
-// A backward call's matrices.  dr, dz and dy may be null: zeros, and not wanted.
+// Whether the backward reads r: where it was kept in full and nothing else wants y.  It
+// forms r again from x and the branch otherwise: a bfloat16 r would put its rounding,
+// 2^-8 of a value, into the vectors' float32 gradients (2e-3 of their norm; from x and y
+// 1e-7), and x costs no more to read.
+template <typename TX>
+constexpr bool rn_from_r(Parts p) { return p == ADD && sizeof(TX) == 4; }
+
+// A backward call's matrices: stream is r or x.  dr, dz and dy may be null: zeros, and
+// not wanted.
 template <typename TX, typename TY>
 struct Grads {
-  const TX *dr, *r;
+  const TX *dr, *stream;
   const TY* dz;
-  int64_t drs, rs, dzs;
+  int64_t drs, ss, dzs;
   TX* dx;
   TY *dy, *dg;
 };
@@ -185,6 +196,8 @@ rn_bwd(Grads<TX, TY> gr, Branch<TY> in, Vectors vec, const float* __restrict__ r
        const float* __restrict__ post_rstd, float* __restrict__ part, int64_t rows, int d) {
   constexpr int RPB = rn_threads(TPR) / TPR;
   constexpr int NP = P == ADD ? 1 : NV, NG = P == GATED ? NV : 1, SUMS = P == ADD ? 1 : 3;
+  constexpr bool FROM_R = rn_from_r<TX>(P);
+  constexpr int NY = FROM_R ? 1 : NV;
   __shared__ float red[2][16];
   const int lr = threadIdx.x / TPR, t = threadIdx.x % TPR;
   int slot = 0;
@@ -209,8 +222,8 @@ rn_bwd(Grads<TX, TY> gr, Branch<TY> in, Vectors vec, const float* __restrict__ r
       store8(lds + 16 * TPR + c, 8, sv[i]);
     }
   }
-  Raw8<TX> ar[NV], rr[NV];  // dr, r
-  Raw8<TY> zr[NV], yr[NP], cr[NG];  // dz, y, gate
+  Raw8<TX> ar[NV], xr[NV];  // dr, r or x
+  Raw8<TY> zr[NV], yr[NY], cr[NG];  // dz, y, gate
   float tau1, rho1;
   auto fetch = [&](int64_t r) {
     const bool live = r < rows;
@@ -219,10 +232,10 @@ rn_bwd(Grads<TX, TY> gr, Branch<TY> in, Vectors vec, const float* __restrict__ r
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = 8 * (i * TPR + t), left = live ? d - c : 0;
-      rr[i].load(gr.r + r * gr.rs + c, left);
+      xr[i].load(gr.stream + r * gr.ss + c, left);
       ar[i].load(gr.dr + r * gr.drs + c, gr.dr ? left : 0);
       zr[i].load(gr.dz + r * gr.dzs + c, gr.dz ? left : 0);
-      if constexpr (P != ADD) yr[i].load(in.y + r * in.ys + c, left);
+      if constexpr (!FROM_R) yr[i].load(in.y + r * in.ys + c, left);
       if constexpr (P == GATED && !IN_LDS) cr[i].load(in.g + r * in.gs + c, left);
     }
   };
@@ -237,21 +250,40 @@ rn_bwd(Grads<TX, TY> gr, Branch<TY> in, Vectors vec, const float* __restrict__ r
     const float tau = tau1, rho = rho1;
     if constexpr (P == GATED && IN_LDS) cr[0].load(in.g + r * in.gs + 8 * t, live ? d - 8 * t : 0);
     if constexpr (IN_LDS) load8(lds + 8 * t, 8, wv[0]);
-    float h[NV][8], g[NV][8], a[NV][8], y[NP][8], u[NG][8];
+    float h[NV][8], g[NV][8], a[NV][8], y[NY][8], u[NG][8];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      rr[i].get(h[i]);
+      xr[i].get(h[i]);
       zr[i].get(g[i]);
       ar[i].get(a[i]);
-      if constexpr (P != ADD) yr[i].get(y[i]);
+      if constexpr (!FROM_R) yr[i].get(y[i]);
       if constexpr (P == GATED) cr[i].get(u[i]);
     }
     if constexpr (AHEAD) fetch(r + step);
+    // the vectors of the thread's piece again, where they are in LDS
+    auto vectors = [&](int i, int j) {
+      if constexpr (IN_LDS) {
+        pv[i][j] = lds[8 * TPR + 8 * t + j];
+        sv[i][j] = lds[16 * TPR + 8 * t + j];
+      }
+    };
     float s0 = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
+        if constexpr (P != ADD) {
+          vectors(i, j);
+          y[i][j] *= rho;  // yh
+          float n = y[i][j] * pv[i][j] * sv[i][j];
+          if constexpr (P == GATED) {
+            u[i][j] = sigmoid(u[i][j]);
+            n *= u[i][j];
+          }
+          h[i][j] += n;
+        } else if constexpr (!FROM_R) {
+          h[i][j] += y[i][j];
+        }
         h[i][j] *= tau;  // rh
         dw[i][j] += g[i][j] * h[i][j];
         g[i][j] *= wv[i][j];
@@ -271,14 +303,10 @@ rn_bwd(Grads<TX, TY> gr, Branch<TY> in, Vectors vec, const float* __restrict__ r
       } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          if constexpr (IN_LDS) {
-            pv[i][j] = lds[8 * TPR + c + j];
-            sv[i][j] = lds[16 * TPR + c + j];
-          }
-          y[i][j] *= rho;  // yh
+          vectors(i, j);
           const float n = y[i][j] * pv[i][j];
           if constexpr (P == GATED) {
-            const float q = sigmoid(u[i][j]);
+            const float q = u[i][j];
             u[i][j] = a[i][j] * sv[i][j] * n * q * (1.f - q);  // dg
             a[i][j] *= q;
           }
@@ -498,21 +526,22 @@ size_t gmdn_residual_norm_bwd_workspace_floats(int64_t rows, int64_t d) {
   return (size_t)(add > full ? add : full);
 }
 
-int gmdn_residual_norm_bwd(const void* dr, const void* dz, const void* r, const void* y, const void* weight,
+int gmdn_residual_norm_bwd(const void* dr, const void* dz, const void* r_or_x, const void* y, const void* weight,
                            const void* post_weight, const void* gate, const void* scale, const float* rstd,
                            const float* post_rstd, void* dx, void* dy, void* dgate, void* dweight, void* dpost_weight,
                            void* dscale, float* workspace, size_t workspace_floats, int64_t rows, int64_t d,
-                           int64_t dr_stride, int64_t dz_stride, int64_t r_stride, int64_t y_stride,
+                           int64_t dr_stride, int64_t dz_stride, int64_t r_or_x_stride, int64_t y_stride,
                            int64_t gate_stride, int32_t x_type, int32_t y_type, int32_t w_type, void* stream) {
   const int rc = check_dims(rows, d);
   if (rc != GMDN_OK) return rc;
   if (!pair_ok(x_type, y_type) || !type_ok(w_type)) return GMDN_ERR_UNSUPPORTED;
-  if (dr_stride < 0 || dz_stride < 0 || r_stride < 0 || y_stride < 0 || gate_stride < 0) return GMDN_ERR_ARG;
+  if (dr_stride < 0 || dz_stride < 0 || r_or_x_stride < 0 || y_stride < 0 || gate_stride < 0) return GMDN_ERR_ARG;
   const bool plain = !post_weight && !gate && !scale;
   const bool wants = dweight || dpost_weight || dscale;
   if ((dweight && !weight) || (dpost_weight && !post_weight) || (dscale && !scale)) return GMDN_ERR_ARG;
   if (rows > 0) {
-    if (!r || !rstd || !dx || (!plain && (!y || !dy)) || (gate && !dgate) || (post_weight && !post_rstd))
+    const bool from_r = plain && x_type == GMDN_DTYPE_F32;
+    if (!r_or_x || !rstd || !dx || (!from_r && !y) || (!plain && !dy) || (gate && !dgate) || (post_weight && !post_rstd))
       return GMDN_ERR_ARG;
     if (plain && !dy && x_type != y_type) return GMDN_ERR_ARG;
   }
@@ -527,7 +556,7 @@ int gmdn_residual_norm_bwd(const void* dr, const void* dz, const void* r, const 
       using TX = decltype(tx);
       using TY = decltype(ty);
       const Branch<TY> in{(const TY*)y, (const TY*)gate, y_stride, gate_stride};
-      const Grads<TX, TY> g{(const TX*)dr, (const TX*)r, (const TY*)dz, dr_stride, r_stride, dz_stride,
+      const Grads<TX, TY> g{(const TX*)dr, (const TX*)r_or_x, (const TY*)dz, dr_stride, r_or_x_stride, dz_stride,
                             (TX*)dx, (TY*)dy, (TY*)dgate};
       with_parts(post_weight, gate, scale, [&](auto w) {
         constexpr Parts P = decltype(w)::P;

@@ -100,32 +100,37 @@ Residual residual_norm_fwd(const Tensor& x, const Tensor& y, const OptTensor& we
   return {out, z, rstd, post_rstd};
 }
 
+// Whether the backward reads the stream that the forward returned, r, and not y:
+// a float32 one with nothing but the sum.
+bool from_r(const Tensor& x, bool plain) { return plain && x.scalar_type() == at::kFloat; }
+
 using Grads6 = std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor>;
-Grads6 residual_norm_bwd(const OptTensor& dr, const OptTensor& dz, const Tensor& r, const Tensor& y,
+Grads6 residual_norm_bwd(const OptTensor& dr, const OptTensor& dz, const Tensor& r_or_x, const Tensor& y,
                          const OptTensor& weight, const OptTensor& post_weight, const OptTensor& gate,
                          const OptTensor& scale, const Tensor& rstd_, const Tensor& post_rstd_) {
-  const c10::DeviceGuard guard(r.device());
-  const ScalarType xt = r.scalar_type(), yt = y.scalar_type();
-  const int32_t xc = type_code(xt, "r"), yc = type_code(yt, "y");
-  const Rows rr = rows_of(r, "r"), a = branch_of(dr, r, xt, "dr"), z = branch_of(dz, r, yt, "dz"),
-             b = branch_of(y, r, yt, "y"), g = branch_of(gate, r, yt, "gate");
-  const Vectors v = vectors_of(weight, post_weight, scale, r, rr.d);
-  const Tensor rstd = stat(rstd_, r, lead(r), "rstd"), post = v.p ? stat(post_rstd_, r, lead(r), "post_rstd") : Tensor();
+  const c10::DeviceGuard guard(r_or_x.device());
+  const Tensor& x = r_or_x;
+  const ScalarType xt = x.scalar_type(), yt = y.scalar_type();
+  const int32_t xc = type_code(xt, "the stream"), yc = type_code(yt, "y");
+  const Rows r = rows_of(x, "the stream"), a = branch_of(dr, x, xt, "dr"), z = branch_of(dz, x, yt, "dz"),
+             b = branch_of(y, x, yt, "y"), g = branch_of(gate, x, yt, "gate");
+  const Vectors v = vectors_of(weight, post_weight, scale, x, r.d);
+  const Tensor rstd = stat(rstd_, x, lead(x), "rstd"), post = v.p ? stat(post_rstd_, x, lead(x), "post_rstd") : Tensor();
   const bool same = !v.p && !v.s && !gate && xt == yt;  // dy is dx
-  Tensor dx = fresh(r, r.sizes(), xt), dy = same ? none_like(r, yt) : fresh(r, r.sizes(), yt);
-  Tensor dg = gate ? fresh(r, r.sizes(), yt) : none_like(r, yt);
-  auto grad = [&](const OptTensor& t) { return t ? at::empty_like(*t) : fresh(r, {0}); };
+  Tensor dx = fresh(x, x.sizes(), xt), dy = same ? none_like(x, yt) : fresh(x, x.sizes(), yt);
+  Tensor dg = gate ? fresh(x, x.sizes(), yt) : none_like(x, yt);
+  auto grad = [&](const OptTensor& t) { return t ? at::empty_like(*t) : fresh(x, {0}); };
   Tensor dw = grad(v.w), dp = grad(v.p), ds = grad(v.s);
   const bool vectors = v.w || v.p || v.s;
-  const size_t need = vectors ? gmdn_residual_norm_bwd_workspace_floats(rr.rows, rr.d) : 0;
-  const Tensor ws = need ? fresh(r, {(int64_t)need}) : Tensor();
-  if (rr.rows || vectors)
-    check(gmdn_residual_norm_bwd(ptr(a), ptr(z), rr.ptr(), b.ptr(), ptr(v.w), ptr(v.p), ptr(g), ptr(v.s), fp(rstd),
+  const size_t need = vectors ? gmdn_residual_norm_bwd_workspace_floats(r.rows, r.d) : 0;
+  const Tensor ws = need ? fresh(x, {(int64_t)need}) : Tensor();
+  if (r.rows || vectors)
+    check(gmdn_residual_norm_bwd(ptr(a), ptr(z), r.ptr(), b.ptr(), ptr(v.w), ptr(v.p), ptr(g), ptr(v.s), fp(rstd),
                                  v.p ? fp(post) : nullptr, dx.data_ptr(), same ? nullptr : dy.data_ptr(),
                                  gate ? dg.data_ptr() : nullptr, v.w ? dw.data_ptr() : nullptr,
                                  v.p ? dp.data_ptr() : nullptr, v.s ? ds.data_ptr() : nullptr, need ? fp(ws) : nullptr,
-                                 need, rr.rows, rr.d, a.stride, z.stride, rr.stride, b.stride, g.stride, xc, yc, v.code,
-                                 stream_of(r)),
+                                 need, r.rows, r.d, a.stride, z.stride, r.stride, b.stride, g.stride, xc, yc, v.code,
+                                 stream_of(x)),
           "gmdn_residual_norm_bwd");
   return {dx, dy, dw, dp, dg, ds};
 }
@@ -222,9 +227,10 @@ struct ResidualNormFwd : torch::autograd::Function<ResidualNormFwd> {
         GMDN_OP(residual_norm_fwd).call(x, y, weight, post_weight, gate, scale, eps);
     *rest = {rstd, post_rstd};
     ctx->set_materialize_grads(false);
-    // without a post norm, a gate and a scale the backward reads y's type only
-    const bool plain = !post_weight && !gate && !scale;
-    ctx->save_for_backward({r, plain ? z : y, opt(weight), opt(post_weight), opt(gate), opt(scale), rstd, post_rstd});
+    // z in y's place: of its type and shape, and not read
+    const bool after = from_r(x, !post_weight && !gate && !scale);
+    ctx->save_for_backward({after ? r : x, after ? z : y, opt(weight), opt(post_weight), opt(gate), opt(scale), rstd,
+                            post_rstd});
     return {r, z};
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& g) {
@@ -303,7 +309,7 @@ TORCH_LIBRARY_FRAGMENT(gmdn, m) {
   m.def("embed_bwd(Tensor dy, Tensor tokens, SymInt vocab, float scale, SymInt padding_idx) -> Tensor", PT2);
   m.def("residual_norm_fwd(Tensor x, Tensor y, Tensor? weight, Tensor? post_weight, Tensor? gate, Tensor? scale, "
         "float eps) -> (Tensor, Tensor, Tensor, Tensor)", PT2);
-  m.def("residual_norm_bwd(Tensor? dr, Tensor? dz, Tensor r, Tensor y, Tensor? weight, Tensor? post_weight, "
+  m.def("residual_norm_bwd(Tensor? dr, Tensor? dz, Tensor r_or_x, Tensor y, Tensor? weight, Tensor? post_weight, "
         "Tensor? gate, Tensor? scale, Tensor rstd, Tensor post_rstd) -> (Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)",
         PT2);
   m.def("linear_logprobs_fwd(Tensor x, Tensor weight, Tensor tokens, SymInt ignore_index) -> (Tensor, Tensor, Tensor)",

@@ -45,11 +45,12 @@ its model, train_ablation.py:420-422):
   ``gmdn::embed_bwd(dy, tokens, vocab, scale, padding_idx) -> dweight`` -- token
   embedding (gmdn_amd.embedding).
 * ``gmdn::residual_norm_fwd(x, y, weight, post_weight, gate, scale, eps) -> (r,
-  z, rstd, post_rstd)`` and ``gmdn::residual_norm_bwd(dr, dz, r, y, weight,
+  z, rstd, post_rstd)`` and ``gmdn::residual_norm_bwd(dr, dz, r_or_x, y, weight,
   post_weight, gate, scale, rstd, post_rstd) -> (dx, dy, dweight, dpost_weight,
   dgate, dscale)`` -- a branch's way back into the residual stream and the norm
-  that follows; gradients of what is absent are empty, and ``dy`` where it is
-  ``dx`` (gmdn_amd.residual).
+  that follows.  The backward takes ``x``; of a float32 stream without post norm,
+  gate and scale it takes ``r``, and of ``y`` the type only.  Gradients of what is
+  absent are empty, and ``dy`` where it is ``dx`` (gmdn_amd.residual).
 * ``gmdn::linear_logprobs_fwd(x, weight, tokens, ignore_index) -> (logprob,
   entropy, stats)`` and ``gmdn::linear_logprobs_bwd(x, weight, tokens, stats,
   entropy, dlogprob, dentropy, ignore_index, need_x, need_weight) -> (dx,
@@ -270,11 +271,11 @@ def _residual_norm_fwd_fake(x, y, weight, post_weight, gate, scale, eps):
             x.new_empty(lead if post_weight is not None else (0,), dtype=torch.float32))
 
 
-def _residual_norm_bwd_fake(dr, dz, r, y, weight, post_weight, gate, scale, rstd, post_rstd):
-    same = post_weight is None and gate is None and scale is None and r.dtype == y.dtype
-    dw, dp, ds = (v.new_empty(v.shape) if v is not None else _empty(r) for v in (weight, post_weight, scale))
-    return (r.new_empty(r.shape), y.new_empty((0,) if same else r.shape), dw, dp,
-            y.new_empty(r.shape if gate is not None else (0,)), ds)
+def _residual_norm_bwd_fake(dr, dz, r_or_x, y, weight, post_weight, gate, scale, rstd, post_rstd):
+    same = post_weight is None and gate is None and scale is None and r_or_x.dtype == y.dtype
+    dw, dp, ds = (v.new_empty(v.shape) if v is not None else _empty(r_or_x) for v in (weight, post_weight, scale))
+    return (r_or_x.new_empty(r_or_x.shape), y.new_empty((0,) if same else r_or_x.shape), dw, dp,
+            y.new_empty(r_or_x.shape if gate is not None else (0,)), ds)
 
 
 def _linear_logprobs_fwd_fake(x, weight, tokens, ignore_index):

@@ -31,8 +31,9 @@ def residual_norm(x: Tensor, y: Tensor, weight: Tensor | None = None, *, post_we
 
     ``x``, ``y``: (..., D) of one shape and type, bfloat16 or float32, or a float32
     stream beside a bfloat16 branch; D up to 8192.  ``gate``: logits, as ``y``.  ``weight``,
-    ``post_weight``, ``scale``: (D,), of one type.  Sums are float32; ``z`` is
-    computed from ``r`` before ``r`` is rounded, and the backward from the rounded one.
+    ``post_weight``, ``scale``: (D,), of one type.  Sums are float32; ``z``, and the
+    gradients, are computed from ``r`` before it is rounded.  Kept for the backward are ``x``,
+    ``y`` and the gate, or for a float32 stream with none of the three parts ``r`` alone.
     """
     ops.ensure()
     r, z, _, _ = torch.ops.gmdn.residual_norm_fwd(x, y, weight, post_weight, gate, scale, eps)

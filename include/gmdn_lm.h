@@ -91,13 +91,14 @@ int gmdn_residual_norm_fwd(const void* x, const void* y, const void* weight, con
 size_t gmdn_residual_norm_bwd_workspace_floats(int64_t rows, int64_t d);
 
 /* The gradients from dr and dz (either may be NULL: zeros) and what the forward
- * kept.  dy may be NULL where it would be dx: no post norm, gate or scale, and
- * one type.  dweight, dpost_weight and dscale may be NULL each. */
-int gmdn_residual_norm_bwd(const void* dr, const void* dz, const void* r, const void* y, const void* weight,
+ * read and kept.  r_or_x is x -- but r, and y may be NULL, for a float32 stream without
+ * post norm, gate and scale.  dy may be NULL where it would be dx: none of the three,
+ * and one type.  dweight, dpost_weight and dscale may be NULL each. */
+int gmdn_residual_norm_bwd(const void* dr, const void* dz, const void* r_or_x, const void* y, const void* weight,
                            const void* post_weight, const void* gate, const void* scale, const float* rstd,
                            const float* post_rstd, void* dx, void* dy, void* dgate, void* dweight, void* dpost_weight,
                            void* dscale, float* workspace, size_t workspace_floats, int64_t rows, int64_t d,
-                           int64_t dr_stride, int64_t dz_stride, int64_t r_stride, int64_t y_stride,
+                           int64_t dr_stride, int64_t dz_stride, int64_t r_or_x_stride, int64_t y_stride,
                            int64_t gate_stride, int32_t x_type, int32_t y_type, int32_t w_type, void* stream);
 
 /* ------------------------------------------------------- 8-bit checkpoints */

@@ -4,11 +4,9 @@ forward and backward, against the formulas in float64.
 Bounds, with u = 2^-24.  A sum over a row passes through at most 16 additions in a
 thread and ten joining ones: 32 u of its sum of magnitudes; the inverse root, the
 logistic function (its argument within 2 u |g|, |g| below 8 here) and the products
-that follow stay within ROW = 64 u of each value.  r adds one rounding.  z and the
-gradients see r's error through the norm.  The backward runs from the rounded r
-that was kept, beside the unrounded one's norm: so does the reference.  A vector's
-gradient adds up to rows / 1024 + 64 products in sequence.  An output adds half a step
-of its type."""
+that follow stay within ROW = 64 u of each value.  z and the gradients see the
+unrounded r's error through the norm.  A vector's gradient adds up to rows / 1024 + 64
+products in sequence.  An output adds half a step of its type."""
 import pytest
 import torch
 
@@ -67,22 +65,22 @@ def _forward(v, eps):
     w = v["weight"].double() if v["weight"] is not None else torch.ones_like(y)
     z = r * tau * w
     tol_z = (w * tau).abs() * tol + z.abs() * (ROW + tau * tol.amax(-1, keepdim=True))
-    return (r, tol), (z, tol_z), (yh, rho, n, u, s, w, tau)
+    th = tau * tol + z.abs() / w.abs() * (ROW + tau * tol.amax(-1, keepdim=True))  # of r tau
+    return (r, tol), (z, tol_z), (yh, rho, n, u, s, w, tau, r * tau, th)
 
 
-def _backward(v, r_kept, dr, dz, state):
-    yh, rho, n, u, s, w, tau = state
-    rh = r_kept.double() * tau
+def _backward(v, dr, dz, state):
+    yh, rho, n, u, s, w, tau, rh, th = state
     dr, dz = dr.double(), dz.double()
     g = w * dz
-    G = g.abs().amax(-1, keepdim=True)
+    G, H = g.abs().amax(-1, keepdim=True), th.amax(-1, keepdim=True)
     dx = dr + tau * (g - rh * (g * rh).mean(-1, keepdim=True))
-    tx = 2 * U * dr.abs() + tau * G * (8 * ROW * (1 + rh.abs() + rh * rh))
+    tx = 2 * U * dr.abs() + tau * G * (8 * ROW * (1 + rh.abs() + rh * rh) + 3 * H * (1 + rh.abs()))
     dn = dx * s * u
     tn = tx * (s * u).abs() + ROW * dn.abs()
     out = {"x": (dx, tx), "y": (dn, tn)}
     seq = (dx.shape[0] / 1024 + 64) * U
-    out["weight"] = ((dz * rh).sum(0), ((seq + 2 * ROW) * (dz * rh).abs()).sum(0))
+    out["weight"] = ((dz * rh).sum(0), (dz.abs() * (th + (seq + 2 * ROW) * rh.abs())).sum(0))
     if rho is not None:
         p = v["post_weight"].double()
         q, tq = p * dn, p.abs() * tn + U * (p * dn).abs()
@@ -120,7 +118,7 @@ def _run(rows, d, x_dtype, y_dtype, parts, seed, w_dtype=F, weight=True, use=(Tr
     cots = [place(t) for t, on in zip((dr, dz), use) if on]
     grads = dict(zip(leaf, torch.autograd.grad(outs, list(leaf.values()), cots, allow_unused=True)))
     dr, dz = (t if on else torch.zeros_like(t) for t, on in zip((dr, dz), use))
-    ref = _backward(v, got_r.detach().cpu(), dr, dz, state)
+    ref = _backward(v, dr, dz, state)
     for name, g in grads.items():
         assert g.dtype == leaf[name].dtype and g.shape == leaf[name].shape
         _close(g, *ref[name], "d" + name)

@@ -65,6 +65,7 @@ def test_residual_argument_checks():
     assert bwd(ws=None) == 3 and bwd(n=1023) == 3
     assert bwd(r=None) == 1 and bwd(rs=None) == 1 and bwd(dx=None) == 1
     assert bwd(dy=None, xt=F32) == 1          # another type than dx's
+    assert bwd(y=None) == 1                   # a bfloat16 r is formed again
     assert bwd(s=P, dy=None) == 1 and bwd(s=P, y=None) == 1
     assert bwd(g=P) == 1                      # the gate's gradient
     assert bwd(p=P) == 1                      # the post norm's statistic
