@@ -185,7 +185,10 @@ def _run_own(s):
         r, z, rstd, post_rstd = op.residual_norm_fwd(s["x"], s["y"], *parts, s["eps"])
         if not train:
             return {"r": r, "z": z}
-        dx, dy, dw, dpost, dgate, dscale = op.residual_norm_bwd(s["dr"], s["dz"], r, s["y"], *parts, rstd, post_rstd)
+        # the backward takes x, but of a float32 stream with nothing but the sum r
+        plain = s["post"] is None and s["gate"] is None and s["scale"] is None
+        stream = r if plain and r.dtype == torch.float32 else s["x"]
+        dx, dy, dw, dpost, dgate, dscale = op.residual_norm_bwd(s["dr"], s["dz"], stream, s["y"], *parts, rstd, post_rstd)
         out = {"r": r, "z": z, "dx": dx, "dy": dy if dy.numel() else dx, "dweight": dw}
         if s["post"] is not None:
             out.update(dpost=dpost, dscale=dscale)
