@@ -33,20 +33,28 @@ constexpr int KPAD = 64;                  // k in planes: a multiple, zeros behi
 constexpr float HALF_LOG2E = 0.5f * LOG2E;
 
 // ------------------------------------------------------------------ planes
-// (rows, d) as P planes (rows, kp) of bfloat16 pieces, zeros behind d.
+// (rows, d) matrices as P planes (rows, kp) of bfloat16 pieces, zeros behind d: one
+// matrix for each y of the grid.
+template <typename T>
+struct Whole {
+  const T* x;
+  int64_t stride, rows;
+  bf16* out;
+};
 template <typename T, int P>
 __global__ void __launch_bounds__(256)
-ll_planes(const T* __restrict__ x, int64_t stride, bf16* __restrict__ out, int64_t rows, int d, int kp) {
+ll_planes(Whole<T> a, Whole<T> b, int d, int kp) {
+  const Whole<T>& m = blockIdx.y == 0 ? a : b;
   const int per = kp / 8;
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   const int64_t r = i / per;
-  if (r >= rows) return;
+  if (r >= m.rows) return;
   const int c = 8 * (int)(i - r * per);
   float v[8];
-  load8(x + r * stride + c, d - c, v);
-  bf16* o = out + r * kp + c;
+  load8(m.x + r * m.stride + c, d - c, v);
+  bf16* o = m.out + r * kp + c;
 #pragma unroll
-  for (int p = 0; p < P; ++p, o += rows * kp) {
+  for (int p = 0; p < P; ++p, o += m.rows * kp) {
     bf16x8 h;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -345,11 +353,11 @@ bool in_place(const void* p, int64_t stride, int64_t d, int32_t dtype) {
 struct Product {
   int edge, per, splits;
 };
-// A product of few tiles is split until the chip is filled, while a part keeps four
-// stages or more.
-int splits_of(int64_t tiles, int64_t steps) {
+// A product of few tiles is split until the chip is filled, while a part keeps sixteen
+// turns of the loop or more: joining the parts is a launch more.
+int splits_of(int64_t tiles, int64_t turns) {
   int64_t s = 256 / tiles;
-  if (s > steps / 4) s = steps / 4;
+  if (s > turns / 16) s = turns / 16;
   return (int)(s < 1 ? 1 : s > 64 ? 64 : s);
 }
 // The tile of the least cost: rounds over the 256 CUs, times a tile's work at the rate that its
@@ -362,7 +370,7 @@ Product product_of(int64_t M, int64_t N, int64_t steps, int pairs, bool split) {
   const int edges[3] = {64, 128, 256}, clocks[3] = {6, 3, 2};
   for (int i = 0; i < 3; ++i) {
     const int64_t e = edges[i], tiles = div_up(M, e) * div_up(N, e);
-    Product p{edges[i], (int)div_up(steps, split ? splits_of(tiles, steps) : 1), 1};
+    Product p{edges[i], (int)div_up(steps, split ? splits_of(tiles, steps * pairs) : 1), 1};
     p.splits = (int)div_up(steps, p.per);
     const double cost = (double)div_up(tiles * p.splits, 256) * (double)(e * e) * (p.per * pairs + 2) * clocks[i];
     if (i == 0 || cost < least) {
@@ -437,18 +445,6 @@ int check_ll(int64_t rows, int64_t V, int64_t d, int64_t xs, int64_t ws, int32_t
   return fits ? GMDN_OK : GMDN_ERR_UNSUPPORTED;
 }
 
-// An operand's planes: where it lies, or made at `at`, which moves on.
-template <typename T>
-const bf16* planes_of(const T* x, int64_t stride, int64_t rows, const Sizes& z, bool in, size_t bytes, char*& at,
-                      hipStream_t st) {
-  if (in) return (const bf16*)x;
-  bf16* const out = (bf16*)at;
-  at += bytes;
-  hipLaunchKernelGGL((ll_planes<T, std::is_same_v<T, float> ? 2 : 1>), dim3((unsigned)div_up(rows * (z.kp / 8), 256)),
-                     dim3(256), 0, st, x, stride, out, rows, (int)z.d, (int)z.kp);
-  return out;
-}
-
 // A product's arguments; the pairs of planes with the small terms first: lo hi, hi lo, hi hi.
 template <class S>
 MMArgs args_of(const MMOperand& a, const MMOperand& b, int64_t M, int64_t N, int64_t k, int pairs, int per) {
@@ -470,15 +466,30 @@ struct Matrices {
   const bf16 *x, *w;
   int64_t xs, ws, xp, wp;  // row strides, plane strides
 };
+// The operands' planes: where they lie, or made at `at`, which moves on.
 template <typename T>
 Matrices matrices_of(const void* x, const void* w, int64_t xs, int64_t ws, const Sizes& z, char*& at, hipStream_t st) {
-  Matrices m;
-  m.x = planes_of((const T*)x, xs, z.rows, z, z.x_in, z.x, at, st);
-  m.w = planes_of((const T*)w, ws, z.V, z, z.w_in, z.w, at, st);
-  m.xs = z.x_in ? xs : z.kp;
-  m.ws = z.w_in ? ws : z.kp;
-  m.xp = z.rows * z.kp;
-  m.wp = z.V * z.kp;
+  Matrices m{(const bf16*)x, (const bf16*)w, xs, ws, z.rows * z.kp, z.V * z.kp};
+  Whole<T> list[2];
+  int n = 0;
+  if (!z.x_in) {
+    list[n++] = {(const T*)x, xs, z.rows, (bf16*)at};
+    m.x = (const bf16*)at;
+    m.xs = z.kp;
+    at += z.x;
+  }
+  if (!z.w_in) {
+    list[n++] = {(const T*)w, ws, z.V, (bf16*)at};
+    m.w = (const bf16*)at;
+    m.ws = z.kp;
+    at += z.w;
+  }
+  if (n) {
+    const int64_t longest = n == 2 && list[1].rows > list[0].rows ? list[1].rows : list[0].rows;
+    hipLaunchKernelGGL((ll_planes<T, std::is_same_v<T, float> ? 2 : 1>),
+                       dim3((unsigned)div_up(longest * (z.kp / 8), 256), (unsigned)n), dim3(256), 0, st, list[0],
+                       list[n - 1], (int)z.d, (int)z.kp);
+  }
   return m;
 }
 

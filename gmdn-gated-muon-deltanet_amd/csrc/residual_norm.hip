@@ -66,7 +66,8 @@ GMDN_DEV void load_ones(const void* w, bool w16, int d, int c, float (&v)[8]) {
   if (c < d && w) load8_weight(w, w16, c, d - c, v);
 }
 
-GMDN_DEV float sigmoid(float g) { return 1.f / (1.f + __builtin_amdgcn_exp2f(-g * LOG2E)); }
+// by the hardware's exponential and reciprocal, one unit in the last place each
+GMDN_DEV float sigmoid(float g) { return hw_rcp(1.f + __builtin_amdgcn_exp2f(-g * LOG2E)); }
 
 // The vectors of a call: the norm's weight, the post norm's, the scale.
 struct Vectors {
@@ -509,9 +510,10 @@ int gmdn_residual_norm_fwd(const void* x, const void* y, const void* weight, con
     const Branch<TY> in{(const TY*)y, (const TY*)gate, y_stride, gate_stride};
     with_parts(post_weight, gate, scale, [&](auto w) {
       constexpr Parts P = decltype(w)::P;
-      const dim3 grid((unsigned)rn_blocks<P>(rows, d, RN_FWD_BLOCKS));
       with_shape<P>(d, [&](auto s) {
         using S = decltype(s);
+        // one workgroup of 1024 threads is what a CU holds of this kernel
+        const dim3 grid((unsigned)rn_blocks<P>(rows, d, S::TPR == 1024 ? RN_FWD_BLOCKS / 2 : RN_FWD_BLOCKS));
         hipLaunchKernelGGL((rn_fwd<TX, TY, S::TPR, S::NV, P>), grid, dim3(rn_threads(S::TPR)), 0, (hipStream_t)stream,
                            (const TX*)x, x_stride, in, vec, (TX*)r, (TY*)z, rstd, post_rstd, rows, (int)d, eps);
       });

@@ -104,7 +104,7 @@ def test_forward_backward(rows, V, D, dtype):
 
 @pytest.mark.parametrize("dtype", [B, F])
 @pytest.mark.parametrize("rows,V,D", [(4001, 4200, 72), (1000, 16500, 64), (4096, 4096, 65), (300, 33000, 128),
-                                      (1500, 3001, 200), (257, 2000, 1000)])
+                                      (1500, 3001, 200), (257, 2000, 1000), (64, 5000, 40), (2100, 70, 64)])
 def test_large_products(rows, V, D, dtype):
     """Sizes at which the products are cut into larger tiles, whole and ragged, and
     split along k."""
