@@ -436,7 +436,7 @@ Sizes sizes_of(const void* x, const void* w, int64_t rows, int64_t V, int64_t d,
 
 int check_ll(int64_t rows, int64_t V, int64_t d, int64_t xs, int64_t ws, int32_t dtype) {
   if (rows < 0 || V <= 0 || d <= 0 || xs < 0 || ws < 0 || rows > ((int64_t)1 << 30)) return GMDN_ERR_ARG;
-  if (!type_ok(dtype) || V > (1 << 27) || d > (1 << 17)) return GMDN_ERR_UNSUPPORTED;
+  if (!type_ok(dtype) || rows > (1 << 27) || V > (1 << 27) || d > (1 << 17)) return GMDN_ERR_UNSUPPORTED;
   // what a launch's grid holds: 2^32 threads (tiles below 256 are taken where one side has
   // few of them)
   const int64_t longer = rows > V ? rows : V, most = 1 << 22;

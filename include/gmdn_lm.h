@@ -147,8 +147,8 @@ int gmdn_logprobs_bwd(const void* logits, const int64_t* tokens, const float* st
 
 /* -------------------------------- log probabilities from hidden states and a head
  * The same of the logits x weight^T, without them in memory: x (rows, d) and weight
- * (vocab, d) of one type, each with a row stride; vocab <= 2^27, d <= 2^17, and
- * none of the three products of more than 2^22 tiles of 256 x 256.
+ * (vocab, d) of one type, each with a row stride; rows and vocab <= 2^27, d <= 2^17,
+ * and none of the three products of more than 2^22 tiles of 256 x 256.
  * logprob, entropy and stats are as above.  bfloat16 operands are multiplied as they
  * are (rows of a multiple of 64 values at 16-byte addresses from where they lie, others
  * from copies in the workspace), float32 ones as three products of bfloat16 pieces,

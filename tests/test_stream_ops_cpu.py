@@ -97,7 +97,8 @@ def test_linear_logprobs_argument_checks():
     assert fwd_(dims=(-1, 300, 64, 64, 64)) == 1 and fwd_(dims=(100, 0, 64, 64, 64)) == 1
     assert fwd_(dims=(100, 300, 0, 64, 64)) == 1 and fwd_(dims=(100, 300, 64, -1, 64)) == 1
     assert fwd_(dims=(100, (1 << 27) + 1, 64, 64, 64)) == 2 and fwd_(dims=(100, 300, (1 << 17) + 1, 64, 64)) == 2
-    assert fwd_(dims=(1 << 24, 1 << 27, 64, 64, 64)) == 2 and fwd_(dims=(1 << 28, 300, 1024, 1024, 1024)) == 2
+    assert fwd_(dims=((1 << 27) + 1, 1, 64, 64, 64)) == 2 and fwd_(dims=(1 << 24, 1 << 27, 64, 64, 64)) == 2
+    assert fwd_(dims=(1 << 28, 300, 1024, 1024, 1024)) == 2
     assert fwd_(dtype=4) == 2
     assert fwd_(x=None, dims=(0, 300, 64, 64, 64)) == 0
 
