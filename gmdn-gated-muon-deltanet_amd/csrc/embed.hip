@@ -20,12 +20,12 @@ constexpr int EM_THREADS = 256;
 // A thread for each piece of eight values of y.
 template <typename T>
 __global__ void __launch_bounds__(EM_THREADS)
-em_gather(const T* __restrict__ w, const int64_t* __restrict__ tokens, T* __restrict__ y, int64_t pieces, int per_row,
-          int d, int64_t vocab, int64_t ws, float scale) {
-  const int64_t i = (int64_t)blockIdx.x * EM_THREADS + threadIdx.x;
+em_gather(const T* __restrict__ w, const int64_t* __restrict__ tokens, T* __restrict__ y, uint32_t pieces,
+          uint32_t per_row, int d, int64_t vocab, int64_t ws, float scale) {
+  const uint32_t i = blockIdx.x * EM_THREADS + threadIdx.x;
   if (i >= pieces) return;
   const int64_t row = i / per_row;
-  const int c = 8 * (int)(i - row * per_row);
+  const int c = 8 * (int)(i % per_row);
   const int64_t token = tokens[row];
   float v[8];
   if (token >= 0 && token < vocab) {
@@ -429,11 +429,12 @@ int gmdn_embed_fwd(const void* weight, const int64_t* tokens, void* y, int64_t r
   if (rows == 0) return GMDN_OK;
   if (!weight || !tokens || !y) return GMDN_ERR_ARG;
   const int64_t per_row = (d + 7) / 8, pieces = rows * per_row, groups = (pieces + EM_THREADS - 1) / EM_THREADS;
-  if (pieces >= (int64_t)1 << 32) return GMDN_ERR_UNSUPPORTED;
+  if (pieces > UINT32_MAX - EM_THREADS) return GMDN_ERR_UNSUPPORTED;
   with_type(dtype, [&](auto t) {
     using T = decltype(t);
     hipLaunchKernelGGL((em_gather<T>), dim3((unsigned)groups), dim3(EM_THREADS), 0, (hipStream_t)stream,
-                       (const T*)weight, tokens, (T*)y, pieces, (int)per_row, (int)d, vocab, w_stride, scale);
+                       (const T*)weight, tokens, (T*)y, (uint32_t)pieces, (uint32_t)per_row, (int)d, vocab, w_stride,
+                       scale);
   });
   return launched();
 }

@@ -45,11 +45,10 @@ template <typename T, int P>
 __global__ void __launch_bounds__(256)
 ll_planes(Whole<T> a, Whole<T> b, int d, int kp) {
   const Whole<T>& m = blockIdx.y == 0 ? a : b;
-  const int per = kp / 8;
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const uint32_t per = kp / 8, i = blockIdx.x * 256 + threadIdx.x;  // below 2^32 (check_ll)
   const int64_t r = i / per;
   if (r >= m.rows) return;
-  const int c = 8 * (int)(i - r * per);
+  const int c = 8 * (int)(i % per);
   float v[8];
   load8(m.x + r * m.stride + c, d - c, v);
   bf16* o = m.out + r * kp + c;
@@ -441,7 +440,7 @@ int check_ll(int64_t rows, int64_t V, int64_t d, int64_t xs, int64_t ws, int32_t
   // few of them)
   const int64_t longer = rows > V ? rows : V, most = 1 << 22;
   const bool fits = div_up(V, 256) * div_up(rows, 256) <= most && div_up(d, 256) * div_up(longer, 256) <= most &&
-                    longer * (round_up(d, KPAD) / 8) < (int64_t)1 << 32;
+                    longer * (round_up(d, KPAD) / 8) < ((int64_t)1 << 32) - 256;
   return fits ? GMDN_OK : GMDN_ERR_UNSUPPORTED;
 }
 

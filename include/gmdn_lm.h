@@ -59,7 +59,7 @@ int gmdn_layer_norm8_rebuild(const int8_t* q, const float* scale, const void* we
 /* ------------------------------------------------------------ token embedding
  * y (rows, d) = scale * weight[token]; a token outside [0, vocab) gives a row of
  * NaN.  weight is (vocab, d) with a row stride; vocab <= 2^27, d <= 2^20, and
- * y at most 2^32 pieces of eight values. */
+ * y less than 2^32 - 256 pieces of eight values. */
 int gmdn_embed_fwd(const void* weight, const int64_t* tokens, void* y, int64_t rows, int64_t vocab, int64_t d,
                    int64_t w_stride, float scale, int32_t dtype, void* stream);
 
