@@ -198,9 +198,9 @@ struct GradEpi {
       int token = -1;  // from the tile's first column
       if (row < e.rows) {
         const int64_t t = e.tokens[row];
-        gl = e.dlp && t != e.ignore ? e.dlp[row] : 0.f;
+        // of a token outside the vocabulary NaN; the entropy's gradient does not see the token
+        if (e.dlp && t != e.ignore) gl = t >= 0 && t < e.V ? e.dlp[row] : NAN;
         gh = e.dent ? e.dent[row] : 0.f;
-        if (t != e.ignore && (t < 0 || t >= e.V)) gl = NAN;
         m = e.stats[2 * row];
         logs = e.stats[2 * row + 1];
         h = e.entropy[row];

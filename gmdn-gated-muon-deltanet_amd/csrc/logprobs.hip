@@ -494,8 +494,9 @@ lp_bwd(const T* __restrict__ logits, int64_t stride, int64_t rows, const int64_t
   const bool empty = stats[2 * row] == -INFINITY;
   const float m = empty ? 0.f : stats[2 * row], logs = stats[2 * row + 1], h = entropy[row];
   const float gh = dent ? dent[row] : 0.f;
-  float gl = dlp && token != ignore ? dlp[row] : 0.f;
-  if (token != ignore && (token < 0 || token >= V)) gl = NAN;
+  // of a token outside the vocabulary NaN; the entropy's and the alternatives' gradients
+  // do not see the token
+  const float gl = !dlp || token == ignore ? 0.f : token >= 0 && token < V ? dlp[row] : NAN;
   float all = gl;
   if constexpr (TOP)
     for (int i = 0; i < top; ++i) all += dtop[row * top + i];

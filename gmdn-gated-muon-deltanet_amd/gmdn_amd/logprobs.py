@@ -61,8 +61,8 @@ def linear_logprobs(x: Tensor, weight: Tensor, tokens: Tensor, ignore_index: int
     float32 sums that are not rounded; their gradient is rounded to bfloat16 beside
     bfloat16 operands.  float32 products are taken as three products of bfloat16
     pieces, about 2^-16 relative error each.  Tokens are treated as in
-    ``token_logprobs``: one outside the vocabulary is NaN, and with it ``weight``'s
-    gradient, which sums over all rows.  Differentiable through both outputs, in ``x``
+    ``token_logprobs``: one outside the vocabulary is NaN, and through its log probability
+    ``weight``'s gradient, which sums over all rows.  Differentiable through both outputs, in ``x``
     and ``weight``.
     """
     ops.ensure()

@@ -139,7 +139,8 @@ int gmdn_logprobs_fwd(const void* logits, const int64_t* tokens, float* logprob,
 size_t gmdn_logprobs_fwd_workspace_bytes(int64_t rows, int64_t vocab, int32_t top);
 
 /* dlogits (rows, vocab) from the cotangents of logprob, entropy and
- * top_logprobs, each of which may be NULL. */
+ * top_logprobs, each of which may be NULL.  Where logprob's is given, a row whose token
+ * is outside the vocabulary (and not ignore_index) gets NaN. */
 int gmdn_logprobs_bwd(const void* logits, const int64_t* tokens, const float* stats, const float* entropy,
                       const int64_t* top_tokens, const float* dlogprob, const float* dentropy, const float* dtop,
                       void* dlogits, int64_t rows, int64_t vocab, int64_t stride, int32_t top, int64_t ignore_index,
@@ -162,7 +163,8 @@ int gmdn_linear_logprobs_fwd(const void* x, const void* weight, const int64_t* t
                              void* stream);
 
 /* dx (rows, d) and dweight (vocab, d), of the operands' type; either may be NULL.
- * dlogprob and dentropy may each be NULL: zeros.  The logits' gradient, of which the
+ * dlogprob and dentropy may each be NULL: zeros, also of the rows whose token is outside
+ * the vocabulary, whose dlogprob gives NaN.  The logits' gradient, of which the
  * workspace holds a piece of the vocabulary at a time, is rounded as the operands
  * are. */
 size_t gmdn_linear_logprobs_bwd_workspace_bytes(const void* x, const void* weight, int64_t rows, int64_t vocab,
