@@ -105,13 +105,16 @@ Residual residual_norm_fwd(const Tensor& x, const Tensor& y, const OptTensor& we
 bool from_r(const Tensor& x, bool plain) { return plain && x.scalar_type() == at::kFloat; }
 
 using Grads6 = std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor>;
-Grads6 residual_norm_bwd(const OptTensor& dr, const OptTensor& dz, const Tensor& r_or_x, const Tensor& y,
+Grads6 residual_norm_bwd(const OptTensor& dr, const OptTensor& dz, const Tensor& r_or_x, const OptTensor& y,
                          const OptTensor& weight, const OptTensor& post_weight, const OptTensor& gate,
-                         const OptTensor& scale, const Tensor& rstd_, const Tensor& post_rstd_) {
+                         const OptTensor& scale, const Tensor& rstd_, const Tensor& post_rstd_,
+                         std::optional<ScalarType> y_dtype) {
   const c10::DeviceGuard guard(r_or_x.device());
   const Tensor& x = r_or_x;
-  const ScalarType xt = x.scalar_type(), yt = y.scalar_type();
+  const ScalarType xt = x.scalar_type(), yt = y ? y->scalar_type() : y_dtype.value_or(xt);
   const int32_t xc = type_code(xt, "the stream"), yc = type_code(yt, "y");
+  TORCH_CHECK(y || from_r(x, !post_weight && !gate && !scale),
+              "y is given but for a float32 stream without post norm, gate and scale");
   const Rows r = rows_of(x, "the stream"), a = branch_of(dr, x, xt, "dr"), z = branch_of(dz, x, yt, "dz"),
              b = branch_of(y, x, yt, "y"), g = branch_of(gate, x, yt, "gate");
   const Vectors v = vectors_of(weight, post_weight, scale, x, r.d);
@@ -227,10 +230,10 @@ struct ResidualNormFwd : torch::autograd::Function<ResidualNormFwd> {
         GMDN_OP(residual_norm_fwd).call(x, y, weight, post_weight, gate, scale, eps);
     *rest = {rstd, post_rstd};
     ctx->set_materialize_grads(false);
-    // z in y's place: of its type and shape, and not read
     const bool after = from_r(x, !post_weight && !gate && !scale);
-    ctx->save_for_backward({after ? r : x, after ? z : y, opt(weight), opt(post_weight), opt(gate), opt(scale), rstd,
-                            post_rstd});
+    ctx->save_for_backward({after ? r : x, after ? Tensor() : y, opt(weight), opt(post_weight), opt(gate), opt(scale),
+                            rstd, post_rstd});
+    ctx->saved_data["y_dtype"] = y.scalar_type();
     return {r, z};
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& g) {
@@ -238,10 +241,11 @@ struct ResidualNormFwd : torch::autograd::Function<ResidualNormFwd> {
     variable_list out(8);
     if (!g[0].defined() && !g[1].defined()) return out;
     const auto s = ctx->get_saved_variables();
+    const ScalarType yt = ctx->saved_data["y_dtype"].toScalarType();
     auto [dx, dy, dw, dp, dg, ds] = GMDN_OP(residual_norm_bwd)
-                                        .call(opt(g[0]), opt(g[1]), s[0], s[1], opt(s[2]), opt(s[3]), opt(s[4]),
-                                              opt(s[5]), s[6], s[7]);
-    const bool same = !s[3].defined() && !s[4].defined() && !s[5].defined() && s[0].scalar_type() == s[1].scalar_type();
+                                        .call(opt(g[0]), opt(g[1]), s[0], opt(s[1]), opt(s[2]), opt(s[3]), opt(s[4]),
+                                              opt(s[5]), s[6], s[7], yt);
+    const bool same = !s[3].defined() && !s[4].defined() && !s[5].defined() && s[0].scalar_type() == yt;
     out[0] = dx;
     out[1] = same ? dx : dy;
     if (s[2].defined()) out[2] = dw;
@@ -309,9 +313,9 @@ TORCH_LIBRARY_FRAGMENT(gmdn, m) {
   m.def("embed_bwd(Tensor dy, Tensor tokens, SymInt vocab, float scale, SymInt padding_idx) -> Tensor", PT2);
   m.def("residual_norm_fwd(Tensor x, Tensor y, Tensor? weight, Tensor? post_weight, Tensor? gate, Tensor? scale, "
         "float eps) -> (Tensor, Tensor, Tensor, Tensor)", PT2);
-  m.def("residual_norm_bwd(Tensor? dr, Tensor? dz, Tensor r_or_x, Tensor y, Tensor? weight, Tensor? post_weight, "
-        "Tensor? gate, Tensor? scale, Tensor rstd, Tensor post_rstd) -> (Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)",
-        PT2);
+  m.def("residual_norm_bwd(Tensor? dr, Tensor? dz, Tensor r_or_x, Tensor? y, Tensor? weight, Tensor? post_weight, "
+        "Tensor? gate, Tensor? scale, Tensor rstd, Tensor post_rstd, ScalarType? y_dtype=None) -> "
+        "(Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)", PT2);
   m.def("linear_logprobs_fwd(Tensor x, Tensor weight, Tensor tokens, SymInt ignore_index) -> (Tensor, Tensor, Tensor)",
         PT2);
   m.def("linear_logprobs_bwd(Tensor x, Tensor weight, Tensor tokens, Tensor stats, Tensor entropy, Tensor? dlogprob, "

@@ -46,10 +46,10 @@ its model, train_ablation.py:420-422):
   embedding (gmdn_amd.embedding).
 * ``gmdn::residual_norm_fwd(x, y, weight, post_weight, gate, scale, eps) -> (r,
   z, rstd, post_rstd)`` and ``gmdn::residual_norm_bwd(dr, dz, r_or_x, y, weight,
-  post_weight, gate, scale, rstd, post_rstd) -> (dx, dy, dweight, dpost_weight,
-  dgate, dscale)`` -- a branch's way back into the residual stream and the norm
-  that follows.  The backward takes ``x``; of a float32 stream without post norm,
-  gate and scale it takes ``r``, and of ``y`` the type only.  Gradients of what is
+  post_weight, gate, scale, rstd, post_rstd, y_dtype) -> (dx, dy, dweight,
+  dpost_weight, dgate, dscale)`` -- a branch's way back into the residual stream and
+  the norm that follows.  The backward takes ``x``; of a float32 stream without post
+  norm, gate and scale it takes ``r``, and no ``y`` (``y_dtype`` says its type).  Gradients of what is
   absent are empty, and ``dy`` where it is ``dx`` (gmdn_amd.residual).
 * ``gmdn::linear_logprobs_fwd(x, weight, tokens, ignore_index) -> (logprob,
   entropy, stats)`` and ``gmdn::linear_logprobs_bwd(x, weight, tokens, stats,
@@ -271,11 +271,12 @@ def _residual_norm_fwd_fake(x, y, weight, post_weight, gate, scale, eps):
             x.new_empty(lead if post_weight is not None else (0,), dtype=torch.float32))
 
 
-def _residual_norm_bwd_fake(dr, dz, r_or_x, y, weight, post_weight, gate, scale, rstd, post_rstd):
-    same = post_weight is None and gate is None and scale is None and r_or_x.dtype == y.dtype
-    dw, dp, ds = (v.new_empty(v.shape) if v is not None else _empty(r_or_x) for v in (weight, post_weight, scale))
-    return (r_or_x.new_empty(r_or_x.shape), y.new_empty((0,) if same else r_or_x.shape), dw, dp,
-            y.new_empty(r_or_x.shape if gate is not None else (0,)), ds)
+def _residual_norm_bwd_fake(dr, dz, r_or_x, y, weight, post_weight, gate, scale, rstd, post_rstd, y_dtype=None):
+    x, y_dtype = r_or_x, y.dtype if y is not None else y_dtype or r_or_x.dtype
+    same = post_weight is None and gate is None and scale is None and x.dtype == y_dtype
+    dw, dp, ds = (v.new_empty(v.shape) if v is not None else _empty(x) for v in (weight, post_weight, scale))
+    return (x.new_empty(x.shape), x.new_empty((0,) if same else x.shape, dtype=y_dtype), dw, dp,
+            x.new_empty(x.shape if gate is not None else (0,), dtype=y_dtype), ds)
 
 
 def _linear_logprobs_fwd_fake(x, weight, tokens, ignore_index):
