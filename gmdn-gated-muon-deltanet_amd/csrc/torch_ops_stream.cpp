@@ -128,7 +128,7 @@ Grads6 residual_norm_bwd(const OptTensor& dr, const OptTensor& dz, const Tensor&
   const size_t need = vectors ? gmdn_residual_norm_bwd_workspace_floats(r.rows, r.d) : 0;
   const Tensor ws = need ? fresh(x, {(int64_t)need}) : Tensor();
   if (r.rows || vectors)
-    check(gmdn_residual_norm_bwd(ptr(a), ptr(z), r.ptr(), b.ptr(), ptr(v.w), ptr(v.p), ptr(g), ptr(v.s), fp(rstd),
+    check(gmdn_residual_norm_bwd(ptr(a), ptr(z), r.ptr(), ptr(b), ptr(v.w), ptr(v.p), ptr(g), ptr(v.s), fp(rstd),
                                  v.p ? fp(post) : nullptr, dx.data_ptr(), same ? nullptr : dy.data_ptr(),
                                  gate ? dg.data_ptr() : nullptr, v.w ? dw.data_ptr() : nullptr,
                                  v.p ? dp.data_ptr() : nullptr, v.s ? ds.data_ptr() : nullptr, need ? fp(ws) : nullptr,
