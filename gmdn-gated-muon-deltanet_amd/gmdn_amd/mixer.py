@@ -298,7 +298,7 @@ class LM(nn.Module):
     def _hidden(self, idx):
         """What the head reads."""
         x = self.emb(idx)
-        if self.blocks and all(blk.fused and _plain(blk, Block) for blk in self.blocks):
+        if self.blocks and all(_plain(blk, Block) and blk.fused for blk in self.blocks):
             norms = [*(blk.n1 for blk in self.blocks[1:]), self.norm_f]
             z = self.blocks[0].n1(x)
             for blk, norm in zip(self.blocks, norms):
