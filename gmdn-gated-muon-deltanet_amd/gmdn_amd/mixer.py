@@ -119,9 +119,11 @@ def _norm(kind: str, dim: int, checkpoint: str | None = None) -> nn.Module:
 
 def _plain(module: nn.Module, kind: type) -> bool:
     """Whether a call of ``module`` is ``kind``'s forward and nothing beside it:
-    not another class's, replaced or hooked."""
+    not another class's, replaced, compiled in place or hooked, by itself or with
+    all modules."""
     return type(module).forward is kind.forward and "forward" not in module.__dict__ and not (
-        module._forward_hooks or module._forward_pre_hooks or module._backward_hooks or module._backward_pre_hooks)
+        module._forward_hooks or module._forward_pre_hooks or module._backward_hooks or module._backward_pre_hooks
+        or module._compiled_call_impl is not None or nn.modules.module._has_any_global_hook())
 
 
 def _norm_eps(norm: nn.RMSNorm) -> float:
@@ -190,8 +192,8 @@ class Block(nn.Module):
     the sum for the next branch in one pass (gmdn_amd.residual); with it ``post_norm``
     norms a branch's output before it is added, ``gated`` multiplies it by a sigmoid
     of a linear layer of the branch's input, and ``layer_scale`` by a learned scale of each
-    channel that begins at this value.  A norm that is replaced or has a hook is
-    called as it is.
+    channel that begins at this value.  A norm that is replaced, compiled in place or
+    has a hook is called as it is.
     """
 
     fused = False  # also of a block that was saved whole before there was a choice
