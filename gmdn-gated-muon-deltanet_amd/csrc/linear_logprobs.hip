@@ -16,8 +16,11 @@
 //
 // bfloat16 operands are multiplied as they are; d is rounded to bfloat16 as the
 // gradient of bfloat16 logits would be.  float32 operands, and d beside them, are
-// split into two bfloat16 pieces (x = hi + lo up to 2^-17 |x|) and multiplied as lo hi +
-// hi lo + hi hi, what this library's other float32 products do.
+// split into bfloat16 pieces, each the rounding of what the ones before it leave:
+// in 'tf32' two (x = hi + lo up to 2^-18 |x|) multiplied as lo hi + hi lo + hi hi, what
+// this library's other float32 products do; in 'ieee' three (up to 2^-27 |x|), with the six
+// products above 2^-27, which leaves float32's rounding (1021 x 32003 x 1001, forward and
+// backward: 866 us and 1486).
 #include "../../include/gmdn_lm.h"
 #include <type_traits>
 #include "bf16mm.h"
@@ -387,7 +390,7 @@ bool with_tile(const Product& p, F&& f) {
 
 struct Sizes {
   int64_t rows, V, d, kp;
-  int P, pairs;
+  int P, pairs;                    // pieces of an operand, and products of two
   bool x_in, w_in;
   size_t x, w;                     // bytes of the operands' planes
   // forward
@@ -407,8 +410,8 @@ Sizes sizes_of(const void* x, const void* w, int64_t rows, int64_t V, int64_t d,
   z.V = V;
   z.d = d;
   z.kp = round_up(d, KPAD);
-  z.P = dtype == GMDN_DTYPE_F32 ? 2 : 1;
-  z.pairs = z.P == 1 ? 1 : 3;
+  z.P = dtype == GMDN_DTYPE_F32_IEEE ? 3 : dtype == GMDN_DTYPE_F32 ? 2 : 1;
+  z.pairs = z.P * (z.P + 1) / 2;
   z.x_in = in_place(x, xs, d, dtype);
   z.w_in = in_place(w, ws, d, dtype);
   z.x = z.x_in ? 0 : up((size_t)(z.P * rows * z.kp * 2));
@@ -435,7 +438,7 @@ Sizes sizes_of(const void* x, const void* w, int64_t rows, int64_t V, int64_t d,
 
 int check_ll(int64_t rows, int64_t V, int64_t d, int64_t xs, int64_t ws, int32_t dtype) {
   if (rows < 0 || V <= 0 || d <= 0 || xs < 0 || ws < 0 || rows > ((int64_t)1 << 30)) return GMDN_ERR_ARG;
-  if (!type_ok(dtype) || rows > (1 << 27) || V > (1 << 27) || d > (1 << 17)) return GMDN_ERR_UNSUPPORTED;
+  if ((!type_ok(dtype) && dtype != GMDN_DTYPE_F32_IEEE) || rows > (1 << 27) || V > (1 << 27) || d > (1 << 17)) return GMDN_ERR_UNSUPPORTED;
   // what a launch's grid holds: 2^32 threads (tiles below 256 are taken where one side has
   // few of them)
   const int64_t longer = rows > V ? rows : V, most = 1 << 22;
@@ -444,7 +447,8 @@ int check_ll(int64_t rows, int64_t V, int64_t d, int64_t xs, int64_t ws, int32_t
   return fits ? GMDN_OK : GMDN_ERR_UNSUPPORTED;
 }
 
-// A product's arguments; the pairs of planes with the small terms first: lo hi, hi lo, hi hi.
+// A product's arguments; the pairs of planes with the small terms first: lo hi, hi lo, hi hi
+// of two, and of three (0 the largest) 2 0, 1 1, 0 2, 1 0, 0 1, 0 0.
 template <class S>
 MMArgs args_of(const MMOperand& a, const MMOperand& b, int64_t M, int64_t N, int64_t k, int pairs, int per) {
   static_assert(S::BK == KPAD, "a stage is what the operands are padded to");
@@ -456,8 +460,8 @@ MMArgs args_of(const MMOperand& a, const MMOperand& b, int64_t M, int64_t N, int
   r.tiles_m = (int)div_up(M, S::TM);
   r.tiles_n = (int)div_up(N, S::TN);
   r.pairs = pairs;
-  r.pair_a = pairs == 1 ? 0 : 0x001;
-  r.pair_b = pairs == 1 ? 0 : 0x010;
+  r.pair_a = pairs == 1 ? 0 : pairs == 3 ? 0x001 : 0x001012;
+  r.pair_b = pairs == 1 ? 0 : pairs == 3 ? 0x010 : 0x010210;
   return r;
 }
 
@@ -466,7 +470,7 @@ struct Matrices {
   int64_t xs, ws, xp, wp;  // row strides, plane strides
 };
 // The operands' planes: where they lie, or made at `at`, which moves on.
-template <typename T>
+template <typename T, int P>
 Matrices matrices_of(const void* x, const void* w, int64_t xs, int64_t ws, const Sizes& z, char*& at, hipStream_t st) {
   Matrices m{(const bf16*)x, (const bf16*)w, xs, ws, z.rows * z.kp, z.V * z.kp};
   Whole<T> list[2];
@@ -485,9 +489,8 @@ Matrices matrices_of(const void* x, const void* w, int64_t xs, int64_t ws, const
   }
   if (n) {
     const int64_t longest = n == 2 && list[1].rows > list[0].rows ? list[1].rows : list[0].rows;
-    hipLaunchKernelGGL((ll_planes<T, std::is_same_v<T, float> ? 2 : 1>),
-                       dim3((unsigned)div_up(longest * (z.kp / 8), 256), (unsigned)n), dim3(256), 0, st, list[0],
-                       list[n - 1], (int)z.d, (int)z.kp);
+    hipLaunchKernelGGL((ll_planes<T, P>), dim3((unsigned)div_up(longest * (z.kp / 8), 256), (unsigned)n), dim3(256),
+                       0, st, list[0], list[n - 1], (int)z.d, (int)z.kp);
   }
   return m;
 }
@@ -505,9 +508,8 @@ void sum_planes(const float* planes, T* out, int64_t n, int count, hipStream_t s
   hipLaunchKernelGGL((ll_sum_planes<T>), dim3((unsigned)div_up(n, 8 * 256)), dim3(256), 0, st, planes, out, n, count);
 }
 
-template <typename T>
+template <typename T, int P>
 bool backward(const Matrices& m, const Sizes& z, GradArgs e, float* x_acc, float* w_acc, T* dx, T* dw, hipStream_t st) {
-  constexpr int P = std::is_same_v<T, float> ? 2 : 1;
   const int64_t plane = z.padded * z.piece;
   for (int64_t i = 0; i < z.pieces; ++i) {
     const int64_t v0 = i * z.piece, left = z.V - v0 < z.piece ? z.V - v0 : z.piece;
@@ -546,6 +548,19 @@ bool backward(const Matrices& m, const Sizes& z, GradArgs e, float* x_acc, float
   return true;
 }
 
+template <typename T_, int P_>
+struct Operands {
+  using T = T_;
+  static constexpr int P = P_;
+};
+// f(type and pieces of the operands)
+template <class F>
+void with_operands(int32_t dtype, F&& f) {
+  if (dtype == GMDN_DTYPE_BF16) f(Operands<bf16, 1>{});
+  else if (dtype == GMDN_DTYPE_F32) f(Operands<float, 2>{});
+  else f(Operands<float, 3>{});
+}
+
 }  // namespace
 }  // namespace gmdn
 
@@ -571,8 +586,11 @@ int gmdn_linear_logprobs_fwd(const void* x, const void* weight, const int64_t* t
   if ((uintptr_t)workspace % 16) return GMDN_ERR_ARG;
   const hipStream_t st = (hipStream_t)stream;
   char* at = (char*)workspace;
-  const Matrices m = dtype == GMDN_DTYPE_F32 ? matrices_of<float>(x, weight, x_stride, w_stride, z, at, st)
-                                             : matrices_of<bf16>(x, weight, x_stride, w_stride, z, at, st);
+  Matrices m;
+  with_operands(dtype, [&](auto o) {
+    using O = decltype(o);
+    m = matrices_of<typename O::T, O::P>(x, weight, x_stride, w_stride, z, at, st);
+  });
   const SumsArgs e{tokens, (float*)at, (float*)(at + z.at_token), rows, (int)vocab};
   const int tiles = (int)div_up(vocab, z.logits.edge);
   const bool ok = with_tile(z.logits, [&](auto s) {
@@ -608,14 +626,17 @@ int gmdn_linear_logprobs_bwd(const void* x, const void* weight, const int64_t* t
   if ((uintptr_t)workspace % 16) return GMDN_ERR_ARG;
   const hipStream_t st = (hipStream_t)stream;
   char* at = (char*)workspace;
-  const Matrices m = dtype == GMDN_DTYPE_F32 ? matrices_of<float>(x, weight, x_stride, w_stride, z, at, st)
-                                             : matrices_of<bf16>(x, weight, x_stride, w_stride, z, at, st);
-  const GradArgs e{tokens, stats, entropy, dlogprob, dentropy, (bf16*)at, rows, z.padded, z.piece, 0, 0, vocab,
-                  ignore_index};
-  float* const xa = (float*)(at + z.grad);
-  float* const wa = (float*)(at + z.grad + z.x_acc);
-  const bool ok = dtype == GMDN_DTYPE_F32 ? backward<float>(m, z, e, xa, wa, (float*)dx, (float*)dweight, st)
-                                          : backward<bf16>(m, z, e, xa, wa, (bf16*)dx, (bf16*)dweight, st);
+  bool ok = false;
+  with_operands(dtype, [&](auto o) {
+    using T = typename decltype(o)::T;
+    constexpr int P = decltype(o)::P;
+    const Matrices m = matrices_of<T, P>(x, weight, x_stride, w_stride, z, at, st);
+    const GradArgs e{tokens, stats, entropy, dlogprob, dentropy, (bf16*)at, rows, z.padded, z.piece, 0, 0, vocab,
+                     ignore_index};
+    float* const xa = (float*)(at + z.grad);
+    float* const wa = (float*)(at + z.grad + z.x_acc);
+    ok = backward<T, P>(m, z, e, xa, wa, (T*)dx, (T*)dweight, st);
+  });
   return ok ? launched() : GMDN_ERR_LAUNCH;
 }
 

@@ -147,10 +147,17 @@ Rows head_of(const Tensor& weight, const Tensor& x, const Rows& r) {
   TORCH_CHECK(w.d == r.d, "weight has rows of ", w.d, " values where x has ", r.d);
   return w;
 }
-std::tuple<Tensor, Tensor, Tensor> linear_logprobs_fwd(const Tensor& x, const Tensor& weight, const Tensor& tokens,
-                                                       int64_t ignore_index) {
-  const c10::DeviceGuard guard(x.device());
+// The operands' type code; `precision` is of float32 ones.
+int32_t operands_code(const Tensor& x, int64_t precision) {
   const int32_t code = type_code(x.scalar_type(), "x");
+  TORCH_CHECK(precision == GMDN_PREC_TF32 || precision == GMDN_PREC_IEEE, "precision is 0 ('tf32') or 1 ('ieee'), got ",
+              precision);
+  return code == GMDN_DTYPE_F32 && precision == GMDN_PREC_IEEE ? GMDN_DTYPE_F32_IEEE : code;
+}
+std::tuple<Tensor, Tensor, Tensor> linear_logprobs_fwd(const Tensor& x, const Tensor& weight, const Tensor& tokens,
+                                                       int64_t ignore_index, int64_t precision) {
+  const c10::DeviceGuard guard(x.device());
+  const int32_t code = operands_code(x, precision);
   const Rows r = rows_of(x, "x"), w = head_of(weight, x, r);
   const Tensor tk = tokens_of(tokens, x, lead(x));
   Tensor lp = fresh(x, lead(x)), entropy = fresh(x, lead(x)), stats = fresh(x, with_last(lead(x), 2));
@@ -167,9 +174,9 @@ std::tuple<Tensor, Tensor, Tensor> linear_logprobs_fwd(const Tensor& x, const Te
 std::tuple<Tensor, Tensor> linear_logprobs_bwd(const Tensor& x, const Tensor& weight, const Tensor& tokens,
                                                const Tensor& stats_, const Tensor& entropy_, const OptTensor& dlogprob,
                                                const OptTensor& dentropy, int64_t ignore_index, bool need_x,
-                                               bool need_weight) {
+                                               bool need_weight, int64_t precision) {
   const c10::DeviceGuard guard(x.device());
-  const int32_t code = type_code(x.scalar_type(), "x");
+  const int32_t code = operands_code(x, precision);
   const Rows r = rows_of(x, "x"), w = head_of(weight, x, r);
   const auto shape = lead(x);
   const Tensor tk = tokens_of(tokens, x, shape);
@@ -271,37 +278,39 @@ Residual residual_norm_fwd_ad(const Tensor& x, const Tensor& y, const OptTensor&
 struct LinearLogprobsFwd : torch::autograd::Function<LinearLogprobsFwd> {
   static constexpr bool is_traceable = true;
   static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const Tensor& tokens,
-                               c10::SymInt ignore_index, Tensor* rest) {
+                               c10::SymInt ignore_index, c10::SymInt precision, Tensor* rest) {
     at::AutoDispatchBelowADInplaceOrView below;
-    auto [lp, entropy, stats] = GMDN_OP(linear_logprobs_fwd).call(x, weight, tokens, ignore_index);
+    auto [lp, entropy, stats] = GMDN_OP(linear_logprobs_fwd).call(x, weight, tokens, ignore_index, precision);
     *rest = stats;
     ctx->set_materialize_grads(false);
     ctx->save_for_backward({x, weight, tokens, stats, entropy});
     ctx->saved_data["ignore_index"] = ignore_index;
+    ctx->saved_data["precision"] = precision;
     ctx->saved_data["need_x"] = x.requires_grad();
     ctx->saved_data["need_weight"] = weight.requires_grad();
     return {lp, entropy};
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& g) {
     const Tensor none;
-    if (!g[0].defined() && !g[1].defined()) return {none, none, none, none, none};
+    if (!g[0].defined() && !g[1].defined()) return {none, none, none, none, none, none};
     const auto s = ctx->get_saved_variables();
     const bool need_x = ctx->saved_data["need_x"].toBool(), need_weight = ctx->saved_data["need_weight"].toBool();
     auto [dx, dw] = GMDN_OP(linear_logprobs_bwd)
                         .call(s[0], s[1], s[2], s[3], s[4], opt(g[0]), opt(g[1]),
-                              ctx->saved_data["ignore_index"].toSymInt(), need_x, need_weight);
-    return {need_x ? dx : none, need_weight ? dw : none, none, none, none};
+                              ctx->saved_data["ignore_index"].toSymInt(), need_x, need_weight,
+                              ctx->saved_data["precision"].toSymInt());
+    return {need_x ? dx : none, need_weight ? dw : none, none, none, none, none};
   }
 };
 std::tuple<Tensor, Tensor, Tensor> linear_logprobs_fwd_ad(const Tensor& x, const Tensor& weight, const Tensor& tokens,
-                                                          c10::SymInt ignore_index) {
+                                                          c10::SymInt ignore_index, c10::SymInt precision) {
   refuse_tangents("linear_logprobs_fwd", {&x, &weight});
   if (!wants_grad({&x, &weight})) {
     at::AutoDispatchBelowADInplaceOrView below;
-    return GMDN_OP(linear_logprobs_fwd).call(x, weight, tokens, ignore_index);
+    return GMDN_OP(linear_logprobs_fwd).call(x, weight, tokens, ignore_index, precision);
   }
   Tensor stats;
-  auto r = LinearLogprobsFwd::apply(x, weight, tokens, ignore_index, &stats);
+  auto r = LinearLogprobsFwd::apply(x, weight, tokens, ignore_index, precision, &stats);
   return {r[0], r[1], stats};
 }
 
@@ -316,10 +325,11 @@ TORCH_LIBRARY_FRAGMENT(gmdn, m) {
   m.def("residual_norm_bwd(Tensor? dr, Tensor? dz, Tensor r_or_x, Tensor? y, Tensor? weight, Tensor? post_weight, "
         "Tensor? gate, Tensor? scale, Tensor rstd, Tensor post_rstd, ScalarType? y_dtype=None) -> "
         "(Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)", PT2);
-  m.def("linear_logprobs_fwd(Tensor x, Tensor weight, Tensor tokens, SymInt ignore_index) -> (Tensor, Tensor, Tensor)",
-        PT2);
+  m.def("linear_logprobs_fwd(Tensor x, Tensor weight, Tensor tokens, SymInt ignore_index, SymInt precision=0) -> "
+        "(Tensor, Tensor, Tensor)", PT2);
   m.def("linear_logprobs_bwd(Tensor x, Tensor weight, Tensor tokens, Tensor stats, Tensor entropy, Tensor? dlogprob, "
-        "Tensor? dentropy, SymInt ignore_index, bool need_x, bool need_weight) -> (Tensor, Tensor)", PT2);
+        "Tensor? dentropy, SymInt ignore_index, bool need_x, bool need_weight, SymInt precision=0) -> (Tensor, Tensor)",
+        PT2);
 }
 
 TORCH_LIBRARY_IMPL(gmdn, CUDA, m) {

@@ -14,7 +14,7 @@ from typing import NamedTuple
 import torch
 from torch import Tensor
 
-from . import ops
+from . import ops, scan
 
 IGNORE = -100
 MAX_TOP = 32
@@ -52,7 +52,8 @@ class LinearLogprobs(NamedTuple):
     entropy: Tensor  # of the distribution, in nats
 
 
-def linear_logprobs(x: Tensor, weight: Tensor, tokens: Tensor, ignore_index: int = IGNORE) -> LinearLogprobs:
+def linear_logprobs(x: Tensor, weight: Tensor, tokens: Tensor, ignore_index: int = IGNORE,
+                    precision: str | None = None) -> LinearLogprobs:
     """``token_logprobs(x @ weight.t(), tokens)`` without the logits: they are
     formed tile by tile, and again a piece of the vocabulary at a time in the backward.
 
@@ -60,7 +61,9 @@ def linear_logprobs(x: Tensor, weight: Tensor, tokens: Tensor, ignore_index: int
     (under autocast they are taken in its type, as by a linear layer).  The logits are
     float32 sums that are not rounded; their gradient is rounded to bfloat16 beside
     bfloat16 operands.  float32 products are taken as three products of bfloat16
-    pieces, about 2^-16 relative error each.  Tokens are treated as in
+    pieces, about 2^-16 relative error each, or in 'ieee' as six, which leave float32's
+    rounding; ``precision`` ('tf32' or 'ieee') overrides the process-wide setting
+    (``set_precision``).  Tokens are treated as in
     ``token_logprobs``: one outside the vocabulary is NaN, and through its log probability
     ``weight``'s gradient, which sums over all rows.  Differentiable through both outputs, in ``x``
     and ``weight``.
@@ -69,7 +72,8 @@ def linear_logprobs(x: Tensor, weight: Tensor, tokens: Tensor, ignore_index: int
     dt = ops.autocast_dtype(x)
     if dt is not None:
         x, weight = x.to(dt), weight.to(dt)
-    lp, entropy, _ = torch.ops.gmdn.linear_logprobs_fwd(x, weight, tokens, ignore_index)
+    lp, entropy, _ = torch.ops.gmdn.linear_logprobs_fwd(x, weight, tokens, ignore_index,
+                                                        scan.precision_code(precision))
     return LinearLogprobs(lp, entropy)
 
 
@@ -77,9 +81,10 @@ def _mean_loss(logprob: Tensor, targets: Tensor, ignore_index: int) -> Tensor:
     return -logprob.sum() / (targets != ignore_index).sum()
 
 
-def linear_cross_entropy(x: Tensor, weight: Tensor, targets: Tensor, ignore_index: int = IGNORE) -> Tensor:
+def linear_cross_entropy(x: Tensor, weight: Tensor, targets: Tensor, ignore_index: int = IGNORE,
+                         precision: str | None = None) -> Tensor:
     """``cross_entropy(x @ weight.t(), targets)`` without the logits."""
-    return _mean_loss(linear_logprobs(x, weight, targets, ignore_index).logprob, targets, ignore_index)
+    return _mean_loss(linear_logprobs(x, weight, targets, ignore_index, precision).logprob, targets, ignore_index)
 
 
 def cross_entropy(logits: Tensor, targets: Tensor, ignore_index: int = IGNORE) -> Tensor:

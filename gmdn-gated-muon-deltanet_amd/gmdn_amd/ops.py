@@ -51,11 +51,12 @@ its model, train_ablation.py:420-422):
   the norm that follows.  The backward takes ``x``; of a float32 stream without post
   norm, gate and scale it takes ``r``, and no ``y`` (``y_dtype`` says its type).  Gradients of what is
   absent are empty, and ``dy`` where it is ``dx`` (gmdn_amd.residual).
-* ``gmdn::linear_logprobs_fwd(x, weight, tokens, ignore_index) -> (logprob,
-  entropy, stats)`` and ``gmdn::linear_logprobs_bwd(x, weight, tokens, stats,
-  entropy, dlogprob, dentropy, ignore_index, need_x, need_weight) -> (dx,
-  dweight)`` -- log probabilities from hidden states and the head's weight,
-  without the logits (gmdn_amd.logprobs).
+* ``gmdn::linear_logprobs_fwd(x, weight, tokens, ignore_index, precision) ->
+  (logprob, entropy, stats)`` and ``gmdn::linear_logprobs_bwd(x, weight, tokens,
+  stats, entropy, dlogprob, dentropy, ignore_index, need_x, need_weight,
+  precision) -> (dx, dweight)`` -- log probabilities from hidden states and the
+  head's weight, without the logits; precision is that of float32 products
+  (gmdn_amd.logprobs).
 * ``gmdn::msign(M, steps, eps) -> X`` -- the outer Muon optimizer's msign of
   a batch of matrices (train_ablation.py:60-73); no autograd (the optimizer
   runs it under ``no_grad``).
@@ -279,12 +280,13 @@ def _residual_norm_bwd_fake(dr, dz, r_or_x, y, weight, post_weight, gate, scale,
             x.new_empty(x.shape if gate is not None else (0,), dtype=y_dtype), ds)
 
 
-def _linear_logprobs_fwd_fake(x, weight, tokens, ignore_index):
+def _linear_logprobs_fwd_fake(x, weight, tokens, ignore_index, precision=nat.PREC_TF32):
     lead = x.shape[:-1]
     return (*(x.new_empty(lead, dtype=torch.float32) for _ in range(2)), x.new_empty((*lead, 2), dtype=torch.float32))
 
 
-def _linear_logprobs_bwd_fake(x, weight, tokens, stats, entropy, dlogprob, dentropy, ignore_index, need_x, need_weight):
+def _linear_logprobs_bwd_fake(x, weight, tokens, stats, entropy, dlogprob, dentropy, ignore_index, need_x, need_weight,
+                              precision=nat.PREC_TF32):
     return x.new_empty(x.shape if need_x else (0,)), weight.new_empty(weight.shape if need_weight else (0,))
 
 

@@ -36,7 +36,8 @@ def _pad_sq(x, d: int):
 
 
 def set_precision(name: str) -> None:
-    """'tf32' (bf16x3 split MFMA on gfx950) or 'ieee' (fp32 MFMA)."""
+    """'tf32' (bf16x3 split MFMA on gfx950) or 'ieee' (fp32 MFMA, and in
+    ``linear_logprobs`` bf16 pieces that leave fp32's rounding)."""
     if name not in ("tf32", "ieee"):
         raise ValueError(f"precision must be 'tf32' or 'ieee', got {name!r}")
     _state["precision"] = name
@@ -55,6 +56,11 @@ def _prec_code_of(precision: str) -> int:
     if precision not in ("tf32", "ieee"):
         raise ValueError(f"precision must be 'tf32' or 'ieee', got {precision!r}")
     return nat.PREC_TF32 if precision == "tf32" else nat.PREC_IEEE
+
+
+def precision_code(precision: str | None = None) -> int:
+    """PREC_* of a call's ``precision``, without one of the process-wide setting."""
+    return _prec_code() if precision is None else _prec_code_of(precision)
 
 
 def _effective_prec(rule: int, save: bool, prec: int) -> int:
@@ -100,7 +106,7 @@ def hip_state_scan(U, K, a, b, m, n, rule: int, ns: int, precision: str | None =
     kd = _padded_dh(dh)
     ins = [_f32(t) for t in (_pad_sq(U, kd), _pad_sq(K, kd), a, b, m, n)]
     save = torch.is_grad_enabled() and any(t.requires_grad for t in (U, K, a, b, m, n))
-    prec = _effective_prec(rule, save, _prec_code() if precision is None else _prec_code_of(precision))
+    prec = _effective_prec(rule, save, precision_code(precision))
     S_all, _, _ = torch.ops.gmdn.state_scan(*ins, rule, ns, prec, save)
     if kd != dh:
         S_all = S_all[..., :dh, :dh]

@@ -146,6 +146,9 @@ int gmdn_logprobs_bwd(const void* logits, const int64_t* tokens, const float* st
                       void* dlogits, int64_t rows, int64_t vocab, int64_t stride, int32_t top, int64_t ignore_index,
                       int32_t dtype, void* stream);
 
+/* A `dtype` of the calls below: float32 operands in GMDN_PREC_IEEE. */
+#define GMDN_DTYPE_F32_IEEE 2
+
 /* -------------------------------- log probabilities from hidden states and a head
  * The same of the logits x weight^T, without them in memory: x (rows, d) and weight
  * (vocab, d) of one type, each with a row stride; rows and vocab <= 2^27, d <= 2^17,
@@ -153,7 +156,8 @@ int gmdn_logprobs_bwd(const void* logits, const int64_t* tokens, const float* st
  * logprob, entropy and stats are as above.  bfloat16 operands are multiplied as they
  * are (rows of a multiple of 64 values at 16-byte addresses from where they lie, others
  * from copies in the workspace), float32 ones as three products of bfloat16 pieces,
- * about 2^-16 relative error a product.  The workspace is 16-byte aligned; its size
+ * about 2^-16 relative error a product, or with GMDN_DTYPE_F32_IEEE as six, which
+ * leave float32's rounding.  The workspace is 16-byte aligned; its size
  * goes by where x and weight lie, too. */
 size_t gmdn_linear_logprobs_fwd_workspace_bytes(const void* x, const void* weight, int64_t rows, int64_t vocab,
                                                 int64_t d, int64_t x_stride, int64_t w_stride, int32_t dtype);
