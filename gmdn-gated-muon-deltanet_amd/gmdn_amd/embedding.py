@@ -32,11 +32,23 @@ def embedding(tokens: Tensor, weight: Tensor, scale: float = 1.0, padding_idx: i
 
 
 class Embedding(nn.Embedding):
-    """``nn.Embedding`` through ``embedding``, with a scale."""
+    """``nn.Embedding`` through ``embedding``, with a scale.  Its further options
+    (``max_norm``, ``scale_grad_by_freq``, ``sparse``) are refused."""
 
-    def __init__(self, num_embeddings: int, embedding_dim: int, padding_idx: int | None = None, scale: float = 1.0):
-        super().__init__(num_embeddings, embedding_dim, padding_idx=padding_idx)
+    def __init__(self, num_embeddings: int, embedding_dim: int, padding_idx: int | None = None, scale: float = 1.0, **options):
+        super().__init__(num_embeddings, embedding_dim, padding_idx=padding_idx, **options)
+        for name in ("max_norm", "scale_grad_by_freq", "sparse"):
+            if getattr(self, name):
+                raise ValueError(f"{name} is not supported")
         self.scale = scale
+
+    @classmethod
+    def from_pretrained(cls, embeddings: Tensor, freeze: bool = True, padding_idx: int | None = None, scale: float = 1.0,
+                        **options):
+        """A module of this table; ``freeze``: without a gradient."""
+        made = super().from_pretrained(embeddings, freeze=freeze, padding_idx=padding_idx, **options)
+        made.scale = scale
+        return made
 
     def forward(self, tokens: Tensor) -> Tensor:
         return embedding(tokens, self.weight, self.scale, self.padding_idx)
