@@ -42,15 +42,16 @@ em_gather(const T* __restrict__ w, const int64_t* __restrict__ tokens, T* __rest
 // ---------------------------------------------------- positions by token
 // Least significant digit first, up to 9 bits a pass.  A workgroup moves one
 // tile of consecutive positions; where they go follows from how often each
-// digit comes in all tiles and in the earlier ones.  Tokens outside the vocabulary
-// and the padding token get the key `vocab`, behind all others.
+// digit comes in all tiles and in the earlier ones, counted by a launch before it
+// (workgroups that count all tokens themselves instead save it, and lose: the whole
+// gradient of 16384 tokens of 32000 x 1024 took 62 us so and takes 52, of 64 tokens 34 and 28,
+// of 65536 161 and 109).  Tokens outside the vocabulary and the padding token get the key
+// `vocab`, behind all others.
 constexpr int SORT_THREADS = 1024;
 constexpr int SORT_WAVES = SORT_THREADS / 64;
 constexpr int SORT_BITS = 9;
 constexpr int SORT_BINS = 1 << SORT_BITS;
-constexpr int SORT_AHEAD = 8;            // keys of a thread in flight while it counts
 constexpr int SORT_TILES = 256;          // at most; a tile is a multiple of SORT_THREADS
-constexpr int64_t SORT_SELF = 32768;     // up to here each workgroup counts all digits itself
 
 struct SortInput {
   const int64_t* tokens;  // the first pass's, else null
@@ -97,54 +98,20 @@ em_count(SortInput in, uint32_t* __restrict__ counts, int64_t tile, int shift, i
 __global__ void __launch_bounds__(SORT_THREADS)
 em_scatter(SortInput in, const uint32_t* __restrict__ counts, uint32_t* __restrict__ keys, uint32_t* __restrict__ at,
            int64_t tile, int shift, int bits) {
-  __shared__ uint32_t total[SORT_BINS], below[SORT_BINS];
   __shared__ uint32_t waves[SORT_WAVES][SORT_BINS];
   __shared__ uint32_t sums[SORT_BINS / 64];
   const int t = threadIdx.x, w = wave_id();
   const uint64_t before = (1ull << lane_id()) - 1;
   const int64_t first = blockIdx.x * tile;
-  auto digit_of = [&](uint32_t key) { return (key >> shift) & ((1u << bits) - 1); };
-  if (t < SORT_BINS) total[t] = below[t] = 0;
-  __syncthreads();
-  if (counts) {
-    if (t < SORT_BINS) {
-      uint32_t all = 0, less = 0;
-      for (unsigned i = 0; i < gridDim.x; ++i) {
-        const uint32_t c = counts[(int64_t)t * gridDim.x + i];
-        all += c;
-        less += i < blockIdx.x ? c : 0;
-      }
-      total[t] = all;
-      below[t] = less;
-    }
-  } else {
-    // eight keys of a thread in flight: one after another they would wait for memory
-    // sixteen times for 16384 tokens
-    for (int64_t i0 = 0; i0 < in.n; i0 += SORT_AHEAD * SORT_THREADS) {
-      uint32_t key[SORT_AHEAD];
-#pragma unroll
-      for (int j = 0; j < SORT_AHEAD; ++j) {
-        const int64_t i = i0 + j * SORT_THREADS + t;
-        key[j] = in.key(i < in.n ? i : in.n - 1);
-      }
-#pragma unroll
-      for (int j = 0; j < SORT_AHEAD; ++j) {
-        const int64_t at = i0 + j * SORT_THREADS;
-        const bool live = at + t < in.n;
-        const uint32_t digit = digit_of(key[j]);
-        const uint64_t peers = same_digit(digit, live, bits);
-        if (live && (peers & before) == 0) {
-          atomicAdd(&total[digit], (uint32_t)__popcll(peers));
-          if (at < first) atomicAdd(&below[digit], (uint32_t)__popcll(peers));
-        }
-      }
-    }
-  }
-  __syncthreads();
-  // where each digit of this tile starts: the smaller digits, and its own in earlier tiles
-  uint32_t mine = 0, run = 0;
+  // how often each digit comes, and where the smaller ones of a wave's 64 end
+  uint32_t mine = 0, below = 0, run = 0;
   if (t < SORT_BINS) {
-    mine = run = total[t];
+    for (unsigned i = 0; i < gridDim.x; ++i) {
+      const uint32_t c = counts[(int64_t)t * gridDim.x + i];
+      mine += c;
+      below += i < blockIdx.x ? c : 0;
+    }
+    run = mine;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
       const uint32_t u = (uint32_t)__shfl_up((int)run, o, 64);
@@ -153,17 +120,18 @@ em_scatter(SortInput in, const uint32_t* __restrict__ counts, uint32_t* __restri
     if (lane_id() == 63) sums[w] = run;
   }
   __syncthreads();
+  // where each digit of this tile starts: the smaller digits, and its own in earlier tiles
   uint32_t base = 0;
   if (t < SORT_BINS) {
     for (int i = 0; i < w; ++i) base += sums[i];
-    base += run - mine + below[t];
+    base += run - mine + below;
   }
   for (int64_t i0 = first; i0 < first + tile && i0 < in.n; i0 += SORT_THREADS) {
     for (int i = t; i < SORT_WAVES * SORT_BINS; i += SORT_THREADS) (&waves[0][0])[i] = 0;
     __syncthreads();
     const int64_t i = i0 + t;
     const bool live = i < in.n;
-    const uint32_t key = live ? in.key(i) : 0, digit = digit_of(key);
+    const uint32_t key = live ? in.key(i) : 0, digit = (key >> shift) & ((1u << bits) - 1);
     const uint64_t peers = same_digit(digit, live, bits);
     const uint32_t rank = (uint32_t)__popcll(peers & before);
     if (live && rank == 0) waves[w][digit] = (uint32_t)__popcll(peers);
@@ -384,7 +352,6 @@ void with_type(int32_t dtype, F&& f) {
 struct Plan {
   int64_t tile, tiles, block, blocks;
   int passes, bits;
-  bool self;
   size_t keys, counts, part;  // bytes
   size_t bytes() const { return 4 * keys + counts + part; }
 };
@@ -398,12 +365,11 @@ Plan plan_of(int64_t n, int64_t vocab, int64_t d) {
   while ((vocab >> width) != 0) ++width;
   p.passes = (width + SORT_BITS - 1) / SORT_BITS;
   p.bits = (width + p.passes - 1) / p.passes;
-  p.self = n <= SORT_SELF;
   p.block = 32;
   while (p.block * p.block * 8 < n) p.block *= 2;
   p.blocks = (n + p.block - 1) / p.block;
   p.keys = up((size_t)n * 4);
-  p.counts = p.self ? 0 : up((size_t)p.tiles * SORT_BINS * 4);
+  p.counts = up((size_t)p.tiles * SORT_BINS * 4);
   p.part = up((size_t)p.blocks * 2 * d * 4);
   return p;
 }
@@ -460,14 +426,13 @@ int gmdn_embed_bwd(const void* dy, const int64_t* tokens, void* dweight, void* w
     b = (uint32_t*)at;
     at += p.keys;
   }
-  uint32_t* const counts = p.self ? nullptr : (uint32_t*)at;
+  uint32_t* const counts = (uint32_t*)at;
   float* const part = (float*)(at + p.counts);
   SortInput in{tokens, nullptr, nullptr, rows, vocab, padding_idx};
   int to = 0;
   for (int pass = 0; pass < p.passes && rows > 0; ++pass, to ^= 1) {
     const int shift = pass * p.bits;
-    if (counts)
-      hipLaunchKernelGGL(em_count, dim3((unsigned)p.tiles), dim3(SORT_THREADS), 0, st, in, counts, p.tile, shift, p.bits);
+    hipLaunchKernelGGL(em_count, dim3((unsigned)p.tiles), dim3(SORT_THREADS), 0, st, in, counts, p.tile, shift, p.bits);
     hipLaunchKernelGGL(em_scatter, dim3((unsigned)p.tiles), dim3(SORT_THREADS), 0, st, in, counts, buf[2 * to],
                        buf[2 * to + 1], p.tile, shift, p.bits);
     in.tokens = nullptr;
