@@ -2,7 +2,10 @@
 //
 //   y_i = s W[t_i],     dW[v] = s sum over the i with t_i = v of dy_i
 //
-// Memory bound both ways.  The forward copies rows.  The gradient is a sum by
+// Memory bound both ways where the table is large: 16384 tokens of 131072 x 4096 bf16 take
+// 55 us forward (4.9 TB/s) and their sums 229 us (5.2 TB/s, nine tenths of it zeros of the
+// table); for 32000 x 1024 the gradient is 25 us of sums beside 23 of the sort, on 16
+// workgroups, and 5 of the join.  The forward copies rows.  The gradient is a sum by
 // token in a fixed order, without atomics on values: the positions are sorted
 // by token (a stable radix sort, so equal tokens keep their order), blocks of
 // the sorted positions add the rows of dy they name, and a token whose run
@@ -342,7 +345,11 @@ void with_type(int32_t dtype, F&& f) {
 
 // How a gradient's work is cut.  A block adds its positions one after another
 // and a token's run of them is joined one after another, so the block grows with the
-// square root of the positions.
+// square root of the positions.  That is for batches where one token fills much of them:
+// 65536 of 32000 x 256, nine in ten a padding token, take 155 us in blocks of 128, 188 of 64,
+// 298 of 32; 16384 x 1024, half of them, 75 in blocks of 64, 85 of 32.  Without such a token
+// less is better by a little (16384: 62 in blocks of 64, 58 of 32; 65536: 109 of 128, 101 of
+// 64), and below 32 nothing is won from a few thousand tokens on.
 struct Plan {
   int64_t tile, tiles, block, blocks;
   int passes, bits;

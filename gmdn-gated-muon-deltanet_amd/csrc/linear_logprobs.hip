@@ -11,8 +11,14 @@
 // in registers and leaves of each row of a tile three sums; they are joined
 // by row afterwards.  The backward forms the logits again, a piece of the
 // vocabulary at a time, writes the piece's d in bfloat16 and takes both
-// products from it: four products in all, and of the logits never more than
-// PIECE_BYTES of memory.
+// products from it: four products in all, and of d no more than PIECE_BYTES of
+// memory, or 256 columns of all rows where those are more.
+//
+// 16384 x 32000 x 1024 bf16: the forward takes 974 us, 1.10 PFLOP/s, and the backward's three
+// products 2.77 ms, 1.16; the matrix units are busy for 52% of the forward's clocks, 44% of the
+// logits' again, 58% of dx's and 65% of dW's, and no LDS read has a bank conflict.  A tile of 256 reads and copies
+// its operands in as many clocks of LDS as its products take, and a tile of logits of k =
+// 1024 has only 16 stages beside its first copies and its epilogue.
 //
 // bfloat16 operands are multiplied as they are; d is rounded to bfloat16 as the
 // gradient of bfloat16 logits would be.  float32 operands, and d beside them, are
@@ -173,7 +179,8 @@ ll_join(const float* __restrict__ part, const float* __restrict__ at_token, cons
   stats[2 * row + 1] = w.logs;
 }
 // One row a workgroup while those are few: the tiles of a large vocabulary are read one
-// after another by each thread.
+// after another by each thread (forward, 16 x 131072 x 64: 16.5 us, 16 rows a workgroup 47;
+// 1024 x 32000 x 256: 33 and 32; 4096: 110 and 105).
 constexpr int64_t JOIN_FEW = 1024;
 
 // ------------------------------------------------------------------ backward
@@ -355,8 +362,10 @@ bool in_place(const void* p, int64_t stride, int64_t d, int32_t dtype) {
 struct Product {
   int edge, per, splits;
 };
-// A product of few tiles is split until the chip is filled, while a part keeps sixteen
-// turns of the loop or more: joining the parts is a launch more.
+// A product of few tiles is split until the chip is filled (dx of 8 x 32000 x 1024, backward:
+// 32 us, whole 179), while a part keeps sixteen turns of the loop or more: joining the
+// parts is a launch more (1024 x 8192 x 1024: 56 us, from four turns on 64; 16384 x 257 x 256,
+// dW: 32 and 41; but 512 x 257 x 256 float32, dW: 22 and 19).
 int splits_of(int64_t tiles, int64_t turns) {
   int64_t s = 256 / tiles;
   if (s > turns / 16) s = turns / 16;
@@ -365,7 +374,9 @@ int splits_of(int64_t tiles, int64_t turns) {
 // The tile of the least cost: rounds over the 256 CUs, times a tile's work at the rate that its
 // reads from LDS leave it, of two stages more than it has (its ramp and epilogue).  For a stage
 // of 32 k the matrix units take 1024, 256 and 64 clocks, LDS at 128 bytes a clock 1024,
-// 384 and 192: rates as 6 to 4 to 2.
+// 384 and 192: rates as 6 to 4 to 2.  It takes the fastest tile or one within 8% of it in
+// all that was measured (forward in tiles of 64, 128 and 256: 8 x 32000 x 1024 bf16: 16, 19
+// and 30 us; 1024 x 8192 x 1024: 35, 25 and 33; 16384 x 32000 x 1024: 1626, 1047 and 908).
 Product product_of(int64_t M, int64_t N, int64_t steps, int pairs, bool split) {
   Product best{};
   double least = 0;
